@@ -25,6 +25,7 @@
 #define PTL_API_H
 
 #include "ptl_structs.h"
+#include "ptl_transformer.h"
 
 #ifdef __cplusplus
 extern "C" {

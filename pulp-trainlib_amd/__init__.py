@@ -117,6 +117,12 @@ NORMED_ENTRY_POINTS = ["ptl_conv2d_%s_fw_batched_normed" % dt for dt in ("fp16",
 # `int f(const pool_args *, const Linear_args *, const loss_args *, int nsamples, ptl_wg_batch *)`
 HEAD_ENTRY_POINTS = ["ptl_pool_linear_loss_%s_batched" % dt for dt in ("fp16", "fp32")]
 
+# include/ptl_transformer.h: `int f(const args *, int nsamples)`, `int f(const args *)`, `int f(const args *, int nsamples, int step)`
+ROW_ENTRY_POINTS = ["ptl_%s_%s_%s_batched" % (n, dt, step) for n in ("rms_norm", "gated_linear") for dt in ("fp32", "fp16")
+                    for step in ("fw", "bw")]
+INT8_ENTRY_POINTS = ["ptl_mm_int8_fp32", "ptl_mm_int8_fp16"]
+DISTILL_ENTRY_POINTS = ["ptl_distill_fp32_batched", "ptl_distill_fp16_batched"]
+
 OTHER_ENTRY_POINTS = ["ptl_init", "ptl_last_error", "ptl_last_status", "ptl_set_stream", "ptl_sync", "ptl_set_gemm_path",
                       "ptl_last_conv_direct", "ptl_last_gemm_streamed", "ptl_last_conv_resident", "ptl_last_gemm_tile", "ptl_last_gemm_form", "ptl_staging_copies", "ptl_timer_begin", "ptl_timer_end_ms", "ptl_mm_fp32", "ptl_mm_fp16", "ptl_copy_bytes",
                       "ptl_reserve", "ptl_reserved", "ptl_probe_mfma_fp16"]
@@ -135,15 +141,15 @@ def load():
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p]
         f.restype = None
-    for name in BATCHED_ENTRY_POINTS:
+    for name in BATCHED_ENTRY_POINTS + ROW_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p, ctypes.c_int]
         f.restype = ctypes.c_int
-    for name in STEP_ENTRY_POINTS:
+    for name in STEP_ENTRY_POINTS + DISTILL_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int]
         f.restype = ctypes.c_int
-    for name in PLAIN_ENTRY_POINTS:
+    for name in PLAIN_ENTRY_POINTS + INT8_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p]
         f.restype = ctypes.c_int

@@ -1,0 +1,121 @@
+// Gated dense layers: y = act(x Wg^T) * (x Wu^T), forward and backward.
+#include "ptl_rows_mm.inc"
+#include "ptl_internal.h"
+
+namespace ptl {
+
+template <typename T>
+int rows_gated(RowsArgs &a) {
+    return rows_launch<T, T, true, 64, 64, 2, 2, 1, false, 2>(a);
+}
+
+// dh = (dy h_up act'(h_gate), dy act(h_gate)): three values read, two written, nothing else.  dh may be h.
+template <typename T>
+__global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__restrict__ dy, T *dh, size_t rows, int outs, int act) {
+    typedef RowPiece<T> Piece;
+    constexpr int VEC = Piece::VEC;
+    const int pieces = (outs + VEC - 1) / VEC, p = (int)(blockIdx.x * 256 + threadIdx.x);
+    if (p >= pieces) return;
+    for (size_t row = blockIdx.y; row < rows; row += gridDim.y) {
+        Piece g, u, d, og, ou;
+        g.load(h + row * 2 * outs, p, outs);
+        u.load(h + row * 2 * outs + outs, p, outs);
+        d.load(dy + row * outs, p, outs);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            float f;
+            const float df = gate_act_back((float)g.e[i], act, f);
+            og.e[i] = (T)((float)d.e[i] * (float)u.e[i] * df);
+            ou.e[i] = (T)((float)d.e[i] * f);
+        }
+        og.store(dh + row * 2 * outs, p, outs);
+        ou.store(dh + row * 2 * outs + outs, p, outs);
+    }
+}
+
+static int linear_bw(const ::Linear_args *l, int ns) { return ptl_linear_fp32_bw_batched(l, ns); }
+static int linear_bw(const ::Linear_args_fp16 *l, int ns) { return ptl_linear_fp16_bw_batched(l, ns); }
+
+template <typename T, typename Linear, typename Args>
+static int gated_step(const Args *a, int ns, bool back, const char *fn) {
+    if (!a || !a->input || !a->coeff || !a->output || (back && !a->hidden)) return rows_bad(fn, "null argument structure");
+    const int in = a->input->dim, outs = a->output->dim;
+    if (in <= 0 || outs <= 0 || in > (1 << 27) || outs >= ROW_MOST / 2) return rows_bad(fn, "invalid tensor geometry");
+    if (a->activation < PTL_GATE_SIGMOID || a->activation > PTL_GATE_RELU) return rows_bad(fn, "unknown activation");
+    const bool bias = a->use_biases == 1;
+    if (bias && !a->bias) return rows_bad(fn, "use_biases=1 with a null bias blob");
+    if (ns <= 0) return 0;
+    auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
+    const size_t nx = (size_t)ns * in, ny = (size_t)ns * outs, nw = (size_t)2 * outs * in;
+    if (!back) {
+        T *h = as(blob_data(a->hidden));
+        if (!a->input->data || !a->coeff->data || !a->output->data || (bias && !a->bias->data)) return rows_bad(fn, "null buffer");
+        if (!ensure_init()) return 2;
+        Stager sg;
+        RowsArgs r = {};
+        r.x = reinterpret_cast<const char *>(sg.in<T>(as(a->input->data), nx));
+        r.w = reinterpret_cast<const char *>(sg.in<T>(as(a->coeff->data), nw));
+        if (bias) r.bias = sg.in<T>(as(a->bias->data), (size_t)2 * outs);
+        r.y = sg.out<T>(as(a->output->data), ny);
+        if (h) r.hidden = sg.out<T>(h, 2 * ny);
+        if (sg.failed()) return 2;
+        r.row_b = in * (int)sizeof(T);
+        r.outs = outs;
+        r.tokens = ns;
+        r.act = a->activation;
+        r.zeros = static_cast<const char *>(state().zeros);
+        return sg.finish(rows_gated<T>(r));
+    }
+    const bool wg = !a->skip_wg_grad, ig = !a->skip_in_grad;
+    if (!a->hidden->data || !a->hidden->diff || !a->output->diff || (wg && (!a->input->data || !a->coeff->diff || (bias && !a->bias->diff))) ||
+        (ig && (!a->coeff->data || !a->input->diff)))
+        return rows_bad(fn, "null buffer");
+    if (nx > 0x7fffffffu || 2 * ny > 0x7fffffffu || nw > 0x7fffffffu) return rows_bad(fn, "tensor larger than 2^31 elements");
+    if (!ensure_init()) return 2;
+    ptl_internal_stage_begin();  // the gradients of the pre-activations are the products' input
+    int rc;
+    {
+        Stager sg;
+        const T *h = sg.in<T>(as(a->hidden->data), 2 * ny), *dy = sg.in<T>(as(a->output->diff), ny);
+        T *dh = sg.out<T>(as(a->hidden->diff), 2 * ny);
+        if (sg.failed()) {
+            rc = 2;
+        } else {
+            const int pieces = (outs + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC;
+            hipLaunchKernelGGL((gate_back_kernel<T>), dim3((pieces + 255) / 256, ns < 65535 ? ns : 65535), dim3(256), 0, state().stream, h, dy, dh,
+                               (size_t)ns, outs, a->activation);
+            rc = sg.finish(hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2);
+        }
+    }
+    if (rc == 0 && (wg || ig)) {
+        auto out = *a->hidden;  // a dense layer of 2 n_out outputs
+        out.dim = 2 * outs;
+        Linear l = {};
+        l.input = a->input;
+        l.coeff = a->coeff;
+        l.bias = a->bias;
+        l.output = &out;
+        l.skip_wg_grad = a->skip_wg_grad;
+        l.skip_in_grad = a->skip_in_grad;
+        l.use_biases = a->use_biases;
+        rc = linear_bw(&l, ns);
+    }
+    return ptl_internal_stage_end(rc);
+}
+
+}  // namespace ptl
+
+extern "C" {
+int ptl_gated_linear_fp32_fw_batched(const struct GatedLinear_args *a, int ns) {
+    return ptl::gated_step<float, ::Linear_args>(a, ns, false, "ptl_gated_linear_fp32_fw_batched");
+}
+int ptl_gated_linear_fp32_bw_batched(const struct GatedLinear_args *a, int ns) {
+    return ptl::gated_step<float, ::Linear_args>(a, ns, true, "ptl_gated_linear_fp32_bw_batched");
+}
+int ptl_gated_linear_fp16_fw_batched(const struct GatedLinear_args_fp16 *a, int ns) {
+    return ptl::gated_step<ptl::half_t, ::Linear_args_fp16>(a, ns, false, "ptl_gated_linear_fp16_fw_batched");
+}
+int ptl_gated_linear_fp16_bw_batched(const struct GatedLinear_args_fp16 *a, int ns) {
+    return ptl::gated_step<ptl::half_t, ::Linear_args_fp16>(a, ns, true, "ptl_gated_linear_fp16_bw_batched");
+}
+}

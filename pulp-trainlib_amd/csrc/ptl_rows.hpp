@@ -1,0 +1,115 @@
+// Rows of tensors in 16-byte pieces, and sums over the threads of a row: shared by the kernels that give a row to a wave or to
+// a workgroup.
+#pragma once
+#include <stdio.h>
+
+#include "ptl_common.hpp"
+#include "ptl_host.hpp"
+
+namespace ptl {
+
+typedef unsigned row_u4 __attribute__((ext_vector_type(4), aligned(1)));  // 16 bytes wherever they start
+typedef unsigned row_u2 __attribute__((ext_vector_type(2), aligned(1)));
+typedef unsigned row_u1 __attribute__((aligned(1)));
+
+template <typename T>
+struct RowPiece {
+    static constexpr int VEC = 16 / (int)sizeof(T);
+    union {
+        row_u4 raw;
+        T e[VEC];
+    };
+    // Piece p of a row of `dim` elements.  No load depends on where the row ends: a piece that reaches over the end is read so that
+    // it ends there, and trim() moves its values down and puts zeros behind them (only the waves that hold such a piece do).  All
+    // of a thread's pieces are fetched before the first is trimmed.
+    __device__ inline void fetch(const T *row, int p, int dim) {
+        if (dim >= VEC) {
+            raw = *reinterpret_cast<const row_u4 *>(row + min(p * VEC, dim - VEC));
+        } else {
+            raw = row_u4{0, 0, 0, 0};
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (p == 0 && i < dim) e[i] = row[i];
+        }
+    }
+    __device__ inline void trim(int p, int dim) {
+        if (dim < VEC) return;
+        const int cut = p * VEC - min(p * VEC, dim - VEC);
+        if (!__any(cut)) return;
+        unsigned long long lo = (unsigned long long)raw.y << 32 | raw.x, hi = (unsigned long long)raw.w << 32 | raw.z;
+        const unsigned bytes = (unsigned)min(cut, VEC) * (unsigned)sizeof(T), bits = (bytes & 7) * 8;
+        if (bytes >= 8) {
+            lo = hi;
+            hi = 0;
+        }
+        if (bytes == 16) lo = 0;
+        lo = lo >> bits | hi << 1 << (63 - bits);
+        hi >>= bits;
+        raw = row_u4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
+    }
+    __device__ inline void load(const T *row, int p, int dim) {
+        fetch(row, p, dim);
+        trim(p, dim);
+    }
+    __device__ inline void store(T *row, int p, int dim) const {
+        const int at = p * VEC;
+        if (at + VEC <= dim) {
+            *reinterpret_cast<row_u4 *>(row + at) = raw;
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i)
+                if (at + i < dim) row[at + i] = e[i];
+        }
+    }
+};
+
+constexpr int ROW_MOST = 1 << 30;  // elements of a row
+
+// Sums (and maxima) of N values over the 64 lanes of a wave, the same in every lane.
+__device__ inline float wave_sum(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v += __shfl_xor(v, off);
+    return v;
+}
+__device__ inline float wave_max(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
+    return v;
+}
+
+// ... over the TPR threads that have a row: one wave, or a workgroup (a float per wave and value in `lds`, which the caller
+// does not use again without a barrier).
+template <int TPR, int N, bool MAX1 = false>  // MAX1: the second value is a maximum
+__device__ inline void row_reduce(float (&v)[N], float (*lds)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = MAX1 && i == 1 ? wave_max(v[i]) : wave_sum(v[i]);
+    if constexpr (TPR > 64) {
+        const int wave = threadIdx.x >> 6;
+        if ((threadIdx.x & 63) == 0) {
+#pragma unroll
+            for (int i = 0; i < N; ++i) lds[wave][i] = v[i];
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+            float s = lds[0][i];
+#pragma unroll
+            for (int w = 1; w < TPR / 64; ++w) s = MAX1 && i == 1 ? fmaxf(s, lds[w][i]) : s + lds[w][i];
+            v[i] = s;
+        }
+    }
+}
+
+// A rejected call: its message, as the other entry points give it.
+inline int rows_bad(const char *fn, const char *what) {
+    printf("[%s] %s\n", fn, what);
+    set_error("%s: %s", fn, what);
+    return 1;
+}
+
+template <typename Blob>
+inline auto *blob_data(const Blob *b) { return b ? b->data : nullptr; }
+template <typename Blob>
+inline auto *blob_diff(const Blob *b) { return b ? b->diff : nullptr; }
+
+}  // namespace ptl

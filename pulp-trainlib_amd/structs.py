@@ -190,6 +190,29 @@ class NormFusion(C.Structure):
     _fields_ = [("relu", I), ("skip", P), ("skip_diff", P), ("diff2", P)]
 
 
+# include/ptl_transformer.h
+
+class RmsNormArgs(C.Structure):
+    _fields_ = [("input", BlobP), ("skip", BlobP), ("sum", BlobP), ("coeff", BlobP), ("output", BlobP), ("q_data", P),
+                ("q_scale", P), ("eps", C.c_float), ("skip_wg_grad", I), ("skip_in_grad", I)]
+
+
+class GatedLinearArgs(C.Structure):
+    _fields_ = [("input", BlobP), ("coeff", BlobP), ("bias", BlobP), ("hidden", BlobP), ("output", BlobP),
+                ("activation", I), ("skip_wg_grad", I), ("skip_in_grad", I), ("use_biases", I)]
+
+
+class MatMulInt8Args(C.Structure):
+    _fields_ = [("A", P), ("B", P), ("C", P), ("A_scale", P), ("B_scale", P), ("bias", P), ("N", I), ("M", I), ("K", I),
+                ("USE_BIASES", I)]
+
+
+class DistillArgs(C.Structure):
+    _fields_ = [("output", BlobP), ("teacher", P), ("classes", P), ("n_top", I), ("temperature", C.c_float),
+                ("weight", C.c_float), ("wr_loss", P)]
+
+
+GATE_SIGMOID, GATE_SILU, GATE_GELU, GATE_RELU = 0, 1, 2, 3
 LAYER_CONV2D, LAYER_DW_CONV, LAYER_PW_CONV, LAYER_LINEAR = 0, 1, 2, 3
 STEP_FW, STEP_WGT_GRAD, STEP_IN_GRAD = 0, 1, 2
 

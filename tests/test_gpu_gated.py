@@ -1,0 +1,198 @@
+"""Gated dense layers against their formula in 64 bits.  u = 2^-24; a sum of n products is at most n u of the sum of their
+magnitudes off, however it is formed."""
+import ctypes
+
+import pytest
+import torch
+
+import transformer as tr
+
+pytestmark = pytest.mark.gpu
+U = tr.U
+
+
+def inputs(seed, dt, n, n_in, n_out, bias):
+    x, w = tr.rand(seed, n, n_in, dt=dt), tr.rand(seed + 1, 2 * n_out, n_in, scale=1.5 / n_in ** 0.5, dt=dt)
+    return x, w, tr.rand(seed + 2, 2 * n_out, scale=0.3, dt=dt) if bias else None
+
+
+def forward(pkg, gpu, dt, act, x, w, b, keep=True):
+    n, n_in, n_out = x.shape[0], x.shape[1], w.shape[0] // 2
+    X, W, B = tr.dev(x), tr.dev(w), None if b is None else tr.dev(b)
+    y = torch.full((n + 1, n_out), 7, dtype=X.dtype, device="cuda")
+    h = torch.full((n + 1, 2 * n_out), 7, dtype=X.dtype, device="cuda") if keep else None
+    a, held = tr.gated_args(pkg, n_in, n_out, tr.ACTS[act], x=X, w=W, b=B, h=h, y=y)
+    pkg.call("ptl_gated_linear_%s_fw_batched" % dt, a, n)
+    assert gpu.ptl_sync() == 0
+    assert (y[n] == 7).all() and (h is None or (h[n] == 7).all())  # behind the last sample
+    return y[:n], None if h is None else h[:n]
+
+
+def check_forward(dt, act, x, w, b, y, h):
+    n_in, n_out = x.shape[1], w.shape[0] // 2
+    x, w = x.double(), w.double()
+    ref = x @ w.t() + (0 if b is None else b.double())
+    off = U * ((n_in + 2) * (x.abs() @ w.abs().t()) + 2 * ref.abs())
+    if h is not None:
+        tr.within(h, ref, off + tr.step(ref, dt), "h")
+    g, up, og, ou = ref[:, :n_out], ref[:, n_out:], off[:, :n_out], off[:, n_out:]
+    f, _ = tr.act64(g, act)
+    # slopes of the activations are at most 1.13
+    of = 1.13 * og + f.abs() * U * tr.act_steps(g, act)
+    tr.within(y, f * up, of * up.abs() + (f.abs() + of) * ou + (f * up).abs() * U * 2 + tr.step(f * up, dt), "y")
+
+
+SHAPES = [(1, 1, 1), (1, 5, 3), (2, 7, 16), (3, 64, 17), (5, 785, 33), (8, 128, 40), (9, 100, 31), (33, 64, 64), (64, 33, 96), (65, 129, 65),
+          (130, 200, 130), (257, 72, 150)]
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,n_in,n_out", SHAPES)
+def test_forward(pkg, gpu, dt, n, n_in, n_out):
+    for act, bias, keep in (("silu", 0, 1), ("gelu", 1, 0), ("relu", 1, 1), ("sigmoid", 0, 0)):
+        x, w, b = inputs(n + n_in, dt, n, n_in, n_out, bias)
+        check_forward(dt, act, x, w, b, *forward(pkg, gpu, dt, act, x, w, b, keep))
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,n_in,n_out", [(1, 4096, 700), (4, 2048, 1001), (12, 1024, 600), (391, 785, 333), (300, 1024, 512), (600, 512, 1000),
+                                          (1024, 256, 2112), (520, 1040, 2051)])
+def test_forward_larger(pkg, gpu, dt, n, n_in, n_out):
+    x, w, b = inputs(n, dt, n, n_in, n_out, n % 2)
+    check_forward(dt, "silu", x, w, b, *forward(pkg, gpu, dt, "silu", x, w, b))
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n", [1, 3, 70])
+def test_forward_values(pkg, gpu, dt, n):
+    """What is no number stays in its sample or its output, also next to the end of a row that ends inside a piece; far values of
+    the gate take their limits."""
+    n_in, n_out = 37, 20
+    x, w, _ = inputs(3, dt, n, n_in, n_out, 0)
+    w[4, 36], w[n_out + 7, 0] = float("nan"), float("inf")
+    y, h = forward(pkg, gpu, dt, "silu", x, w, None)
+    good = [i for i in range(n_out) if i not in (4, 7)]
+    assert torch.isnan(h[:, 4]).all() and not torch.isfinite(h[:, n_out + 7]).any() and torch.isfinite(h[:, good]).all()
+    assert torch.isnan(y[:, 4]).all() and torch.isfinite(y[:, good]).all()
+    # gates of +-1000 and 0
+    x = torch.zeros(n, 3, dtype=tr.t_dtype(dt))
+    x[:, 0], x[:, 1] = 1000, 1
+    w = torch.zeros(6, 3, dtype=tr.t_dtype(dt))
+    w[0, 0], w[1, 0] = 1, -1
+    w[3:, 1] = 2
+    for act, want in (("silu", (2000, 0, 0)), ("gelu", (2000, 0, 0)), ("sigmoid", (2, 0, 1)), ("relu", (2000, 0, 0))):
+        y, _ = forward(pkg, gpu, dt, act, x, w, None)
+        assert torch.equal(y.double().cpu(), torch.tensor([want], dtype=torch.float64).expand(n, 3)), act
+
+
+def backward(pkg, gpu, dt, act, x, w, h, dy, bias, **more):
+    n, n_in, n_out = x.shape[0], x.shape[1], w.shape[0] // 2
+    X, W, H, DY = (tr.dev(t) for t in (x, w, h, dy))
+    dx, dw, dh = torch.full_like(X, 7), torch.full_like(W, 7), H if more.pop("over", 0) else torch.full_like(H, 7)
+    db = torch.full((2 * n_out,), 7, dtype=X.dtype, device="cuda") if bias else None
+    a, keep = tr.gated_args(pkg, n_in, n_out, tr.ACTS[act], x=X, dx=dx, w=W, dw=dw, db=db, h=H, dh=dh, dy=DY, **more)
+    pkg.call("ptl_gated_linear_%s_bw_batched" % dt, a, n)
+    assert gpu.ptl_sync() == 0
+    return dh, dx, dw, db
+
+
+def check_backward(dt, act, x, w, h, dy, dh, dx, dw, db):
+    n, n_out = x.shape[0], w.shape[0] // 2
+    g, up, d = h[:, :n_out].double(), h[:, n_out:].double(), dy.double()
+    f, df = tr.act64(g, act)
+    ref = torch.cat([d * up * df, d * f], 1)
+    # the slope is a sum of two terms: act / g (gate 1: its limit) and the rest
+    first = torch.where(g != 0, f / g, torch.ones_like(g)).abs() if act in ("silu", "gelu") else torch.zeros_like(g)
+    slope = U * (tr.act_steps(g, act) + 8) * (2 * first + df.abs())
+    tol = torch.cat([(d * up).abs() * slope, (d * f).abs() * U * (tr.act_steps(g, act) + 2)], 1)
+    tr.within(dh, ref, tol + tr.step(ref, dt), "dh")
+    got = dh.double().cpu()  # what the products read
+    x, w = x.double(), w.double()
+    if dx is not None:
+        ref = got @ w
+        tr.within(dx, ref, U * (2 * n_out + 4) * (got.abs() @ w.abs()) + tr.step(ref, dt), "dx")
+    if dw is not None:
+        ref = got.t() @ x
+        tr.within(dw, ref, U * (n + 4) * (got.abs().t() @ x.abs()) + tr.step(ref, dt), "dw")
+    if db is not None:
+        ref = got.sum(0)
+        tr.within(db, ref, U * (n + 4) * got.abs().sum(0) + tr.step(ref, dt), "db")
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,n_in,n_out", SHAPES + [(391, 785, 333), (512, 1024, 704)])
+def test_backward(pkg, gpu, dt, n, n_in, n_out):
+    for act, bias in (("silu", 0), ("gelu", 1), ("relu", 0), ("sigmoid", 1)):
+        x, w, _ = inputs(n, dt, n, n_in, n_out, 0)
+        h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt=dt), tr.rand(n + 6, n, n_out, scale=0.5, dt=dt)
+        check_backward(dt, act, x, w, h, dy, *backward(pkg, gpu, dt, act, x, w, h, dy, bias))
+
+
+def test_backward_skips_and_in_place(pkg, gpu):
+    n, n_in, n_out = 20, 50, 30
+    x, w, _ = inputs(1, "fp32", n, n_in, n_out, 0)
+    h, dy = tr.rand(5, n, 2 * n_out), tr.rand(6, n, n_out)
+    full = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, 1)
+    dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, 1, over=1)
+    assert all(torch.equal(a, b) for a, b in zip(full, (dh, dx, dw, db)))
+    dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, 1, skip_wg=1)
+    assert torch.equal(dh, full[0]) and (dw == 7).all() and (db == 7).all()
+    check_backward("fp32", "silu", x, w, h, dy, dh, dx, None, None)
+    dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, 1, skip_ig=1)
+    assert torch.equal(dh, full[0]) and (dx == 7).all()
+    check_backward("fp32", "silu", x, w, h, dy, dh, None, dw, db)
+    dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, 1, skip_ig=1, skip_wg=1)
+    assert torch.equal(dh, full[0]) and (dx == 7).all() and (dw == 7).all()
+
+
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+def test_backward_far_gates(pkg, gpu, act):
+    """Gates far from 0, where the slope is 0 or 1 and squares overflow."""
+    g = torch.tensor([-3e38, -1e20, -2e4, -90.0, -20.0, 0.0, 20.0, 90.0, 2e4, 1e20, 3e38])
+    n_out = g.numel()
+    h, dy = torch.cat([g, torch.ones(n_out)])[None], torch.full((1, n_out), 0.5)
+    x, w = torch.ones(1, 2), torch.zeros(2 * n_out, 2)
+    dh = backward(pkg, gpu, "fp32", act, x, w, h, dy, 0)[0].double().cpu()
+    f, df = tr.act64(g.double(), act)
+    df = torch.where(g.abs() >= 90, (g > 0).double() * (0 if act == "sigmoid" else 1), df)
+    want = torch.cat([0.5 * df, 0.5 * f])[None]
+    assert torch.allclose(dh, want, rtol=1e-5, atol=1e-7), (dh, want)
+
+
+def test_gradients_against_differences(pkg, gpu):
+    n, n_in, n_out, h = 2, 5, 4, 1e-5
+    x, w, b = inputs(7, "fp32", n, n_in, n_out, 1)
+    dy = tr.rand(8, n, n_out)
+    for act in ("silu", "gelu", "sigmoid"):
+        _, hidden = forward(pkg, gpu, "fp32", act, x, w, b)
+        _, dx, dw, db = backward(pkg, gpu, "fp32", act, x, w, hidden.cpu(), dy, 1)
+
+        def f(x_, w_, b_):
+            p = x_ @ w_.t() + b_
+            return (tr.act64(p[:, :n_out], act)[0] * p[:, n_out:] * dy.double()).sum()
+
+        at = [x.double(), w.double(), b.double()]
+        for k, got in enumerate((dx, dw, db)):
+            for i in range(got.numel()):
+                e = [torch.zeros_like(t) for t in at]
+                e[k].view(-1)[i] = h
+                up, down = (f(*(t + s * d for t, d in zip(at, e))) for s in (1, -1))
+                assert abs((up - down) / (2 * h) - float(got.view(-1)[i])) < 1e-5
+
+
+def test_host_arrays(pkg, gpu):
+    n, n_in, n_out = 5, 33, 12
+    x, w, b = inputs(9, "fp16", n, n_in, n_out, 1)
+    dy = tr.rand(10, n, n_out, dt="fp16")
+    y, h = forward(pkg, gpu, "fp16", "silu", x, w, b)
+    z = lambda *s: torch.zeros(*s, dtype=torch.float16).numpy()  # noqa: E731
+    hy, hh = z(n, n_out), z(n, 2 * n_out)
+    a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=x.numpy(), w=w.numpy(), b=b.numpy(), h=hh, y=hy)
+    pkg.call("ptl_gated_linear_fp16_fw_batched", a, n)
+    assert torch.equal(torch.from_numpy(hy), y.cpu()) and torch.equal(torch.from_numpy(hh), h.cpu())
+    want = backward(pkg, gpu, "fp16", "silu", x, w, h.cpu(), dy, 1)
+    dh, dx, dw, db = z(n, 2 * n_out), z(n, n_in), z(2 * n_out, n_in), z(2 * n_out)
+    a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=x.numpy(), dx=dx, w=w.numpy(), dw=dw, db=db, h=hh, dh=dh, dy=dy.numpy())
+    pkg.call("ptl_gated_linear_fp16_bw_batched", a, n)
+    for got, ref in zip((dh, dx, dw, db), want):
+        assert torch.equal(torch.from_numpy(got), ref.cpu())
