@@ -6,7 +6,7 @@ namespace ptl {
 
 template <typename T>
 int rows_gated(RowsArgs &a) {
-    return rows_launch<T, T, true, 64, 64, 2, 2, 1, false, 2>(a);
+    return rows_product<T, T, true>(a);
 }
 
 // dh = (dy h_up act'(h_gate), dy act(h_gate)): three values read, two written, nothing else.  dh may be h.
@@ -16,6 +16,7 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
     constexpr int VEC = Piece::VEC;
     const int pieces = (outs + VEC - 1) / VEC, p = (int)(blockIdx.x * 256 + threadIdx.x);
     if (p >= pieces) return;
+    const Gate gate(act);
     for (size_t row = blockIdx.y; row < rows; row += gridDim.y) {
         Piece g, u, d, og, ou;
         g.load(h + row * 2 * outs, p, outs);
@@ -24,7 +25,7 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             float f;
-            const float df = gate_act_back((float)g.e[i], act, f);
+            const float df = gate.back((float)g.e[i], f);
             og.e[i] = (T)((float)d.e[i] * (float)u.e[i] * df);
             ou.e[i] = (T)((float)d.e[i] * f);
         }

@@ -6,7 +6,7 @@ namespace ptl {
 
 template <typename OUT>
 int rows_int8(RowsArgs &a) {
-    return rows_launch<int8_t, OUT, false, 64, 64, 2, 2, 1, false, 2>(a);
+    return rows_product<int8_t, OUT, false>(a);
 }
 
 template <typename OUT, typename Args>

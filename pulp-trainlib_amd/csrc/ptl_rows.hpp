@@ -3,6 +3,8 @@
 #pragma once
 #include <stdio.h>
 
+#include <type_traits>
+
 #include "ptl_common.hpp"
 #include "ptl_host.hpp"
 
@@ -26,10 +28,16 @@ struct RowPiece {
         if (dim >= VEC) {
             raw = *reinterpret_cast<const row_u4 *>(row + min(p * VEC, dim - VEC));
         } else {
-            raw = row_u4{0, 0, 0, 0};
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (p == 0 && i < dim) e[i] = row[i];
+            // (rows shorter than a piece: value by value, the last one first)
+            typedef typename std::conditional<sizeof(T) == 4, unsigned, typename std::conditional<sizeof(T) == 2, unsigned short, unsigned char>::type>::type Bits;
+            constexpr int B = 8 * (int)sizeof(T);
+            unsigned long long lo = 0, hi = 0;
+#pragma nounroll
+            for (int i = p == 0 ? dim - 1 : -1; i >= 0; --i) {
+                hi = hi << B | lo >> (64 - B);
+                lo = lo << B | __builtin_bit_cast(Bits, row[i]);
+            }
+            raw = row_u4{(unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32)};
         }
     }
     __device__ inline void trim(int p, int dim) {

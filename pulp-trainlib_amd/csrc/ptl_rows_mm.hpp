@@ -20,42 +20,43 @@ struct RowsArgs {
     int tiles_w, tiles_t;
 };
 
-// The activation of a gated layer and its derivative.  e = exp(-|v|) is at most 1: nothing overflows, and 1 - s keeps the bits of
-// small values.
-__device__ inline float gate_sigmoid(float v, float &rest) {  // rest = 1 - sigmoid
-    const float e = expf(-fabsf(v)), r = 1.f / (1.f + e), s = e * r;
-    rest = v < 0.f ? r : s;
-    return v < 0.f ? s : r;
-}
-constexpr float GATE_C = 0.7978845608028654f, GATE_C3 = 0.044715f;  // sqrt(2 / pi)
-__device__ inline float gate_act(float g, int act) {
-    float rest;
-    if (act == GATE_RELU) return g > 0.f ? g : (g != g ? g : 0.f);
-    if (act == GATE_SIGMOID) return gate_sigmoid(g, rest);
-    if (act == GATE_SILU) return g * gate_sigmoid(g, rest);
-    return g * gate_sigmoid(2.f * GATE_C * g * fmaf(GATE_C3 * g, g, 1.f), rest);  // (1 + tanh(u)) / 2 = sigmoid(2 u)
-}
-__device__ inline float gate_act_back(float g, int act, float &f) {  // f: the activation itself
-    float rest, s;
-    if (act == GATE_RELU) {
-        f = g > 0.f ? g : (g != g ? g : 0.f);
-        return g > 0.f ? 1.f : (g != g ? g : 0.f);
+// The activations of a gated layer, all but the last as m sigmoid(p): silu m = p = x, sigmoid m = 1, p = x, and gelu m = x,
+// p = 2 sqrt(2 / pi) (x + 0.044715 x^3), since (1 + tanh(u)) / 2 = sigmoid(2 u).  Which one it is decides uniform constants and
+// selects, not branches: a tile has 32768 outputs a compute unit, at expf(), a division and a branch each 10 us of 200 (4096 tokens,
+// 2048 -> 5632 in fp16), this way 2.
+struct Gate {
+    float k1, k3;  // p = x (k1 + k3 x^2)
+    bool one, relu;
+    __device__ inline Gate(int act) {
+        const bool gelu = act == GATE_GELU;
+        k1 = gelu ? 1.5957691216057308f : 1.f;
+        k3 = gelu ? 0.07135481627260025f : 0.f;  // 0.044715 k1
+        one = act == GATE_SIGMOID;
+        relu = act == GATE_RELU;
     }
-    if (act == GATE_SIGMOID) {
-        f = s = gate_sigmoid(g, rest);
-        return s * rest;
+    // sigmoid(p) and 1 - sigmoid(p): exp(-|p|) is at most 1, nothing overflows and small values keep their bits.  log2(e) is the sum of
+    // two floats, so that the exponent is formed to 2^-24 of itself.
+    __device__ static inline float sigmoid(float p, float &rest) {
+        const float n = -fabsf(p), e = __builtin_amdgcn_exp2f(fmaf(n, 1.44269502f, n * 1.92596299e-8f));
+        const float r = __builtin_amdgcn_rcpf(1.f + e), s = e * r;
+        rest = p < 0.f ? r : s;
+        return p < 0.f ? s : r;
     }
-    if (act == GATE_SILU) {
-        s = gate_sigmoid(g, rest);
-        f = g * s;
-        return s + f * rest;
+    __device__ inline float act(float x) const {
+        float rest;
+        const float s = sigmoid(x * fmaf(k3 * x, x, k1), rest), f = (one ? 1.f : x) * s;
+        return relu ? (x < 0.f ? 0.f : x) : f;
     }
-    s = gate_sigmoid(2.f * GATE_C * g * fmaf(GATE_C3 * g, g, 1.f), rest);
-    f = g * s;
-    // (far from 0 the slope of s is 0, whatever the square of g grows to)
-    const float slope = s * rest;
-    return slope > 0.f ? s + g * slope * 2.f * GATE_C * fmaf(3.f * GATE_C3 * g, g, 1.f) : (g != g ? g : s);
-}
+    // The derivative; f: the activation itself.
+    __device__ inline float back(float x, float &f) const {
+        float rest;
+        const float s = sigmoid(x * fmaf(k3 * x, x, k1), rest), slope = s * rest;  // of sigmoid, to p
+        f = relu ? (x < 0.f ? 0.f : x) : (one ? 1.f : x) * s;
+        // d p / d x = k1 + 3 k3 x^2; far from 0 the slope is 0, whatever that grows to
+        const float d = slope > 0.f ? slope * (one ? 1.f : x * fmaf(3.f * k3 * x, x, k1)) : (x != x ? x : 0.f);
+        return relu ? (x > 0.f ? 1.f : x != x ? x : 0.f) : one ? d : s + d;
+    }
+};
 
 // 0: launched, 2: HIP error.
 template <typename T>
