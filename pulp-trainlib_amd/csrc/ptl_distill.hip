@@ -14,6 +14,13 @@ namespace ptl {
 
 constexpr int DISTILL_TOP = 2048;  // entries of a row at most: they are kept in LDS
 
+struct DistillEntry {
+    int to;         // the class, -1 where the entry is left out or another one before names the same class
+    float sum;      // of the probabilities of all entries that name it
+    float zc;       // the student's logit of the class, which the second launch may not read any more (grad may be z)
+    float p, log_p;
+    float pad[3];
+};
 template <typename T>
 struct DistillArgs {
     const T *z, *u;
@@ -21,98 +28,145 @@ struct DistillArgs {
     T *grad;      // (NULL: not wanted)
     float *loss;  // (NULL: not wanted)
     float2 *part;  // of each part of a row: its largest logit, the sum of exponentials relative to that
-    float *zc;     // the student's logits of a row's entries, which the second launch may not read any more (grad may be z)
+    struct DistillEntry *entry;  // of each row, behind those: what the first launch finds out about the teacher's entries
     int dim, top, parts, per_part;  // per_part: pieces
     float inv_t, hi, lo;  // 1 / T; log2(e) / T as the sum of two floats above 0
     float weight, scale;  // scale = weight / T
 };
 
-// exp((z - m) / T): the exponent is formed to 2^-24 of itself, where a product with a rounded constant would be off twice as far.
+// exp((z - m) / T).  fp32: the exponent is formed to 2^-24 of itself, where a product with a rounded constant would be off twice
+// as far.  fp16: one fused multiply-add on the value as it was read; its error, 2^-24 of m / T, is far below a step of the output,
+// and the walks over a row are bound by their instructions (2048 rows of 32000: 75 us with the other form, 61 so).
+template <typename T>
+struct DistillExp {
+    float m, hi, lo;
+    __device__ inline DistillExp(float max, const DistillArgs<T> &a) {
+        if constexpr (sizeof(T) == 4) {
+            m = max;
+            hi = a.hi;
+            lo = a.lo;
+        } else {
+            hi = a.hi;
+            m = -max * a.hi;  // (an infinite maximum gives NaN in every class, as z - m does)
+            lo = 0.f;
+        }
+    }
+    __device__ inline float operator()(T z) const {
+        if constexpr (sizeof(T) == 4) {
+            const float d = z - m;
+            return __builtin_amdgcn_exp2f(fmaf(d, hi, d * lo));
+        } else {
+            return __builtin_amdgcn_exp2f(fmaf((float)z, hi, m));
+        }
+    }
+};
 template <typename T>
 __device__ inline float distill_exp(float z, float m, const DistillArgs<T> &a) {
     const float d = z - m;
     return __builtin_amdgcn_exp2f(fmaf(d, a.hi, d * a.lo));
 }
 
-// Over a workgroup of NT threads.  `lds` holds a float per wave and is not written again before another barrier.
+// Two values over a workgroup of NT threads.  `lds` holds two floats per wave and is not written again before another barrier.
 template <int NT, bool MAX>
-__device__ inline float group_reduce(float v, float *lds) {
-    v = MAX ? wave_max(v) : wave_sum(v);
-    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
-    __syncthreads();
-    float r = lds[0];
+__device__ inline void group_reduce(float (&v)[2], float *lds) {
 #pragma unroll
-    for (int w = 1; w < NT / 64; ++w) r = MAX ? fmaxf(r, lds[w]) : r + lds[w];
-    return r;
+    for (int i = 0; i < 2; ++i) v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
+    if ((threadIdx.x & 63) == 0) *reinterpret_cast<float2 *>(lds + 2 * (threadIdx.x >> 6)) = make_float2(v[0], v[1]);
+    __syncthreads();
+    const float2 r = *reinterpret_cast<const float2 *>(lds + 2 * (threadIdx.x & (NT / 64 - 1)));
+    v[0] = r.x;
+    v[1] = r.y;
+#pragma unroll
+    for (int off = NT / 128; off > 0; off >>= 1)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const float o = __shfl_xor(v[i], off);
+            v[i] = MAX ? fmaxf(v[i], o) : v[i] + o;
+        }
 }
 
-// In LDS: 6 x 16 floats for the sums, then `top` each of classes, logits of the teacher (later probabilities) and of the
-// student (later gradients).
+// In LDS: room for three reductions, then `top` (in whole fours) each of classes, logits of the teacher (later probabilities) and
+// of the student (later gradients).
 constexpr int DISTILL_RED = 96;
-constexpr size_t distill_lds(int top) { return sizeof(float) * (DISTILL_RED + 3 * (size_t)top); }
+inline int distill_room(int top) { return (top + 3) & ~3; }
+inline size_t distill_lds(int top) { return sizeof(float) * (DISTILL_RED + 5 * (size_t)distill_room(top)); }
 struct DistillTop {
     float *red;
     int *at;
-    float *p, *zc;
-    __device__ inline DistillTop(float *lds, int top) : red(lds), at((int *)(lds + DISTILL_RED)), p(lds + DISTILL_RED + top), zc(p + top) {}
+    float *p, *zc, *sum;
+    int *to;
+    __device__ inline DistillTop(float *lds, int top) : red(lds), at((int *)(lds + DISTILL_RED)) {
+        const int room = (top + 3) & ~3;
+        p = lds + DISTILL_RED + room;
+        zc = p + room;
+        sum = zc + room;
+        to = at + 4 * room;
+    }
 };
 
-// The row's entries; a class that is left out becomes -1.  No barrier: a thread reads what it wrote itself.
+// The row's entries; a class that is left out becomes -1.  No barrier: a thread reads what it wrote itself.  Returns the largest
+// logit of the teacher that the thread has.
 template <typename T, int NT>
-__device__ inline void distill_fetch(const DistillArgs<T> &a, size_t row, const DistillTop &t) {
+__device__ inline float distill_fetch(const DistillArgs<T> &a, size_t row, const DistillTop &t) {
+    float m = -__builtin_inff();
     for (int i = threadIdx.x; i < a.top; i += NT) {
         const int c = a.at[row * a.top + i];
         const bool in = (unsigned)c < (unsigned)a.dim;
+        const float u = in ? (float)a.u[row * a.top + i] : -__builtin_inff();
         t.at[i] = in ? c : -1;
-        t.p[i] = in ? (float)a.u[row * a.top + i] : -__builtin_inff();
-        t.zc[i] = !in ? 0.f : a.zc ? a.zc[row * a.top + i] : (float)a.z[row * a.dim + c];
+        t.p[i] = u;
+        t.zc[i] = in ? (float)a.z[row * a.dim + c] : 0.f;
+        m = fmaxf(m, u);
     }
+    if (threadIdx.x < 4 && a.top + threadIdx.x < (((unsigned)a.top + 3) & ~3u)) {
+        t.at[a.top + threadIdx.x] = -1;
+        t.p[a.top + threadIdx.x] = 0.f;
+    }
+    return m;
+}
+// ... and the thread's sum of exp((u - um) / T); um is the teacher's largest, 0 where it has none (the sum is then 0, or NaN with one).
+template <typename T, int NT>
+__device__ inline float distill_total(const DistillArgs<T> &a, const DistillTop &t, float &um) {
+    if (um == -__builtin_inff()) um = 0.f;
+    float s = 0.f;
+    for (int i = threadIdx.x; i < a.top; i += NT) s += distill_exp(t.p[i], um, a);
+    return s;
 }
 
-// Loss of a row, and gradients of its entries' classes (into t.zc; t.at becomes -1 where another entry before names the same
-// class).  m, sum: of the student.  Returns whether the row has entries.  Barriers: every thread of the workgroup comes here.
-template <typename T, int NT>
-__device__ inline bool distill_entries(const DistillArgs<T> &a, size_t row, const DistillTop &t, float m, float sum, bool loss) {
-    const int tid = threadIdx.x;
-    float um = -__builtin_inff(), total = 0.f;
-    for (int i = tid; i < a.top; i += NT) um = fmaxf(um, t.p[i]);
-    um = group_reduce<NT, true>(um, t.red + 32);
-    if (um == -__builtin_inff()) um = 0.f;  // no entry, or all of them -inf: the sum is 0 (a NaN among them makes it NaN)
-    for (int i = tid; i < a.top; i += NT) total += distill_exp(t.p[i], um, a);
-    total = group_reduce<NT, false>(total, t.red + 48);
-    const bool some = total != 0.f;
-    const float inv_total = some ? 1.f / total : 0.f, inv_sum = 1.f / sum;
-    const float log_total = some ? logf(total) : 0.f, log_sum = logf(sum);
-    float terms = 0.f;
-    for (int i = tid; i < a.top; i += NT) {
-        const float p = distill_exp(t.p[i], um, a) * inv_total;
-        if (p != 0.f) terms += p * ((t.p[i] - um) * a.inv_t - log_total - ((t.zc[i] - m) * a.inv_t - log_sum));  // 0 log 0 = 0
+// Probabilities in the place of the logits; f(i, p, u - um) for each of the thread's.
+template <typename T, int NT, typename F>
+__device__ inline void distill_probabilities(const DistillArgs<T> &a, const DistillTop &t, float um, float total, F f) {
+    const float inv_total = total != 0.f ? 1.f / total : 0.f;
+    for (int i = threadIdx.x; i < a.top; i += NT) {
+        const float u = t.p[i], p = distill_exp(u, um, a) * inv_total;
+        f(i, p, u - um);
         t.p[i] = p;
     }
-    if (loss) {
-        terms = group_reduce<NT, false>(terms, t.red + 64);
-        if (tid == 0) a.loss[row] = terms * a.weight;
-    }
-    if (!a.grad) return some;
+}
+// Sums of the probabilities of entries that name one class, and which of them is the first.
+template <typename T, int NT>
+__device__ inline void distill_merge(const DistillArgs<T> &a, const DistillTop &t) {
     __syncthreads();  // all probabilities and classes are in LDS
-    int keep[(DISTILL_TOP + NT - 1) / NT];
-    int n = 0;
-    for (int i = tid; i < a.top; i += NT, ++n) {
+    for (int i = threadIdx.x; i < a.top; i += NT) {
         const int c = t.at[i];
         int first = c;
         float p = 0.f;
-        for (int k = 0; k < a.top; ++k) {  // (the same k in all threads: one read of LDS serves them all)
-            const bool same = t.at[k] == c;
-            p += same ? t.p[k] : 0.f;
-            if (same && k < i) first = -1;
+#pragma unroll 4
+        for (int k = 0; k < a.top; k += 4) {  // (the same k in all threads: one read of LDS serves them all)
+            const int4 o = *reinterpret_cast<const int4 *>(t.at + k);
+            const float4 q = *reinterpret_cast<const float4 *>(t.p + k);
+            p += (o.x == c ? q.x : 0.f) + (o.y == c ? q.y : 0.f) + ((o.z == c ? q.z : 0.f) + (o.w == c ? q.w : 0.f));
+            const int before = (o.x == c && k < i) | (o.y == c && k + 1 < i) | (o.z == c && k + 2 < i) | (o.w == c && k + 3 < i);
+            first = before ? -1 : first;
         }
-        t.zc[i] = some ? a.scale * (distill_exp(t.zc[i], m, a) * inv_sum - p) : 0.f;
-        keep[n] = first;
+        t.to[i] = first;
+        t.sum[i] = p;
     }
-    __syncthreads();
-    n = 0;
-    for (int i = tid; i < a.top; i += NT, ++n) t.at[i] = keep[n];
-    return some;
+}
+// One term of the loss: 0 log 0 = 0.
+template <typename T>
+__device__ inline float distill_term(float p, float log_p, float zc, float m, float log_sum, const DistillArgs<T> &a) {
+    return p != 0.f ? p * (log_p - ((zc - m) * a.inv_t - log_sum)) : 0.f;
 }
 
 // NP pieces of logits in each of NT threads, from piece `first` on; what the row does not have is -inf.
@@ -139,44 +193,52 @@ __device__ inline void distill_as_read(RowPiece<T> (&z)[NP]) {
 }
 template <typename T, int NP>
 __device__ inline float distill_max(const RowPiece<T> (&z)[NP]) {
-    float m = -__builtin_inff();
+    if constexpr (sizeof(T) == 2) {  // (two at a time)
+        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+        h2 m = {(T)-__builtin_inff(), (T)-__builtin_inff()};
 #pragma unroll
-    for (int j = 0; j < NP; ++j)
+        for (int j = 0; j < NP; ++j) {
+            const unsigned w[4] = {z[j].raw.x, z[j].raw.y, z[j].raw.z, z[j].raw.w};
 #pragma unroll
-        for (int i = 0; i < RowPiece<T>::VEC; ++i) m = fmaxf(m, (float)z[j].e[i]);
-    return m;
+            for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(h2, w[i]));
+        }
+        return fmaxf((float)m.x, (float)m.y);
+    } else {
+        float m = -__builtin_inff();
+#pragma unroll
+        for (int j = 0; j < NP; ++j)
+#pragma unroll
+            for (int i = 0; i < RowPiece<T>::VEC; ++i) m = fmaxf(m, (float)z[j].e[i]);
+        return m;
+    }
 }
 template <typename T, int NP>
-__device__ inline float distill_sum(const RowPiece<T> (&z)[NP], float m, const DistillArgs<T> &a) {
+__device__ inline float distill_sum(const RowPiece<T> (&z)[NP], const DistillExp<T> &e) {
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NP; ++j)
 #pragma unroll
-        for (int i = 0; i < RowPiece<T>::VEC; ++i) s += distill_exp((float)z[j].e[i], m, a);
+        for (int i = 0; i < RowPiece<T>::VEC; ++i) s += e(z[j].e[i]);
     return s;
 }
 // The gradient of the classes that are held.
 template <typename T, int NT, int NP>
-__device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, float m, float f, bool some, const DistillArgs<T> &a) {
+__device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const DistillExp<T> &e, float f, bool some, int dim) {
+    int mine = first + (int)threadIdx.x;
+    asm volatile("" : "+v"(mine));  // (the loads' addresses are not kept for the stores)
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int p = first + j * NT + (int)threadIdx.x;
+        const int p = mine + j * NT;
         RowPiece<T> o;
+        if (some) {
 #pragma unroll
-        for (int i = 0; i < RowPiece<T>::VEC; ++i) o.e[i] = some ? (T)(distill_exp((float)z[j].e[i], m, a) * f) : (T)0.f;
-        if (p < end) o.store(row, p, a.dim);
+            for (int i = 0; i < RowPiece<T>::VEC; ++i) o.e[i] = (T)(e(z[j].e[i]) * f);
+        } else {
+            o.raw = row_u4{0, 0, 0, 0};
+        }
+        if (p < end) o.store(row, p, dim);
     }
 }
-// ... and, behind all of those, of the entries' classes among them.
-template <typename T, int NT>
-__device__ inline void distill_put_entries(const DistillArgs<T> &a, size_t row, const DistillTop &t, int lo, int hi) {
-    __syncthreads();
-    for (int i = threadIdx.x; i < a.top; i += NT) {
-        const int c = t.at[i];
-        if (c >= lo && c < hi) a.grad[row * a.dim + c] = (T)t.zc[i];
-    }
-}
-
 // A row to a workgroup.  NP = 0: it is read three times.
 template <typename T, int NT, int NP>
 __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a) {
@@ -188,87 +250,137 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a)
     const T *zr = a.z + row * a.dim;
     T *gr = a.grad + row * a.dim;
     RowPiece<T> z[HELD];
-    float m, s = 0.f;
+    float top[2], sum[2] = {0.f, 0.f};  // of the student, of the teacher
     if constexpr (NP > 0) {
         distill_hold<T, NT>(z, zr, 0, pieces, a.dim);
-        distill_fetch<T, NT>(a, row, t);
-        m = group_reduce<NT, true>(distill_max<T>(z), t.red);
-        distill_as_read<T>(z);
-        s = group_reduce<NT, false>(distill_sum<T>(z, m, a), t.red + 16);
-        distill_as_read<T>(z);
+        top[1] = distill_fetch<T, NT>(a, row, t);
+        top[0] = distill_max<T>(z);
     } else {
-        distill_fetch<T, NT>(a, row, t);
-        m = -__builtin_inff();
+        top[1] = distill_fetch<T, NT>(a, row, t);
+        top[0] = -__builtin_inff();
         for (int p = 0; p < pieces; p += NT * HELD) {
             distill_hold<T, NT>(z, zr, p, pieces, a.dim);
-            m = fmaxf(m, distill_max<T>(z));
+            top[0] = fmaxf(top[0], distill_max<T>(z));
         }
-        m = group_reduce<NT, true>(m, t.red);
-        for (int p = 0; p < pieces; p += NT * HELD) {
-            distill_hold<T, NT>(z, zr, p, pieces, a.dim);
-            s += distill_sum<T>(z, m, a);
-        }
-        s = group_reduce<NT, false>(s, t.red + 16);
     }
-    const bool some = distill_entries<T, NT>(a, row, t, m, s, a.loss != nullptr);
-    if (!a.grad) return;
-    const float f = a.scale / s;
+    group_reduce<NT, true>(top, t.red);
+    const DistillExp<T> e(top[0], a);
     if constexpr (NP > 0) {
-        distill_put<T, NT>(z, gr, 0, pieces, m, f, some, a);
+        distill_as_read<T>(z);
+        sum[0] = distill_sum<T>(z, e);
+        distill_as_read<T>(z);
     } else {
         for (int p = 0; p < pieces; p += NT * HELD) {
             distill_hold<T, NT>(z, zr, p, pieces, a.dim);
-            distill_put<T, NT>(z, gr, p, pieces, m, f, some, a);
+            sum[0] += distill_sum<T>(z, e);
         }
     }
-    distill_put_entries<T, NT>(a, row, t, 0, a.dim);
+    sum[1] = distill_total<T, NT>(a, t, top[1]);
+    group_reduce<NT, false>(sum, t.red + 32);
+    const bool some = sum[1] != 0.f;  // (no entry, or all of them -inf)
+    float terms[2] = {0.f, 0.f};
+    const float log_total = some ? logf(sum[1]) : 0.f, log_sum = logf(sum[0]);
+    distill_probabilities<T, NT>(a, t, top[1], sum[1], [&](int i, float p, float d) {
+        terms[0] += distill_term(p, d * a.inv_t - log_total, t.zc[i], top[0], log_sum, a);
+    });
+    if (a.loss) {
+        group_reduce<NT, false>(terms, t.red + 64);
+        if (threadIdx.x == 0) a.loss[row] = terms[0] * a.weight;
+    }
+    if (!a.grad) return;
+    distill_merge<T, NT>(a, t);
+    const float f = a.scale / sum[0];
+    if constexpr (NP > 0) {
+        distill_put<T, NT>(z, gr, 0, pieces, e, f, some, a.dim);
+    } else {
+        for (int p = 0; p < pieces; p += NT * HELD) {
+            distill_hold<T, NT>(z, zr, p, pieces, a.dim);
+            distill_put<T, NT>(z, gr, p, pieces, e, f, some, a.dim);
+        }
+    }
+    __syncthreads();  // behind all of those, the classes that the entries name
+    for (int i = threadIdx.x; i < a.top; i += NT) {
+        const int c = t.to[i];
+        if (c >= 0) gr[c] = some ? (T)(a.scale * (distill_exp(t.zc[i], top[0], a) / sum[0] - t.sum[i])) : (T)0.f;
+    }
 }
 
-// A part of a row to a workgroup: its maximum and sum ...
+// A part of a row to a workgroup: its maximum and sum; one more has the teacher's entries ...
 constexpr int DISTILL_NT = 256, DISTILL_NP = 4;
 template <typename T>
 __global__ __launch_bounds__(DISTILL_NT) void distill_part_kernel(const DistillArgs<T> a) {
     constexpr int NT = DISTILL_NT, NP = DISTILL_NP, VEC = RowPiece<T>::VEC;
-    __shared__ float red[32];
+    extern __shared__ __attribute__((aligned(16))) float lds[];
+    const DistillTop t(lds, a.top);
     const size_t row = blockIdx.y;
-    const int pieces = (a.dim + VEC - 1) / VEC, first = (int)blockIdx.x * a.per_part, end = min(first + a.per_part, pieces);
+    if (blockIdx.x == 0) {
+        float top[2] = {0.f, distill_fetch<T, NT>(a, row, t)}, sum[2] = {0.f, 0.f};
+        group_reduce<NT, true>(top, t.red);
+        sum[1] = distill_total<T, NT>(a, t, top[1]);
+        group_reduce<NT, false>(sum, t.red + 32);
+        DistillEntry *e = a.entry + row * a.top;
+        const float log_total = sum[1] != 0.f ? logf(sum[1]) : 0.f;
+        distill_probabilities<T, NT>(a, t, top[1], sum[1], [&](int i, float p, float d) {
+            e[i].p = p;
+            e[i].log_p = d * a.inv_t - log_total;
+        });
+        if (threadIdx.x == 0) a.part[row * (a.parts + 1) + a.parts] = make_float2(sum[1], 0.f);
+        distill_merge<T, NT>(a, t);
+        for (int i = threadIdx.x; i < a.top; i += NT) {
+            e[i].to = t.to[i];
+            e[i].sum = t.sum[i];
+            e[i].zc = t.zc[i];
+        }
+        return;
+    }
+    const int part = (int)blockIdx.x - 1;
+    const int pieces = (a.dim + VEC - 1) / VEC, first = part * a.per_part, end = min(first + a.per_part, pieces);
     RowPiece<T> z[NP];
     distill_hold<T, NT>(z, a.z + row * a.dim, first, end, a.dim);
-    const float m = group_reduce<NT, true>(distill_max<T>(z), red);
-    // (a part of nothing but -inf adds nothing to a row that has more)
-    const float s = group_reduce<NT, false>(m == -__builtin_inff() ? 0.f : distill_sum<T>(z, m, a), red + 16);
-    // a NaN among them is no maximum, but in the sum
-    if (threadIdx.x == 0) a.part[row * a.parts + blockIdx.x] = make_float2(m, s);
-    if (blockIdx.x == 0) {
-        for (int i = threadIdx.x; i < a.top; i += NT) {
-            const int c = a.at[row * a.top + i];
-            a.zc[row * a.top + i] = (unsigned)c < (unsigned)a.dim ? (float)a.z[row * a.dim + c] : 0.f;
-        }
-    }
+    float m[2] = {distill_max<T>(z), 0.f}, s[2] = {0.f, 0.f};
+    group_reduce<NT, true>(m, t.red);
+    // (a part of nothing but -inf adds nothing to a row that has more; a NaN among them is no maximum, but in the sum)
+    const DistillExp<T> e(m[0] == -__builtin_inff() ? 0.f : m[0], a);
+    s[0] = distill_sum<T>(z, e);
+    group_reduce<NT, false>(s, t.red + 32);
+    if (threadIdx.x == 0) a.part[row * (a.parts + 1) + part] = make_float2(m[0], s[0]);
 }
 // ... which every workgroup of the row joins before it writes its part's gradient; the first one has the loss.
 template <typename T>
 __global__ __launch_bounds__(DISTILL_NT) void distill_join_kernel(const DistillArgs<T> a) {
     constexpr int NT = DISTILL_NT, NP = DISTILL_NP, VEC = RowPiece<T>::VEC;
-    extern __shared__ __attribute__((aligned(16))) float lds[];
-    const DistillTop t(lds, a.top);
+    __shared__ __attribute__((aligned(16))) float red[96];
     const size_t row = blockIdx.y;
     const int pieces = (a.dim + VEC - 1) / VEC, first = (int)blockIdx.x * a.per_part, end = min(first + a.per_part, pieces);
+    const float2 *part = a.part + row * (a.parts + 1);
+    const DistillEntry *entry = a.entry + row * a.top;
     RowPiece<T> z[NP];
     if (a.grad) distill_hold<T, NT>(z, a.z + row * a.dim, first, end, a.dim);
-    distill_fetch<T, NT>(a, row, t);
-    float m = -__builtin_inff(), s = 0.f;
-    for (int i = threadIdx.x; i < a.parts; i += NT) m = fmaxf(m, a.part[row * a.parts + i].x);
-    m = group_reduce<NT, true>(m, t.red);
+    const bool some = part[a.parts].x != 0.f;
+    float top[2] = {-__builtin_inff(), 0.f}, sum[2] = {0.f, 0.f};
+    for (int i = threadIdx.x; i < a.parts; i += NT) top[0] = fmaxf(top[0], part[i].x);
+    group_reduce<NT, true>(top, red);
     for (int i = threadIdx.x; i < a.parts; i += NT) {
-        const float2 v = a.part[row * a.parts + i];
-        s += v.x == -__builtin_inff() ? v.y : v.y * distill_exp(v.x, m, a);
+        const float2 v = part[i];
+        sum[0] += v.x == -__builtin_inff() ? v.y : v.y * distill_exp(v.x, top[0], a);
     }
-    s = group_reduce<NT, false>(s, t.red + 16);
-    const bool some = distill_entries<T, NT>(a, row, t, m, s, a.loss && blockIdx.x == 0);
+    group_reduce<NT, false>(sum, red + 32);
+    if (a.loss && blockIdx.x == 0) {
+        float terms[2] = {0.f, 0.f};
+        const float log_sum = logf(sum[0]);
+        for (int i = threadIdx.x; i < a.top; i += NT) terms[0] += distill_term(entry[i].p, entry[i].log_p, entry[i].zc, top[0], log_sum, a);
+        group_reduce<NT, false>(terms, red + 64);
+        if (threadIdx.x == 0) a.loss[row] = terms[0] * a.weight;
+    }
     if (!a.grad) return;
-    distill_put<T, NT>(z, a.grad + row * a.dim, first, end, m, a.scale / s, some, a);
-    distill_put_entries<T, NT>(a, row, t, first * VEC, end == pieces ? a.dim : end * VEC);
+    T *gr = a.grad + row * a.dim;
+    distill_put<T, NT>(z, gr, first, end, DistillExp<T>(top[0], a), a.scale / sum[0], some, a.dim);
+    __syncthreads();  // behind all of those, the classes among them that the entries name
+    const int lo = first * VEC, hi = end == pieces ? a.dim : end * VEC;
+    for (int i = threadIdx.x; i < a.top; i += NT) {
+        const DistillEntry e = entry[i];
+        if (e.to >= lo && e.to < hi) gr[e.to] = some ? (T)(a.scale * (distill_exp(e.zc, top[0], a) / sum[0] - e.sum)) : (T)0.f;
+    }
 }
 
 template <typename T, int NT, int NP>
@@ -287,12 +399,13 @@ static int distill_launch(DistillArgs<T> &a, int ns) {
         parts = parts > least ? parts : least;
         a.per_part = (pieces + parts - 1) / parts;
         a.parts = (pieces + a.per_part - 1) / a.per_part;
-        float *ws = workspace(sizeof(float) * ((size_t)ns * a.parts * 2 + (size_t)ns * a.top));
+        const size_t entries = sizeof(DistillEntry) * (size_t)ns * a.top;
+        char *ws = reinterpret_cast<char *>(workspace(entries + sizeof(float2) * (size_t)ns * (a.parts + 1)));
         if (!ws) return 2;
-        a.part = reinterpret_cast<float2 *>(ws);
-        a.zc = ws + (size_t)ns * a.parts * 2;
-        hipLaunchKernelGGL((distill_part_kernel<T>), dim3(a.parts, ns), dim3(DISTILL_NT), 0, state().stream, a);
-        hipLaunchKernelGGL((distill_join_kernel<T>), dim3(a.grad ? a.parts : 1, ns), dim3(DISTILL_NT), distill_lds(a.top), state().stream, a);
+        a.entry = reinterpret_cast<DistillEntry *>(ws);
+        a.part = reinterpret_cast<float2 *>(ws + entries);
+        hipLaunchKernelGGL((distill_part_kernel<T>), dim3(a.parts + 1, ns), dim3(DISTILL_NT), distill_lds(a.top), state().stream, a);
+        hipLaunchKernelGGL((distill_join_kernel<T>), dim3(a.grad ? a.parts : 1, ns), dim3(DISTILL_NT), 0, state().stream, a);
     } else if (pieces <= 256) {
         distill_rows<T, 256, 1>(a, ns);
     } else if (pieces <= 512) {
@@ -305,8 +418,8 @@ static int distill_launch(DistillArgs<T> &a, int ns) {
         distill_rows<T, 512, 8>(a, ns);
     } else if (pieces <= 8192) {
         distill_rows<T, 1024, 8>(a, ns);
-    } else if (pieces <= 16384) {
-        distill_rows<T, 1024, 16>(a, ns);
+    } else if (pieces <= 12288) {
+        distill_rows<T, 1024, 12>(a, ns);
     } else {
         distill_rows<T, 1024, 0>(a, ns);
     }
