@@ -29,7 +29,7 @@ struct DistillArgs {
     float *loss;  // (NULL: not wanted)
     float2 *part;  // of each part of a row: its largest logit, the sum of exponentials relative to that
     struct DistillEntry *entry;  // of each row, behind those: what the first launch finds out about the teacher's entries
-    int dim, top, parts, per_part;  // per_part: pieces
+    int rows, dim, top, parts, per_part;  // per_part: pieces
     float inv_t, hi, lo;  // 1 / T; log2(e) / T as the sum of two floats above 0
     float weight, scale;  // scale = weight / T
 };
@@ -66,11 +66,28 @@ __device__ inline float distill_exp(float z, float m, const DistillArgs<T> &a) {
     return __builtin_amdgcn_exp2f(fmaf(d, a.hi, d * a.lo));
 }
 
-// Two values over a workgroup of NT threads.  `lds` holds two floats per wave and is not written again before another barrier.
+// NT threads have a row: a workgroup, or (64) one wave of a workgroup of four, which needs no barriers.
+template <int NT>
+__device__ inline int row_thread() { return NT == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x; }
+template <int NT>
+__device__ inline void row_sync() {
+    if constexpr (NT == 64) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    } else {
+        __syncthreads();
+    }
+}
+template <int NT>
+__device__ inline void row_sync_wave() {  // where a reduction follows, which is a barrier for a workgroup
+    if constexpr (NT == 64) row_sync<NT>();
+}
+// Two values over them.  `lds` holds two floats per wave and is not written again before another barrier.
 template <int NT, bool MAX>
 __device__ inline void group_reduce(float (&v)[2], float *lds) {
 #pragma unroll
     for (int i = 0; i < 2; ++i) v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
+    if constexpr (NT == 64) return;
     if ((threadIdx.x & 63) == 0) *reinterpret_cast<float2 *>(lds + 2 * (threadIdx.x >> 6)) = make_float2(v[0], v[1]);
     __syncthreads();
     const float2 r = *reinterpret_cast<const float2 *>(lds + 2 * (threadIdx.x & (NT / 64 - 1)));
@@ -87,7 +104,7 @@ __device__ inline void group_reduce(float (&v)[2], float *lds) {
 
 // In LDS: room for three reductions, then `top` (in whole fours) each of classes, logits of the teacher (later probabilities) and
 // of the student (later gradients).
-constexpr int DISTILL_RED = 96;
+constexpr int DISTILL_RED = 100;  // (the last four: whether a class is named twice)
 inline int distill_room(int top) { return (top + 3) & ~3; }
 inline size_t distill_lds(int top) { return sizeof(float) * (DISTILL_RED + 5 * (size_t)distill_room(top)); }
 struct DistillTop {
@@ -109,7 +126,7 @@ struct DistillTop {
 template <typename T, int NT>
 __device__ inline float distill_fetch(const DistillArgs<T> &a, size_t row, const DistillTop &t) {
     float m = -__builtin_inff();
-    for (int i = threadIdx.x; i < a.top; i += NT) {
+    for (int i = row_thread<NT>(); i < a.top; i += NT) {
         const int c = a.at[row * a.top + i];
         const bool in = (unsigned)c < (unsigned)a.dim;
         const float u = in ? (float)a.u[row * a.top + i] : -__builtin_inff();
@@ -118,18 +135,41 @@ __device__ inline float distill_fetch(const DistillArgs<T> &a, size_t row, const
         t.zc[i] = in ? (float)a.z[row * a.dim + c] : 0.f;
         m = fmaxf(m, u);
     }
-    if (threadIdx.x < 4 && a.top + threadIdx.x < (((unsigned)a.top + 3) & ~3u)) {
-        t.at[a.top + threadIdx.x] = -1;
-        t.p[a.top + threadIdx.x] = 0.f;
+    if (row_thread<NT>() < 4 && a.top + row_thread<NT>() < ((a.top + 3) & ~3)) {
+        t.at[a.top + row_thread<NT>()] = -1;
+        t.p[a.top + row_thread<NT>()] = 0.f;
     }
+    const int size = 2 * ((a.top + 3) & ~3);
+    int *table = reinterpret_cast<int *>(t.sum);
+    for (int i = row_thread<NT>(); i < size; i += NT) table[i] = -1;
+    if (row_thread<NT>() == 0) reinterpret_cast<int *>(t.red)[96] = 0;
     return m;
+}
+// Whether two entries name the same class: each puts its class into a table twice their number, at a place that follows from it or the
+// next free one, and finds it there if another one was first.  (Every entry compared with all others took 64 us of 74 for 8192 rows
+// of 300 classes with 250 entries.)
+template <typename T, int NT>
+__device__ inline void distill_insert(const DistillArgs<T> &a, const DistillTop &t) {
+    const int size = 2 * ((a.top + 3) & ~3);
+    int *table = reinterpret_cast<int *>(t.sum);
+    for (int i = row_thread<NT>(); i < a.top; i += NT) {
+        const int c = t.at[i];
+        if (c < 0) continue;
+        int h = (int)__umulhi((unsigned)c * 2654435761u, (unsigned)size);
+        for (;;) {
+            const int was = atomicCAS(table + h, -1, c);
+            if (was == c) reinterpret_cast<int *>(t.red)[96] = 1;
+            if (was == c || was == -1) break;
+            h = h + 1 == size ? 0 : h + 1;
+        }
+    }
 }
 // ... and the thread's sum of exp((u - um) / T); um is the teacher's largest, 0 where it has none (the sum is then 0, or NaN with one).
 template <typename T, int NT>
 __device__ inline float distill_total(const DistillArgs<T> &a, const DistillTop &t, float &um) {
     if (um == -__builtin_inff()) um = 0.f;
     float s = 0.f;
-    for (int i = threadIdx.x; i < a.top; i += NT) s += distill_exp(t.p[i], um, a);
+    for (int i = row_thread<NT>(); i < a.top; i += NT) s += distill_exp(t.p[i], um, a);
     return s;
 }
 
@@ -137,7 +177,7 @@ __device__ inline float distill_total(const DistillArgs<T> &a, const DistillTop 
 template <typename T, int NT, typename F>
 __device__ inline void distill_probabilities(const DistillArgs<T> &a, const DistillTop &t, float um, float total, F f) {
     const float inv_total = total != 0.f ? 1.f / total : 0.f;
-    for (int i = threadIdx.x; i < a.top; i += NT) {
+    for (int i = row_thread<NT>(); i < a.top; i += NT) {
         const float u = t.p[i], p = distill_exp(u, um, a) * inv_total;
         f(i, p, u - um);
         t.p[i] = p;
@@ -145,9 +185,16 @@ __device__ inline void distill_probabilities(const DistillArgs<T> &a, const Dist
 }
 // Sums of the probabilities of entries that name one class, and which of them is the first.
 template <typename T, int NT>
-__device__ inline void distill_merge(const DistillArgs<T> &a, const DistillTop &t) {
-    __syncthreads();  // all probabilities and classes are in LDS
-    for (int i = threadIdx.x; i < a.top; i += NT) {
+__device__ inline void distill_merge(const DistillArgs<T> &a, const DistillTop &t, bool twice) {
+    if (!twice) {
+        for (int i = row_thread<NT>(); i < a.top; i += NT) {
+            t.to[i] = t.at[i];
+            t.sum[i] = t.p[i];
+        }
+        return;
+    }
+    row_sync<NT>();  // all probabilities and classes are in LDS
+    for (int i = row_thread<NT>(); i < a.top; i += NT) {
         const int c = t.at[i];
         int first = c;
         float p = 0.f;
@@ -174,10 +221,10 @@ template <typename T, int NT, int NP>
 __device__ inline void distill_hold(RowPiece<T> (&z)[NP], const T *row, int first, int end, int dim) {
     constexpr int VEC = RowPiece<T>::VEC;
 #pragma unroll
-    for (int j = 0; j < NP; ++j) z[j].fetch(row, min(first + j * NT + (int)threadIdx.x, end - 1), dim);
+    for (int j = 0; j < NP; ++j) z[j].fetch(row, min(first + j * NT + row_thread<NT>(), end - 1), dim);
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        const int p = first + j * NT + (int)threadIdx.x;
+        const int p = first + j * NT + row_thread<NT>();
         z[j].trim(min(p, end - 1), dim);
         if (!__any(p >= end || (p + 1) * VEC > dim)) continue;
 #pragma unroll
@@ -224,7 +271,7 @@ __device__ inline float distill_sum(const RowPiece<T> (&z)[NP], const DistillExp
 // The gradient of the classes that are held.
 template <typename T, int NT, int NP>
 __device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const DistillExp<T> &e, float f, bool some, int dim) {
-    int mine = first + (int)threadIdx.x;
+    int mine = first + row_thread<NT>();
     asm volatile("" : "+v"(mine));  // (the loads' addresses are not kept for the stores)
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
@@ -239,12 +286,14 @@ __device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first
         if (p < end) o.store(row, p, dim);
     }
 }
-// A row to a workgroup.  NP = 0: it is read three times.
+// NP = 0: the row is read three times.
 template <typename T, int NT, int NP>
-__global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a) {
+__global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_row_kernel(const DistillArgs<T> a) {
     extern __shared__ __attribute__((aligned(16))) float lds[];
-    const DistillTop t(lds, a.top);
-    const size_t row = blockIdx.x;
+    const int wave = NT == 64 ? (int)(threadIdx.x >> 6) : 0;
+    const DistillTop t(lds + (size_t)wave * (DISTILL_RED + 5 * ((a.top + 3) & ~3)), a.top);
+    const size_t row = NT == 64 ? (size_t)blockIdx.x * 4 + wave : blockIdx.x;
+    if (NT == 64 && row >= (size_t)a.rows) return;
     constexpr int VEC = RowPiece<T>::VEC, HELD = NP ? NP : 4;
     const int pieces = (a.dim + VEC - 1) / VEC;
     const T *zr = a.z + row * a.dim;
@@ -263,8 +312,10 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a)
             top[0] = fmaxf(top[0], distill_max<T>(z));
         }
     }
+    row_sync_wave<NT>();
     group_reduce<NT, true>(top, t.red);
     const DistillExp<T> e(top[0], a);
+    distill_insert<T, NT>(a, t);
     if constexpr (NP > 0) {
         distill_as_read<T>(z);
         sum[0] = distill_sum<T>(z, e);
@@ -276,7 +327,9 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a)
         }
     }
     sum[1] = distill_total<T, NT>(a, t, top[1]);
+    row_sync_wave<NT>();
     group_reduce<NT, false>(sum, t.red + 32);
+    const bool twice = reinterpret_cast<const int *>(t.red)[96] != 0;
     const bool some = sum[1] != 0.f;  // (no entry, or all of them -inf)
     float terms[2] = {0.f, 0.f};
     const float log_total = some ? logf(sum[1]) : 0.f, log_sum = logf(sum[0]);
@@ -285,10 +338,10 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a)
     });
     if (a.loss) {
         group_reduce<NT, false>(terms, t.red + 64);
-        if (threadIdx.x == 0) a.loss[row] = terms[0] * a.weight;
+        if (row_thread<NT>() == 0) a.loss[row] = terms[0] * a.weight;
     }
     if (!a.grad) return;
-    distill_merge<T, NT>(a, t);
+    distill_merge<T, NT>(a, t, twice);
     const float f = a.scale / sum[0];
     if constexpr (NP > 0) {
         distill_put<T, NT>(z, gr, 0, pieces, e, f, some, a.dim);
@@ -298,8 +351,8 @@ __global__ __launch_bounds__(NT) void distill_row_kernel(const DistillArgs<T> a)
             distill_put<T, NT>(z, gr, p, pieces, e, f, some, a.dim);
         }
     }
-    __syncthreads();  // behind all of those, the classes that the entries name
-    for (int i = threadIdx.x; i < a.top; i += NT) {
+    row_sync<NT>();  // behind all of those, the classes that the entries name
+    for (int i = row_thread<NT>(); i < a.top; i += NT) {
         const int c = t.to[i];
         if (c >= 0) gr[c] = some ? (T)(a.scale * (distill_exp(t.zc[i], top[0], a) / sum[0] - t.sum[i])) : (T)0.f;
     }
@@ -316,8 +369,10 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_part_kernel(const DistillA
     if (blockIdx.x == 0) {
         float top[2] = {0.f, distill_fetch<T, NT>(a, row, t)}, sum[2] = {0.f, 0.f};
         group_reduce<NT, true>(top, t.red);
+        distill_insert<T, NT>(a, t);
         sum[1] = distill_total<T, NT>(a, t, top[1]);
         group_reduce<NT, false>(sum, t.red + 32);
+        const bool twice = reinterpret_cast<const int *>(t.red)[96] != 0;
         DistillEntry *e = a.entry + row * a.top;
         const float log_total = sum[1] != 0.f ? logf(sum[1]) : 0.f;
         distill_probabilities<T, NT>(a, t, top[1], sum[1], [&](int i, float p, float d) {
@@ -325,7 +380,7 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_part_kernel(const DistillA
             e[i].log_p = d * a.inv_t - log_total;
         });
         if (threadIdx.x == 0) a.part[row * (a.parts + 1) + a.parts] = make_float2(sum[1], 0.f);
-        distill_merge<T, NT>(a, t);
+        distill_merge<T, NT>(a, t, twice);
         for (int i = threadIdx.x; i < a.top; i += NT) {
             e[i].to = t.to[i];
             e[i].sum = t.sum[i];
@@ -385,7 +440,8 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_join_kernel(const DistillA
 
 template <typename T, int NT, int NP>
 static void distill_rows(const DistillArgs<T> &a, int ns) {
-    hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3(ns), dim3(NT), distill_lds(a.top), state().stream, a);
+    if (NT == 64) hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3((ns + 3) / 4), dim3(256), 4 * distill_lds(a.top), state().stream, a);
+    else hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3(ns), dim3(NT), distill_lds(a.top), state().stream, a);
 }
 
 template <typename T>
@@ -406,6 +462,11 @@ static int distill_launch(DistillArgs<T> &a, int ns) {
         a.part = reinterpret_cast<float2 *>(ws + entries);
         hipLaunchKernelGGL((distill_part_kernel<T>), dim3(a.parts + 1, ns), dim3(DISTILL_NT), distill_lds(a.top), state().stream, a);
         hipLaunchKernelGGL((distill_join_kernel<T>), dim3(a.grad ? a.parts : 1, ns), dim3(DISTILL_NT), 0, state().stream, a);
+    } else if ((pieces <= 256 && ns >= 4 * cu) || (pieces <= 512 && ns >= 16 * cu)) {
+        if (pieces <= 64) distill_rows<T, 64, 1>(a, ns);
+        else if (pieces <= 128) distill_rows<T, 64, 2>(a, ns);
+        else if (pieces <= 256) distill_rows<T, 64, 4>(a, ns);
+        else distill_rows<T, 64, 8>(a, ns);
     } else if (pieces <= 256) {
         distill_rows<T, 256, 1>(a, ns);
     } else if (pieces <= 512) {
@@ -420,6 +481,8 @@ static int distill_launch(DistillArgs<T> &a, int ns) {
         distill_rows<T, 1024, 8>(a, ns);
     } else if (pieces <= 12288) {
         distill_rows<T, 1024, 12>(a, ns);
+    } else if (pieces <= 16384) {
+        distill_rows<T, 1024, 16>(a, ns);
     } else {
         distill_rows<T, 1024, 0>(a, ns);
     }
@@ -448,6 +511,7 @@ static int distill_step(const Args *a, int ns, int step, const char *fn) {
     if (loss) d.loss = sg.out<float>(a->wr_loss, (size_t)ns);
     if (grad) d.grad = sg.out(reinterpret_cast<T *>(a->output->diff), n);
     if (sg.failed()) return 2;
+    d.rows = ns;
     d.dim = dim;
     d.top = top;
     const double log2e = 1.4426950408889634074 / a->temperature;

@@ -140,3 +140,21 @@ def test_host_arrays(pkg, gpu):
     a, keep = tr.distill_args(pkg, z.numpy(), hg, teacher.numpy(), classes.numpy(), hl, 2.0, 3.0)
     assert gpu.ptl_distill_fp16_batched(ctypes.byref(a), 3, 2) == 0
     assert torch.equal(torch.from_numpy(hl), loss.cpu()) and torch.equal(torch.from_numpy(hg), grad.cpu())
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,v,k", [(1027, 300, 5), (1030, 500, 250), (1025, 1500, 64), (1025, 2000, 70), (4100, 4000, 9), (1100, 9, 12)])
+def test_rows_by_the_wave(pkg, gpu, dt, n, v, k):
+    """Rows enough that each has one wave; some name a class twice, among them classes far apart in the row of entries."""
+    z, teacher, classes = case(n, n, v, k, dt)
+    classes[5, -1] = classes[5, 0] = 3
+    classes[7] = 4
+    check(dt, z, teacher, classes, *run(pkg, gpu, dt, z, teacher, classes))
+
+
+@pytest.mark.parametrize("n,v,k", [(3, 5000, 2048), (3, 100000, 2048), (200, 3000, 1000)])
+def test_many_entries_named_twice(pkg, gpu, n, v, k):
+    g = torch.Generator().manual_seed(n)
+    z, teacher, _ = case(n, n, v, k, "fp32")
+    classes = torch.randint(0, v, (n, k), generator=g, dtype=torch.int32)
+    check("fp32", z, teacher, classes, *run(pkg, gpu, "fp32", z, teacher, classes))
