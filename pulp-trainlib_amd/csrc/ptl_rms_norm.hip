@@ -8,7 +8,6 @@
 // A row has a wave of its own where there are rows enough to fill the chip with waves (no barrier, no LDS), else a
 // workgroup.  Rows that no workgroup can hold (more than 65536 values in fp16, 32768 in fp32) are read twice.
 #include "ptl_rows.hpp"
-#include "ptl_sum.hpp"
 #include "ptl_transformer.h"
 
 namespace ptl {
@@ -303,36 +302,6 @@ __global__ __launch_bounds__(256) void rms_norm_columns_kernel(const NormBw<T> a
         if (p * VEC + i < dim) a.part[(size_t)blockIdx.y * dim + p * VEC + i] = dw[i];
 }
 
-// dw[c] = the sum over the shares of part[share][c]: 32 columns (a 128-byte line) a workgroup, 32 shares at a time with four loads in
-// flight, so that a few thousand columns fill the chip (1024 shares of 4096: 18 us with 64 columns and 4 shares at a time, 5 so).
-template <typename T>
-__global__ __launch_bounds__(1024) void norm_dw_kernel(const float *__restrict__ part, T *__restrict__ out, int dim, int shares) {
-    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + o;
-    LongSum<T> s;
-    s.clear();
-    if (c < dim) {
-        int z = g;
-        for (; z + 96 < shares; z += 128) {
-            float v[4];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(z + 32 * u) * dim + c];
-#pragma unroll
-            for (int u = 0; u < 4; ++u) s.add(v[u]);
-        }
-        for (; z < shares; z += 32) s.add(part[(size_t)z * dim + c]);
-    }
-    __shared__ LongSum<T> red[32][32];
-    red[g][o] = s;
-    __syncthreads();
-    if (g != 0 || c >= dim) return;
-    for (int k = 1; k < 32; ++k) s.add(red[k][o]);
-    out[c] = (T)s.value();
-}
-template <typename T>
-static void norm_dw(const float *part, T *dw, int dim, int shares) {
-    hipLaunchKernelGGL((norm_dw_kernel<T>), dim3((dim + 31) / 32), dim3(1024), 0, state().stream, part, dw, dim, shares);
-}
-
 template <typename T, int TPR, int NP>
 static int norm_bw_launch(NormBw<T> &a, T *dw) {
     constexpr int PER = TPR == 64 ? 4 : 1;
@@ -341,7 +310,7 @@ static int norm_bw_launch(NormBw<T> &a, T *dw) {
     const int grid = (int)(want < most ? want : most), shares = grid * PER;
     if (dw && !(a.part = workspace((size_t)shares * a.dim * sizeof(float)))) return 2;
     hipLaunchKernelGGL((rms_norm_bw_kernel<T, TPR, NP>), dim3(grid), dim3(TPR == 64 ? 256 : TPR), 0, state().stream, a);
-    if (dw) norm_dw<T>(a.part, dw, a.dim, shares);
+    if (dw) row_shares<T>(a.part, dw, a.dim, shares);
     return hip_ok(hipGetLastError(), "rms norm launch") ? 0 : 2;
 }
 
@@ -361,7 +330,7 @@ static int norm_bw(NormBw<T> &a, T *dw) {
     a.part = dw ? ws + stat : nullptr;
     hipLaunchKernelGGL((rms_norm_stat_kernel<T>), dim3(a.rows), dim3(1024), 0, state().stream, a);
     hipLaunchKernelGGL((rms_norm_columns_kernel<T>), dim3((pieces + 255) / 256, shares), dim3(256), 0, state().stream, a);
-    if (dw) norm_dw<T>(a.part, dw, a.dim, shares);
+    if (dw) row_shares<T>(a.part, dw, a.dim, shares);
     return hip_ok(hipGetLastError(), "rms norm launch") ? 0 : 2;
 }
 

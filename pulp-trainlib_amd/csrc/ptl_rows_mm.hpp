@@ -58,6 +58,9 @@ struct Gate {
     }
 };
 
+// Both products behind the gradients of a gated layer's pre-activations (dw or dx NULL: not wanted), of whole 16-byte pieces.
+int gated_products(const _Float16 *x, const _Float16 *w, const _Float16 *dh, _Float16 *dw, _Float16 *dx, int ns, int in, int rows);
+
 // 0: launched, 2: HIP error.
 template <typename T>
 int rows_gated(RowsArgs &a);  // T: tensors and products

@@ -209,3 +209,19 @@ def test_every_kernel(pkg, gpu, dt, n, n_in, n_out, tile):
     x, w, b = inputs(n, dt, n, n_in, n_out, 1)
     check_forward(dt, "gelu", x, w, b, *forward(pkg, gpu, dt, "gelu", x, w, b))
     assert gpu.ptl_last_gemm_tile() == tile
+
+
+@pytest.mark.parametrize("n,n_in,n_out,bias", [(64, 2048, 800, 1), (70, 1032, 2500, 0), (1000, 256, 804, 1), (2056, 520, 260, 1), (520, 1024, 1024, 0),
+                                               (1300, 384, 1000, 1), (2500, 136, 900, 0)])
+def test_backward_own_products(pkg, gpu, n, n_in, n_out, bias):
+    """Layers from 1.5 GFLOP on, whose products are made in one launch: in parts and not, ends of k and of rows inside a tile."""
+    x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    full = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias)
+    check_backward("fp16", "silu", x, w, h, dy, *full)
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, skip_ig=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, None, dw, db)
+    assert (dx == 7).all()
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, skip_wg=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, dx, None, None)
+    assert (dw == 7).all() and (db is None or (db == 7).all())
