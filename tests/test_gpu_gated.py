@@ -198,7 +198,7 @@ def test_host_arrays(pkg, gpu):
         assert torch.equal(torch.from_numpy(got), ref.cpu())
 
 
-@pytest.mark.parametrize("dt,n,n_in,n_out,tile", [("fp16", 3, 1000, 300, 0), ("fp16", 40, 1024, 300, 32032), ("fp16", 40, 1025, 300, 32032),
+@pytest.mark.parametrize("dt,n,n_in,n_out,tile", [("fp16", 2, 1000, 300, 0), ("fp16", 3, 1000, 300, 32032), ("fp16", 40, 1024, 300, 32032), ("fp16", 40, 1025, 300, 32032),
                                                   ("fp16", 40, 1026, 300, 32032), ("fp16", 700, 512, 600, 64064), ("fp16", 700, 511, 600, 64064),
                                                   ("fp16", 700, 510, 600, 64064), ("fp16", 1500, 1024, 1100, 128128), ("fp16", 2100, 1025, 1500, 128128),
                                                   ("fp16", 2048, 1024, 2100, 256256), ("fp16", 2048, 1021, 2100, 256256), ("fp32", 4, 600, 300, 0),

@@ -105,7 +105,7 @@ def test_unaligned_operands_and_host_arrays(pkg, gpu):
 
 
 @pytest.mark.parametrize("n,m,k,tile", [(4, 300, 1000, 0), (30, 500, 2048, 32032), (30, 500, 2049, 32032), (900, 1000, 1024, 64064),
-                                        (900, 1000, 1022, 64064), (900, 1000, 1025, 64064), (2048, 2048, 1024, 128128), (4096, 2048, 2045, 128128),
+                                        (900, 1000, 1022, 64064), (900, 1000, 1025, 64064), (900, 1000, 1028, 64064), (2048, 2048, 1024, 128128), (4096, 2048, 2045, 128128),
                                         (2300, 4100, 2048, 256256), (2048, 4100, 2045, 256256)])
 def test_every_kernel(pkg, gpu, n, m, k, tile):
     """Each kernel on sizes that it is chosen for, the ones that copy rows first among them (their rows do not start on 16 bytes)."""
