@@ -59,7 +59,8 @@ static int linear_bw(const ::Linear_args_fp16 *l, int ns) { return ptl_linear_fp
 template <typename T>
 static bool own_products(const T *x, const T *w, const T *dh, int ns, int in, int outs) {
     const uintptr_t all = (uintptr_t)x | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)in * 2 | (uintptr_t)outs * 4;
-    return sizeof(T) == 2 && all % 16 == 0 && 8.0 * ns * in * outs >= 1.5e9 && state().gemm_path == 0;
+    const bool fits = in < 1 << 23 && outs < 1 << 22;  // (64 rows of the first operand and 128 of the second within 32 bits)
+    return sizeof(T) == 2 && fits && all % 16 == 0 && 8.0 * ns * in * outs >= 1.5e9 && state().gemm_path == 0;
 }
 
 template <typename T, typename Linear, typename Args>

@@ -152,7 +152,7 @@ def test_rows_by_the_wave(pkg, gpu, dt, n, v, k):
     check(dt, z, teacher, classes, *run(pkg, gpu, dt, z, teacher, classes))
 
 
-@pytest.mark.parametrize("n,v,k", [(3, 5000, 2048), (3, 100000, 2048), (200, 3000, 1000)])
+@pytest.mark.parametrize("n,v,k", [(3, 5000, 2048), (3, 100000, 2048), (200, 3000, 1000), (1030, 300, 700), (1030, 300, 512), (1030, 2000, 2048)])
 def test_many_entries_named_twice(pkg, gpu, n, v, k):
     g = torch.Generator().manual_seed(n)
     z, teacher, _ = case(n, n, v, k, "fp32")
