@@ -5,8 +5,10 @@
 // Both passes move bytes and nothing else (ten flops an element): a row is read once, into registers, its sums are formed
 // over the threads that hold it, and what the pass writes is formed from the same registers.  The statistics are not kept
 // for the way back: s is read there anyway, and its sum of squares comes with the other sum of the row.
-// A row has a wave of its own where there are rows enough to fill the chip with waves (no barrier, no LDS), else a
-// workgroup.  Rows that no workgroup can hold (more than 65536 values in fp16, 32768 in fp32) are read twice.
+// A row of up to 2048 bytes (4096 backward, in fp32) has a wave of its own (no barrier), a longer one a workgroup; rows that no workgroup
+// holds (more than 4096 pieces of 16 bytes forward, 2048 backward) are read twice.  Measured, with the residual's addition: 8192 rows of
+// 4096 fp16 values forward 45 us, 5.9 TB/s (in 8 bits 42 us), backward with the weights' gradient 62 us, 5.4 TB/s of five tensors;
+// 8192 x 1024 14 and 23 us; a few rows 3.7 us, which is an empty launch, and 7.3 us for the two launches backward.
 #include "ptl_rows.hpp"
 #include "ptl_transformer.h"
 
@@ -22,11 +24,10 @@ struct NormFw {
     float eps;
 };
 
-// The eight-bit integers of VEC values: one store of VEC bytes where the row has all of them.
-template <int VEC>
-__device__ inline void put_q(int8_t *row, int p, int dim, const int (&q)[VEC]) {
-    const int at = p * VEC;
-    if (at + VEC <= dim) {
+// The eight-bit integers of VEC values, from element `at` on: one store of VEC bytes where the row has all of them (WHOLE: it has).
+template <int VEC, bool WHOLE>
+__device__ inline void put_q(int8_t *row, int at, int dim, const int (&q)[VEC]) {
+    if (WHOLE || at + VEC <= dim) {
         unsigned u[VEC / 4];
 #pragma unroll
         for (int i = 0; i < VEC / 4; ++i)
@@ -45,56 +46,60 @@ template <typename T, int TPR, int NP, bool Q8>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(const NormFw<T> a) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC, HELD = NP ? NP : 1;
+    constexpr bool SHORT = TPR * NP == 64;  // rows of less than a piece come here too
     __shared__ float red[16][2];
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x;
-    const long row = TPR == 64 ? (long)blockIdx.x * 4 + (threadIdx.x >> 6) : blockIdx.x;
+    const long row = TPR == 64 ? (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
     if (row >= a.rows) return;  // (a whole wave, which has no barrier to meet)
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     const size_t at = (size_t)row * dim;
     float s[HELD][VEC];
     Piece w[HELD];
     float v[2] = {0.f, 0.f};  // sum of squares, largest |s w|
-    auto join = [&](Piece x, Piece k, int p, float (&f)[VEC]) {
-        x.trim(p, dim);
-        if (a.skip) k.trim(p, dim);
+    auto join = [&](const Piece &x, const Piece &k, float (&f)[VEC]) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) f[i] = a.skip ? (float)x.e[i] + (float)k.e[i] : (float)x.e[i];
     };
-    auto fetch = [&](int p, float (&f)[VEC]) {
-        Piece x, k;
-        x.fetch(a.x + at, p, dim);
-        if (a.skip) k.fetch(a.skip + at, p, dim);
-        join(x, k, p, f);
-    };
-    auto add = [&](const float (&f)[VEC], const Piece &w) {
+    auto add = [&](const float (&f)[VEC], const Piece &w, int cut) {
+        if (__any(cut)) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) v[0] = fmaf(f[i], f[i], v[0]);
+            for (int i = 0; i < VEC; ++i) v[0] = i < cut ? v[0] : fmaf(f[i], f[i], v[0]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) v[0] = fmaf(f[i], f[i], v[0]);
+        }
         if constexpr (Q8) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) v[1] = fmaxf(v[1], fabsf(f[i] * (float)w.e[i]));
         }
     };
+    // (rows that are walked: a thread reads behind the barrier what another may have written over by then, so each has its own elements)
+    auto walk = [&](int p, float (&f)[VEC], Piece &w) {
+        Piece x, k;
+        x.load(a.x + at, p, dim);
+        if (a.skip) k.load(a.skip + at, p, dim);
+        w.load(a.w, p, dim);
+        join(x, k, f);
+    };
     if constexpr (NP > 0) {
         Piece x[HELD], k[HELD];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) x[j].fetch(a.x + at, j * TPR + t, dim);
+        for (int j = 0; j < NP; ++j) x[j].template hold<SHORT>(a.x + at, j * TPR + t, dim);
 #pragma unroll
-        for (int j = 0; j < NP; ++j) w[j].fetch(a.w, j * TPR + t, dim);
+        for (int j = 0; j < NP; ++j) w[j].template hold<SHORT>(a.w, j * TPR + t, dim);
         if (a.skip) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) k[j].fetch(a.skip + at, j * TPR + t, dim);
+            for (int j = 0; j < NP; ++j) k[j].template hold<SHORT>(a.skip + at, j * TPR + t, dim);
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            join(x[j], k[j], j * TPR + t, s[j]);  // (pieces behind the end are zeros)
-            w[j].trim(j * TPR + t, dim);
-            add(s[j], w[j]);
+            join(x[j], k[j], s[j]);
+            add(s[j], w[j], Piece::cut(j * TPR + t, dim));
         }
     } else {
         for (int p = t; p < pieces; p += TPR) {
-            fetch(p, s[0]);
-            w[0].load(a.w, p, dim);
-            add(s[0], w[0]);
+            walk(p, s[0], w[0]);
+            add(s[0], w[0], 0);
         }
     }
     row_reduce<TPR, 2, true>(v, red);
@@ -104,21 +109,25 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     auto put = [&](int p, const float (&f)[VEC], const Piece &w) {
         if (p >= pieces) return;
         Piece o;
+        auto out = [&](T *to) {
+            if constexpr (NP > 0) o.template put<SHORT>(to, p, dim);
+            else o.store(to, p, dim);
+        };
         if (a.skip) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) o.e[i] = (T)f[i];
-            o.store(a.sum + at, p, dim);
+            out(a.sum + at);
         }
         if (a.y) {
 #pragma unroll
             for (int i = 0; i < VEC; ++i) o.e[i] = (T)(f[i] * r * (float)w.e[i]);
-            o.store(a.y + at, p, dim);
+            out(a.y + at);
         }
         if constexpr (Q8) {
             int q[VEC];
 #pragma unroll
             for (int i = 0; i < VEC; ++i) q[i] = (int)fminf(fmaxf(rintf(f[i] * (float)w.e[i] * unit), -127.f), 127.f);
-            put_q<VEC>(a.q + at, p, dim, q);
+            put_q<VEC, (NP > 0 && !SHORT)>(a.q + at, p * VEC - (NP > 0 ? Piece::cut(p, dim) : 0), dim, q);
         }
     };
     if constexpr (NP > 0) {
@@ -126,8 +135,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
         for (int j = 0; j < NP; ++j) put(j * TPR + t, s[j], w[j]);
     } else {
         for (int p = t; p < pieces; p += TPR) {
-            fetch(p, s[0]);
-            w[0].load(a.w, p, dim);
+            walk(p, s[0], w[0]);
             put(p, s[0], w[0]);
         }
     }
@@ -145,18 +153,18 @@ static void norm_fw_launch(const NormFw<T> &a) {
 template <typename T>
 static void norm_fw(const NormFw<T> &a) {
     const int pieces = (a.dim + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC;
-    if (a.rows >= 1024 && pieces <= 512) {
-        if (pieces <= 64) return norm_fw_launch<T, 64, 1>(a);
-        if (pieces <= 128) return norm_fw_launch<T, 64, 2>(a);
-        if (pieces <= 256) return norm_fw_launch<T, 64, 4>(a);
-        return norm_fw_launch<T, 64, 8>(a);
-    }
+    // A wave with four pieces would lose to a workgroup with one where rows are few (300 x 2048 fp16 in 8 bits: 4.1 against 3.9 us) and
+    // gain nothing where they are many (8192 x 2048: 24.8 against 25.1); with two it gains (8192 x 1024: 13.8 against 15.2).
     if (pieces <= 64) return norm_fw_launch<T, 64, 1>(a);
+    if (pieces <= 128) return norm_fw_launch<T, 64, 2>(a);
     if (pieces <= 256) return norm_fw_launch<T, 256, 1>(a);
     if (pieces <= 512) return norm_fw_launch<T, 256, 2>(a);
-    if (pieces <= 1024) return norm_fw_launch<T, 256, 4>(a);
-    if (pieces <= 4096) return norm_fw_launch<T, 1024, 4>(a);
-    if (pieces <= 8192) return norm_fw_launch<T, 1024, 8>(a);
+    if (pieces <= 1024) return norm_fw_launch<T, 512, 2>(a);
+    // (every CU with rows: four waves a row, 2000 x 8192 fp32 48 against 51 us with eight; few rows: eight, 4 x 14144 fp16 3.7 against 4.2)
+    if (pieces <= 2048 && a.rows >= state().num_cu) return norm_fw_launch<T, 256, 8>(a);
+    if (pieces <= 2048) return norm_fw_launch<T, 512, 4>(a);
+    if (pieces <= 4096) return norm_fw_launch<T, 512, 8>(a);
+    // (1024 threads with eight pieces each would spill registers: 1000 x 40000 fp16 112 us, in 8 bits 172; read twice 71 and 63)
     norm_fw_launch<T, 1024, 0>(a);
 }
 
@@ -170,78 +178,119 @@ struct NormBw {
     float eps;
 };
 
-template <typename T>
 __device__ inline float norm_dx(float s, float g, float add, float r, float m) { return fmaf(r, g, fmaf(-m, s, add)); }
 
-// Workgroups walk over rows and keep their share of dw in registers: it is written once, at the end.
+// Workgroups walk over rows and keep their share of dw in registers: it is written once, at the end.  The next row is on its way while
+// one is worked on, as far as registers go.
 template <typename T, int TPR, int NP>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(const NormBw<T> a) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC, PER = TPR == 64 ? 4 : 1;
+    constexpr bool AHEAD = NP * VEC <= 16 && TPR <= 256, SHORT = TPR * NP == 64;  // (rows of less than a piece come to the latter)
     __shared__ float red[2][16][2];
-    const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x;
-    const int first = TPR == 64 ? (int)blockIdx.x * 4 + (int)(threadIdx.x >> 6) : (int)blockIdx.x;
+    const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const long first = TPR == 64 ? (long)blockIdx.x * 4 + wave : blockIdx.x, stride = (long)gridDim.x * PER;
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     Piece w[NP];
     float dw[NP][VEC];
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        w[j].load(a.w, j * TPR + t, dim);
+        w[j].template hold<SHORT>(a.w, j * TPR + t, dim);
 #pragma unroll
         for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
     }
-    int turn = 0;
-    for (long row = first; row < a.rows; row += (long)gridDim.x * PER, turn ^= 1) {
-        const size_t at = (size_t)row * dim;
+    struct Row {
         Piece s[NP], g[NP], d[NP];
+    };
+    auto fetch = [&](long row, Row &r) {
+        const size_t at = (size_t)row * dim;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
-            s[j].fetch(a.s + at, j * TPR + t, dim);
-            g[j].fetch(a.dy + at, j * TPR + t, dim);
+            r.s[j].template hold<SHORT>(a.s + at, j * TPR + t, dim);
+            r.g[j].template hold<SHORT>(a.dy + at, j * TPR + t, dim);
         }
         if (a.add) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) d[j].fetch(a.add + at, j * TPR + t, dim);
+            for (int j = 0; j < NP; ++j) r.d[j].template hold<SHORT>(a.add + at, j * TPR + t, dim);
         }
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            s[j].trim(j * TPR + t, dim);
-            g[j].trim(j * TPR + t, dim);
-            if (a.add) d[j].trim(j * TPR + t, dim);
-        }
+    };
+    int turn = 0;
+    auto work = [&](long row, Row &x) {
+        const size_t at = (size_t)row * dim;
         float v[2] = {0.f, 0.f};
 #pragma unroll
-        for (int j = 0; j < NP; ++j)
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) {
-                const float f = (float)s[j].e[i];
+        for (int j = 0; j < NP; ++j) {
+            const int cut = Piece::cut(j * TPR + t, dim);
+            auto add = [&](int i) {
+                const float f = (float)x.s[j].e[i];
                 v[0] = fmaf(f, f, v[0]);
-                v[1] = fmaf((float)g[j].e[i] * (float)w[j].e[i], f, v[1]);
+                v[1] = fmaf((float)x.g[j].e[i] * (float)w[j].e[i], f, v[1]);
+            };
+            if (__any(cut)) {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (i >= cut) add(i);
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) add(i);
             }
+        }
         row_reduce<TPR, 2>(v, red[turn]);
+        turn ^= 1;
         const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps), m = r * r * r * (v[1] / (float)dim);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int p = j * TPR + t;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) dw[j][i] = fmaf((float)g[j].e[i], (float)s[j].e[i] * r, dw[j][i]);
+            for (int i = 0; i < VEC; ++i) dw[j][i] = fmaf((float)x.g[j].e[i], (float)x.s[j].e[i] * r, dw[j][i]);
             if (!a.dx || p >= pieces) continue;
             Piece o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                o.e[i] = (T)norm_dx<T>((float)s[j].e[i], (float)g[j].e[i] * (float)w[j].e[i], a.add ? (float)d[j].e[i] : 0.f, r, m);
-            o.store(a.dx + at, p, dim);
-            if (a.dx2) o.store(a.dx2 + at, p, dim);
+                o.e[i] = (T)norm_dx((float)x.s[j].e[i], (float)x.g[j].e[i] * (float)w[j].e[i], a.add ? (float)x.d[j].e[i] : 0.f, r, m);
+            o.template put<SHORT>(a.dx + at, p, dim);
+            if (a.dx2) o.template put<SHORT>(a.dx2 + at, p, dim);
+        }
+    };
+    if constexpr (AHEAD) {
+        Row x, y;
+        long row = first;
+        if (row < a.rows) fetch(row, x);
+        for (; row < a.rows; row += 2 * stride) {
+            if (row + stride < a.rows) fetch(row + stride, y);
+            work(row, x);
+            if (row + stride >= a.rows) break;
+            if (row + 2 * stride < a.rows) fetch(row + 2 * stride, x);
+            work(row + stride, y);
+        }
+    } else {
+        Row x;
+        for (long row = first; row < a.rows; row += stride) {
+            fetch(row, x);
+            work(row, x);
         }
     }
     if (!a.part) return;
-    float *out = a.part + (size_t)first * dim;
+    float *out = a.part + (size_t)blockIdx.x * dim;
+    if constexpr (TPR == 64) {  // the four waves' shares as one
+        __shared__ float all[4][64 * NP * VEC];
 #pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int at = (j * TPR + t) * VEC;
+        for (int j = 0; j < NP; ++j)
 #pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (at + i < dim) out[at + i] = dw[j][i];
+            for (int i = 0; i < VEC; ++i)
+                if (i >= Piece::cut(j * 64 + t, dim)) all[wave][(j * 64 + t) * VEC - Piece::cut(j * 64 + t, dim) + i] = dw[j][i];
+        __syncthreads();
+        for (int c = threadIdx.x; c < dim; c += 256) out[c] = all[0][c] + all[1][c] + (all[2][c] + all[3][c]);
+    } else {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            const int p = j * TPR + t;
+            if (p >= pieces) continue;
+#pragma unroll
+            for (int i = 0; i < VEC; i += 4)
+                *reinterpret_cast<row_u4 *>(out + p * VEC - Piece::cut(p, dim) + i) =
+                    __builtin_bit_cast(row_u4, row_f4{dw[j][i], dw[j][i + 1], dw[j][i + 2], dw[j][i + 3]});
+        }
     }
 }
 
@@ -291,7 +340,7 @@ __global__ __launch_bounds__(256) void rms_norm_columns_kernel(const NormBw<T> a
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
             dw[i] = fmaf((float)g.e[i], (float)s.e[i] * r, dw[i]);
-            o.e[i] = (T)norm_dx<T>((float)s.e[i], (float)g.e[i] * (float)w.e[i], a.add ? (float)d.e[i] : 0.f, r, m);
+            o.e[i] = (T)norm_dx((float)s.e[i], (float)g.e[i] * (float)w.e[i], a.add ? (float)d.e[i] : 0.f, r, m);
         }
         if (a.dx) o.store(a.dx + at, p, dim);
         if (a.dx2) o.store(a.dx2 + at, p, dim);
@@ -302,22 +351,33 @@ __global__ __launch_bounds__(256) void rms_norm_columns_kernel(const NormBw<T> a
         if (p * VEC + i < dim) a.part[(size_t)blockIdx.y * dim + p * VEC + i] = dw[i];
 }
 
+// How many workgroups: the more of them, the faster the rows pass (a workgroup moves about 35 GB/s, up to what memory gives), and the
+// more shares of dw are written and read (8 bytes a column and workgroup, at 5 TB/s); the sum of both times is least at
+// sqrt(72 rows sizeof(T)).  Measured with 72, 208 and 600: 8192 x 1024 fp16 23.4, 26.4 and 26.5 us, 2000 x 8192 fp16 39.1, 37.9 and 43.5,
+// 8192 x 2048 fp32 57.8, 63.5 and 68.1.
+template <typename T>
+static int norm_groups(int rows, int per) {
+    const int groups = (rows + per - 1) / per, best = (int)sqrtf(72.f * (float)rows * sizeof(T));
+    return groups < best ? groups : best > 1 ? best : 1;
+}
 template <typename T, int TPR, int NP>
 static int norm_bw_launch(NormBw<T> &a, T *dw) {
-    constexpr int PER = TPR == 64 ? 4 : 1;
-    const int per_cu = TPR == 512 ? 2 : 4;
-    const long want = ((long)a.rows + PER - 1) / PER, most = (long)per_cu * state().num_cu;
-    const int grid = (int)(want < most ? want : most), shares = grid * PER;
-    if (dw && !(a.part = workspace((size_t)shares * a.dim * sizeof(float)))) return 2;
+    const int grid = norm_groups<T>(a.rows, TPR == 64 ? 4 : 1);
+    if (dw && !(a.part = workspace((size_t)grid * a.dim * sizeof(float)))) return 2;
     hipLaunchKernelGGL((rms_norm_bw_kernel<T, TPR, NP>), dim3(grid), dim3(TPR == 64 ? 256 : TPR), 0, state().stream, a);
-    if (dw) row_shares<T>(a.part, dw, a.dim, shares);
+    if (dw) row_shares<T>(a.part, dw, a.dim, grid);
     return hip_ok(hipGetLastError(), "rms norm launch") ? 0 : 2;
 }
 
 template <typename T>
 static int norm_bw(NormBw<T> &a, T *dw) {
     const int pieces = (a.dim + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC;
+    // (a wave for up to 1024 values: 8192 x 1024 fp16 23.4 us, by workgroups of one piece a thread 38.6; fp32 33.3 and 36.1)
     if (pieces <= 64) return norm_bw_launch<T, 64, 1>(a, dw);
+    if (pieces <= 128) return norm_bw_launch<T, 64, 2>(a, dw);
+    if constexpr (sizeof(T) == 4) {
+        if (pieces <= 256) return norm_bw_launch<T, 64, 4>(a, dw);
+    }
     if (pieces <= 256) return norm_bw_launch<T, 256, 1>(a, dw);
     if (pieces <= 512) return norm_bw_launch<T, 256, 2>(a, dw);
     if (pieces <= 1024) return norm_bw_launch<T, 256, 4>(a, dw);

@@ -12,6 +12,7 @@
 namespace ptl {
 
 typedef unsigned row_u4 __attribute__((ext_vector_type(4), aligned(1)));  // 16 bytes wherever they start
+typedef float row_f4 __attribute__((ext_vector_type(4)));
 typedef unsigned row_u2 __attribute__((ext_vector_type(2), aligned(1)));
 typedef unsigned row_u1 __attribute__((aligned(1)));
 
@@ -22,6 +23,24 @@ struct RowPiece {
         row_u4 raw;
         T e[VEC];
     };
+    // How a thread holds piece p of a row of at least VEC elements where the whole row is in registers before any of it is written:
+    // the piece that reaches over the end covers the row's last VEC elements, the first cut() of which are another piece's too
+    // (pieces behind the end: all of them).  They are left out of sums and written twice with the same values, so that no load and
+    // no store depends on where the row ends: kernels of a few pieces a thread are bound by fetching their own instructions, and
+    // values written one by one were most of those (a row of 14144 fp16 values through a gradient: 11 us, 5 so).
+    static __device__ inline int cut(int p, int dim) { return p * VEC - min(p * VEC, max(dim - VEC, 0)); }
+    // (a row held in registers is far shorter than 4 GB: the row's address plus an unsigned offset is one instruction's operand)
+    static __device__ inline unsigned place(int p, int dim) { return (unsigned)min(p * VEC, dim - VEC) * (unsigned)sizeof(T); }
+    template <bool SHORT>
+    __device__ inline void hold(const T *row, int p, int dim) {
+        if (SHORT && dim < VEC) fetch(row, p, dim);
+        else raw = *reinterpret_cast<const row_u4 *>(reinterpret_cast<const char *>(row) + place(p, dim));
+    }
+    template <bool SHORT>
+    __device__ inline void put(T *row, int p, int dim) const {
+        if (SHORT && dim < VEC) store(row, p, dim);
+        else if (p * VEC < dim) *reinterpret_cast<row_u4 *>(reinterpret_cast<char *>(row) + place(p, dim)) = raw;
+    }
     // Piece p of a row of `dim` elements.  No load depends on where the row ends: a piece that reaches over the end is read so that
     // it ends there, and trim() moves its values down and puts zeros behind them (only the waves that hold such a piece do).  All
     // of a thread's pieces are fetched before the first is trimmed.
