@@ -53,6 +53,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     if (row >= a.rows) return;  // (a whole wave, which has no barrier to meet)
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     const size_t at = (size_t)row * dim;
+    auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };  // (pieces that no thread has; half of them someone has)
     float s[HELD][VEC];
     Piece w[HELD];
     float v[2] = {0.f, 0.f};  // sum of squares, largest |s w|
@@ -84,15 +85,25 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     if constexpr (NP > 0) {
         Piece x[HELD], k[HELD];
 #pragma unroll
-        for (int j = 0; j < NP; ++j) x[j].template hold<SHORT>(a.x + at, j * TPR + t, dim);
-#pragma unroll
-        for (int j = 0; j < NP; ++j) w[j].template hold<SHORT>(a.w, j * TPR + t, dim);
-        if (a.skip) {
-#pragma unroll
-            for (int j = 0; j < NP; ++j) k[j].template hold<SHORT>(a.skip + at, j * TPR + t, dim);
+        for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
+            x[j].template hold<SHORT>(a.x + at, j * TPR + t, dim);
         }
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
+            w[j].template hold<SHORT>(a.w, j * TPR + t, dim);
+        }
+        if (a.skip) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                if (none(j)) break;
+                k[j].template hold<SHORT>(a.skip + at, j * TPR + t, dim);
+            }
+        }
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
             join(x[j], k[j], s[j]);
             add(s[j], w[j], Piece::cut(j * TPR + t, dim));
         }
@@ -132,7 +143,10 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     };
     if constexpr (NP > 0) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) put(j * TPR + t, s[j], w[j]);
+        for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
+            put(j * TPR + t, s[j], w[j]);
+        }
     } else {
         for (int p = t; p < pieces; p += TPR) {
             walk(p, s[0], w[0]);
@@ -191,6 +205,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long first = TPR == 64 ? (long)blockIdx.x * 4 + wave : blockIdx.x, stride = (long)gridDim.x * PER;
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
+    auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };  // (pieces that no thread has; half of them someone has)
     Piece w[NP];
     float dw[NP][VEC];
 #pragma unroll
@@ -206,12 +221,16 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
         const size_t at = (size_t)row * dim;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
             r.s[j].template hold<SHORT>(a.s + at, j * TPR + t, dim);
             r.g[j].template hold<SHORT>(a.dy + at, j * TPR + t, dim);
         }
         if (a.add) {
 #pragma unroll
-            for (int j = 0; j < NP; ++j) r.d[j].template hold<SHORT>(a.add + at, j * TPR + t, dim);
+            for (int j = 0; j < NP; ++j) {
+                if (none(j)) break;
+                r.d[j].template hold<SHORT>(a.add + at, j * TPR + t, dim);
+            }
         }
     };
     int turn = 0;
@@ -220,6 +239,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
         float v[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
             const int cut = Piece::cut(j * TPR + t, dim);
             auto add = [&](int i) {
                 const float f = (float)x.s[j].e[i];
@@ -240,6 +260,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
         const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps), m = r * r * r * (v[1] / (float)dim);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
             const int p = j * TPR + t;
 #pragma unroll
             for (int i = 0; i < VEC; ++i) dw[j][i] = fmaf((float)x.g[j].e[i], (float)x.s[j].e[i] * r, dw[j][i]);
