@@ -6,9 +6,10 @@
 // over the threads that hold it, and what the pass writes is formed from the same registers.  The statistics are not kept
 // for the way back: s is read there anyway, and its sum of squares comes with the other sum of the row.
 // A row of up to 2048 bytes (4096 backward, in fp32) has a wave of its own (no barrier), a longer one a workgroup; rows that no workgroup
-// holds (more than 4096 pieces of 16 bytes forward, 2048 backward) are read twice.  Measured, with the residual's addition: 8192 rows of
+// holds (more than 4096 pieces of 16 bytes forward, 16384 values backward) are read twice.  Measured, with the residual's addition: 8192 rows of
 // 4096 fp16 values forward 45 us, 5.9 TB/s (in 8 bits 42 us), backward with the weights' gradient 62 us, 5.4 TB/s of five tensors;
-// 8192 x 1024 14 and 23 us; a few rows 3.7 us, which is an empty launch, and 7.3 us for the two launches backward.
+// 8192 x 1024 14 and 23 us; a few rows 3.7 us, which is an empty launch, and backward 4 us for one to three,
+// 7.3 for the two launches of more.
 #include "ptl_rows.hpp"
 #include "ptl_transformer.h"
 
@@ -186,7 +187,8 @@ template <typename T>
 struct NormBw {
     const T *s, *dy, *add, *w;
     T *dx, *dx2;  // (NULL: not wanted)
-    float *part;  // of dw: a row for each wave or workgroup (NULL: not wanted)
+    T *dw;        // where one workgroup has all the rows (else NULL)
+    float *part;  // of dw: a row for each workgroup (NULL: not wanted)
     float *stat;  // long rows: r and r^3 mean(g s) of each row
     int rows, dim;
     float eps;
@@ -194,38 +196,69 @@ struct NormBw {
 
 __device__ inline float norm_dx(float s, float g, float add, float r, float m) { return fmaf(r, g, fmaf(-m, s, add)); }
 
+// Whether registers hold two rows.
+template <typename T, int TPR, int NP>
+constexpr bool norm_ahead() { return NP * RowPiece<T>::VEC <= 16 && TPR <= 256; }
 // Workgroups walk over rows and keep their share of dw in registers: it is written once, at the end.  The next row is on its way while
 // one is worked on, as far as registers go.
 template <typename T, int TPR, int NP>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(const NormBw<T> a) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC, PER = TPR == 64 ? 4 : 1;
-    constexpr bool AHEAD = NP * VEC <= 16 && TPR <= 256, SHORT = TPR * NP == 64;  // (rows of less than a piece come to the latter)
+    constexpr bool AHEAD = norm_ahead<T, TPR, NP>(), SHORT = TPR * NP == 64;  // (rows of less than a piece come to the latter)
+    // 128 registers a thread: the weights and their gradient are in LDS, the gradient along the residual is fetched when the sums are known
+    constexpr bool LATE = TPR == 1024;
     __shared__ float red[2][16][2];
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const long first = TPR == 64 ? (long)blockIdx.x * 4 + wave : blockIdx.x, stride = (long)gridDim.x * PER;
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };  // (pieces that no thread has; half of them someone has)
-    Piece w[NP];
-    float dw[NP][VEC];
+    __shared__ row_u4 w_lds[LATE ? NP * TPR : 1];
+    __shared__ row_f4 dw_lds[LATE ? NP * TPR : 1];
+    Piece w[LATE ? 1 : NP];
+    float dw[LATE ? 1 : NP][VEC];
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        w[j].template hold<SHORT>(a.w, j * TPR + t, dim);
+        w[LATE ? 0 : j].template hold<SHORT>(a.w, j * TPR + t, dim);
+        if constexpr (LATE) {  // (a thread's own)
+            w_lds[j * TPR + t] = w[0].raw;
+            dw_lds[j * TPR + t] = row_f4{0.f, 0.f, 0.f, 0.f};
+        } else {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
+            for (int i = 0; i < VEC; ++i) dw[j][i] = 0.f;
+        }
     }
+    auto weights = [&](int j) {
+        if constexpr (LATE) w[0].raw = w_lds[j * TPR + t];
+        return w[LATE ? 0 : j];
+    };
+    auto gather = [&](int j) {
+        if constexpr (LATE) {
+            const row_f4 f = dw_lds[j * TPR + t];
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) dw[0][i] = f[i];
+        }
+    };
     struct Row {
-        Piece s[NP], g[NP], d[NP];
+        Piece s[NP], g[NP], d[LATE ? 1 : NP];
+    };
+    // Where a row starts.  With the barrier it is one scalar, not an address for each piece of each tensor that goes along with the rows in
+    // registers: 8192 x 4096 fp16 63.2 -> 61.6 us, 8192 x 1024 23.1 -> 21.9; with one piece a thread or four the addresses cost less than
+    // what they save (8192 x 2048 35.3 us, 38.2 without them; 5946 x 8243 125 and 132).
+    auto start = [&](long row) {
+        size_t at = (size_t)row * dim;
+        if constexpr (NP == 2 || LATE) asm volatile("" : "+s"(at));
+        return at;
     };
     auto fetch = [&](long row, Row &r) {
-        const size_t at = (size_t)row * dim;
+        const size_t at = start(row);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
             r.s[j].template hold<SHORT>(a.s + at, j * TPR + t, dim);
             r.g[j].template hold<SHORT>(a.dy + at, j * TPR + t, dim);
         }
-        if (a.add) {
+        if (!LATE && a.add) {
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 if (none(j)) break;
@@ -235,16 +268,17 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
     };
     int turn = 0;
     auto work = [&](long row, Row &x) {
-        const size_t at = (size_t)row * dim;
+        const size_t at = start(row);
         float v[2] = {0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
             const int cut = Piece::cut(j * TPR + t, dim);
+            const Piece wj = weights(j);
             auto add = [&](int i) {
                 const float f = (float)x.s[j].e[i];
                 v[0] = fmaf(f, f, v[0]);
-                v[1] = fmaf((float)x.g[j].e[i] * (float)w[j].e[i], f, v[1]);
+                v[1] = fmaf((float)x.g[j].e[i] * (float)wj.e[i], f, v[1]);
             };
             if (__any(cut)) {
 #pragma unroll
@@ -261,14 +295,31 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
+            if constexpr (LATE) __builtin_amdgcn_sched_barrier(0);  // (one piece at a time, for its registers)
             const int p = j * TPR + t;
+            gather(j);
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) dw[j][i] = fmaf((float)x.g[j].e[i], (float)x.s[j].e[i] * r, dw[j][i]);
+            for (int i = 0; i < VEC; ++i) dw[LATE ? 0 : j][i] = fmaf((float)x.g[j].e[i], (float)x.s[j].e[i] * r, dw[LATE ? 0 : j][i]);
+            if constexpr (LATE) dw_lds[j * TPR + t] = row_f4{dw[0][0], dw[0][1], dw[0][2], dw[0][3]};
             if (!a.dx || p >= pieces) continue;
+            if constexpr (LATE) {
+                if (a.add) x.d[0].template hold<SHORT>(a.add + at, p, dim);
+            }
+            const Piece wj = weights(j), &d = x.d[LATE ? 0 : j];
             Piece o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                o.e[i] = (T)norm_dx((float)x.s[j].e[i], (float)x.g[j].e[i] * (float)w[j].e[i], a.add ? (float)x.d[j].e[i] : 0.f, r, m);
+                o.e[i] = (T)norm_dx((float)x.s[j].e[i], (float)x.g[j].e[i] * (float)wj.e[i], a.add ? (float)d.e[i] : 0.f, r, m);
+            const int cut = LATE ? Piece::cut(p, dim) : 0;
+            if (cut) {  // (a.add, read late, may be in the place of dx: another thread's elements are left to it)
+#pragma unroll
+                for (int i = 1; i < VEC; ++i) {
+                    if (i < cut) continue;
+                    a.dx[at + p * VEC - cut + i] = o.e[i];
+                    if (a.dx2) a.dx2[at + p * VEC - cut + i] = o.e[i];
+                }
+                continue;
+            }
             o.template put<SHORT>(a.dx + at, p, dim);
             if (a.dx2) o.template put<SHORT>(a.dx2 + at, p, dim);
         }
@@ -291,8 +342,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
             work(row, x);
         }
     }
-    if (!a.part) return;
-    float *out = a.part + (size_t)blockIdx.x * dim;
+    if (!a.part && !a.dw) return;
+    auto out = [&](int c, float v) {
+        if (a.dw) a.dw[c] = (T)v;
+        else a.part[(size_t)blockIdx.x * dim + c] = v;
+    };
     if constexpr (TPR == 64) {  // the four waves' shares as one
         __shared__ float all[4][64 * NP * VEC];
 #pragma unroll
@@ -301,16 +355,27 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
             for (int i = 0; i < VEC; ++i)
                 if (i >= Piece::cut(j * 64 + t, dim)) all[wave][(j * 64 + t) * VEC - Piece::cut(j * 64 + t, dim) + i] = dw[j][i];
         __syncthreads();
-        for (int c = threadIdx.x; c < dim; c += 256) out[c] = all[0][c] + all[1][c] + (all[2][c] + all[3][c]);
+        for (int c = threadIdx.x; c < dim; c += 256) out(c, all[0][c] + all[1][c] + (all[2][c] + all[3][c]));
+    } else if (a.dw) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            gather(j);
+            Piece o;
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) o.e[i] = (T)dw[LATE ? 0 : j][i];
+            o.template put<SHORT>(a.dw, j * TPR + t, dim);
+        }
     } else {
+        float *part = a.part + (size_t)blockIdx.x * dim;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int p = j * TPR + t;
             if (p >= pieces) continue;
+            gather(j);
 #pragma unroll
             for (int i = 0; i < VEC; i += 4)
-                *reinterpret_cast<row_u4 *>(out + p * VEC - Piece::cut(p, dim) + i) =
-                    __builtin_bit_cast(row_u4, row_f4{dw[j][i], dw[j][i + 1], dw[j][i + 2], dw[j][i + 3]});
+                *reinterpret_cast<row_u4 *>(part + p * VEC - Piece::cut(p, dim) + i) =
+                    __builtin_bit_cast(row_u4, row_f4{dw[LATE ? 0 : j][i], dw[LATE ? 0 : j][i + 1], dw[LATE ? 0 : j][i + 2], dw[LATE ? 0 : j][i + 3]});
         }
     }
 }
@@ -383,10 +448,15 @@ static int norm_groups(int rows, int per) {
 }
 template <typename T, int TPR, int NP>
 static int norm_bw_launch(NormBw<T> &a, T *dw) {
-    const int grid = norm_groups<T>(a.rows, TPR == 64 ? 4 : 1);
-    if (dw && !(a.part = workspace((size_t)grid * a.dim * sizeof(float)))) return 2;
+    constexpr int per = TPR == 64 ? 4 : 1;
+    // Few rows: one workgroup writes dw itself, no second launch (3 x 4096 fp16 5.2 us, with it 7.7; of the longer rows, which wait for
+    // memory one by one, only one: 2 x 16384 8.0 us either way, 3 10.8 against 8.0).
+    constexpr int few = norm_ahead<T, TPR, NP>() ? 3 : 1;
+    const int grid = a.rows <= few * per ? 1 : norm_groups<T>(a.rows, per);
+    if (grid == 1) a.dw = dw;
+    else if (dw && !(a.part = workspace((size_t)grid * a.dim * sizeof(float)))) return 2;
     hipLaunchKernelGGL((rms_norm_bw_kernel<T, TPR, NP>), dim3(grid), dim3(TPR == 64 ? 256 : TPR), 0, state().stream, a);
-    if (dw) row_shares<T>(a.part, dw, a.dim, grid);
+    if (a.part) row_shares<T>(a.part, dw, a.dim, grid);
     return hip_ok(hipGetLastError(), "rms norm launch") ? 0 : 2;
 }
 
@@ -403,6 +473,9 @@ static int norm_bw(NormBw<T> &a, T *dw) {
     if (pieces <= 512) return norm_bw_launch<T, 256, 2>(a, dw);
     if (pieces <= 1024) return norm_bw_launch<T, 256, 4>(a, dw);
     if (pieces <= 2048) return norm_bw_launch<T, 512, 4>(a, dw);
+    if constexpr (sizeof(T) == 4) {  // (5946 x 8243 180 us, read twice 314; 300 x 16384 32 and 34)
+        if (pieces <= 4096) return norm_bw_launch<T, 1024, 4>(a, dw);
+    }
     const int shares = a.rows < 64 ? a.rows : 64;
     const size_t stat = (size_t)a.rows * 2;
     float *ws = workspace((stat + (dw ? (size_t)shares * a.dim : 0)) * sizeof(float));

@@ -218,3 +218,31 @@ def test_unaligned_tensors(pkg, gpu):
         pkg.call("ptl_rms_norm_%s_fw_batched" % dt, a, n)
         for got, ref in zip((T, Y, Q, C), forward(pkg, gpu, dt, x, skip, w)):
             assert torch.equal(got, ref)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,dim", [(2, 130), (3, 1001), (13, 515), (2, 2051), (4, 4099), (300, 9001), (5, 10001), (3, 12291), (1, 16383)])
+def test_rows_that_end_inside_a_piece(pkg, gpu, dt, n, dim):
+    """Up to a few rows (one workgroup has the weights' gradient) and many, forward and backward, also in the place of what is read."""
+    x, w, skip = tr.rand(dim, n, dim, dt=dt), 1 + tr.rand(dim + 1, dim, scale=0.2, dt=dt), tr.rand(dim + 2, n, dim, dt=dt)
+    T, Y, Q, C = forward(pkg, gpu, dt, x, skip, w)
+    check_forward(dt, x, skip, w, T, Y, Q, C)
+    X, S, W = tr.dev(x), tr.dev(skip), tr.dev(w)
+    a, keep = tr.norm_args(pkg, dim, x=X, skip=S, total=S, w=W, y=X)
+    pkg.call("ptl_rms_norm_%s_fw_batched" % dt, a, n)
+    assert torch.equal(S, T) and torch.equal(X, Y)
+    dy = tr.rand(dim + 3, n, dim, scale=0.5, dt=dt)
+    DX, DK, DW = backward(pkg, gpu, dt, x, dy, skip, w, 1)
+    check_backward(dt, x, dy, skip, w, DX, DK, DW)
+    for which in ("dy", "add", "s"):
+        S, DY, A = tr.dev(x), tr.dev(dy), tr.dev(skip)
+        out, dw = {"dy": DY, "add": A, "s": S}[which], torch.empty_like(W)
+        a, keep = tr.norm_args(pkg, dim, dx=out, dskip=out, total=S, dtotal=A, w=W, dw=dw, dy=DY)
+        pkg.call("ptl_rms_norm_%s_bw_batched" % dt, a, n)
+        assert torch.equal(out, DX) and torch.equal(dw, DW), which
+    # without the gradient along the residual, rows around the batch as they were
+    big = torch.full((n + 2, dim), 7.0, dtype=W.dtype, device="cuda")
+    a, keep = tr.norm_args(pkg, dim, x=tr.dev(x), dx=big[1:n + 1], w=W, dw=torch.empty_like(W), dy=tr.dev(dy))
+    pkg.call("ptl_rms_norm_%s_bw_batched" % dt, a, n)
+    check_backward(dt, x, dy, None, w, big[1:n + 1], None, None)
+    assert (big[0] == 7).all() and (big[n + 1] == 7).all()
