@@ -470,8 +470,10 @@ static void distill_rows(const DistillArgs<T> &a, int ns) {
 template <typename T>
 static int distill_launch(DistillArgs<T> &a, int ns) {
     const int pieces = (a.dim + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC, cu = state().num_cu;
-    // Too few rows for the chip, each long enough for two workgroups and more.
-    if (2L * ns <= cu && pieces > 2 * DISTILL_NT) {
+    // Rows in parts: a second launch costs 3 us, so rows have to be long and, where a workgroup holds one easily, few.  In parts and by
+    // the row, us: 32 of 24000 in fp16 9.7 and 8.0, of 50000 10.0 and 10.3, 64 10.7 and 11.0, 100 13.1 and 11.3; 100 of 131072 18.8 and
+    // 21.0; in fp32 32 of 50000 10.2 and 12.0, 64 13.9 and 13.1, of 131072 21.3 and 30.5, 128 35.5 and 36.3.
+    if (pieces > 4096 && (long)ns * (a.dim > 65536 ? 2 : 6) <= cu) {
         const int most = DISTILL_NT * DISTILL_NP;
         int parts = 2 * cu / ns, least = (pieces + most - 1) / most;
         parts = parts < (pieces + DISTILL_NT - 1) / DISTILL_NT ? parts : (pieces + DISTILL_NT - 1) / DISTILL_NT;

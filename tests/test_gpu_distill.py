@@ -158,3 +158,20 @@ def test_many_entries_named_twice(pkg, gpu, n, v, k):
     z, teacher, _ = case(n, n, v, k, "fp32")
     classes = torch.randint(0, v, (n, k), generator=g, dtype=torch.int32)
     check("fp32", z, teacher, classes, *run(pkg, gpu, "fp32", z, teacher, classes))
+
+
+@pytest.mark.parametrize("dt,n,v", [("fp16", 5, 40001), ("fp32", 130, 70001), ("fp16", 130, 131075)])
+def test_values_in_rows_that_no_workgroup_holds(pkg, gpu, dt, n, v):
+    """Few rows in parts, many that are walked: stretches of -inf at either end, one class left, a NaN; in the place of the logits."""
+    z, teacher, classes = case(v, n, v, 20, dt, empty=False)
+    z[0, :33000], z[1, 20000:] = -float("inf"), -float("inf")
+    z[2], z[2, v - 1] = -float("inf"), 1.5
+    classes[0] = torch.arange(20, dtype=torch.int32) + 34000
+    classes[1], classes[2] = torch.arange(20, dtype=torch.int32), v - 1
+    z[3, 9] = float("nan")
+    loss, grad = run(pkg, gpu, dt, z, teacher, classes)
+    keep = [i for i in range(n) if i != 3]
+    check(dt, z[keep], teacher[keep], classes[keep], loss[keep], grad[keep])
+    assert torch.isnan(loss[3]) and torch.isnan(grad[3]).all()
+    again, over = run(pkg, gpu, dt, z, teacher, classes, in_place=True)
+    assert torch.equal(again[keep], loss[keep]) and torch.equal(over[keep], grad[keep])

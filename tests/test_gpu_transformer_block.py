@@ -234,7 +234,7 @@ def growth_in_a_capture(what):
     assert gpu.ptl_init(0) == 0
     z = lambda *s: torch.zeros(*s, dtype=torch.float16, device="cuda")  # noqa: E731
     if what == "distill":  # the entries of 100 rows in parts: 6.5 MB
-        n, v, top = 100, 60000, 2048
+        n, v, top = 100, 70000, 2048
         a, keep = tr.distill_args(pkg, z(n, v), z(n, v), z(n, top), torch.zeros(n, top, dtype=torch.int32, device="cuda"),
                                   torch.zeros(n, device="cuda"), 1.0, 1.0)
         call = lambda: gpu.ptl_distill_fp16_batched(ctypes.byref(a), n, 2)  # noqa: E731
