@@ -7,7 +7,9 @@
  * Conventions are those of ptl_api.h, which includes this file: blobs describe ONE sample (a token) of `dim` elements,
  * sample n lies at data + n * dim; pointers may be host or device pointers; the calls return 0, 1 after rejecting their
  * arguments (message printed, outputs untouched) or 2 where a HIP call failed, and run on the library's stream.
- * nsamples <= 0 is an empty batch: nothing is read or written, 0 is returned.  Tensors a call writes must not overlap
+ * nsamples <= 0 is an empty batch: nothing is read or written, 0 is returned.  A call takes at most 2^30 samples, and a
+ * product as many outputs as 2^31 threads form (some 4 * 10^9 and more; 33 million outputs of a few tokens); larger ones
+ * are rejected.  Tensors a call writes must not overlap
  * those it reads or the other ones it writes except where a comment says so.
  */
 #ifndef PTL_TRANSFORMER_H

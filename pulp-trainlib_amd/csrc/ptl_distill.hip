@@ -32,7 +32,7 @@ struct DistillArgs {
     float *loss;  // (NULL: not wanted)
     float2 *part;  // of each part of a row: its largest logit, the sum of exponentials relative to that
     struct DistillEntry *entry;  // of each row, behind those: what the first launch finds out about the teacher's entries
-    int rows, dim, top, parts, per_part;  // per_part: pieces
+    int rows, first, dim, top, parts, per_part;  // first: the launch's first row; per_part: pieces
     float inv_t, hi, lo, least;  // 1 / T; log2(e) / T as the sum of two floats above 0; z - m from which on exp((z - m) / T) is 0
     float weight, scale;  // scale = weight / T
 };
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_row_kernel(const 
     extern __shared__ __attribute__((aligned(16))) float lds[];
     const int wave = NT == 64 ? (int)(threadIdx.x >> 6) : 0;
     const DistillTop t(lds + (size_t)wave * (DISTILL_RED + 5 * ((a.top + 3) & ~3)), a.top);
-    const size_t row = NT == 64 ? (size_t)blockIdx.x * 4 + wave : blockIdx.x;
+    const size_t row = a.first + (NT == 64 ? (size_t)blockIdx.x * 4 + wave : blockIdx.x);
     if (NT == 64 && row >= (size_t)a.rows) return;
     constexpr int VEC = RowPiece<T>::VEC, HELD = NP ? NP : 4;
     constexpr bool MINE = NP == 0;  // (the row is read behind what is written, which may be in its place)
@@ -462,9 +462,14 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_join_kernel(const DistillA
 }
 
 template <typename T, int NT, int NP>
-static void distill_rows(const DistillArgs<T> &a, int ns) {
-    if (NT == 64) hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3((ns + 3) / 4), dim3(256), 4 * distill_lds(a.top), state().stream, a);
-    else hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3(ns), dim3(NT), distill_lds(a.top), state().stream, a);
+static void distill_rows(DistillArgs<T> a, int ns) {
+    const int most = (int)(ROW_THREADS / NT);
+    for (; a.first < ns; a.first += most) {
+        const int n = ns - a.first < most ? ns - a.first : most;
+        a.rows = a.first + n;
+        if (NT == 64) hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3((n + 3) / 4), dim3(256), 4 * distill_lds(a.top), state().stream, a);
+        else hipLaunchKernelGGL((distill_row_kernel<T, NT, NP>), dim3(n), dim3(NT), distill_lds(a.top), state().stream, a);
+    }
 }
 
 template <typename T>
@@ -526,6 +531,7 @@ static int distill_step(const Args *a, int ns, int step, const char *fn) {
     if (!(fabsf(a->weight) < __builtin_inff())) return rows_bad(fn, "the weight is no finite number");
     const bool loss = step != 1, grad = step != 0;
     if (!a->output->data || !a->teacher || !a->classes || (loss && !a->wr_loss) || (grad && !a->output->diff)) return rows_bad(fn, "null buffer");
+    if (ns > ROW_MOST) return rows_bad(fn, "more than 2^30 samples");
     if (ns <= 0) return 0;
     if (!ensure_init()) return 2;
     const size_t n = (size_t)ns * dim, k = (size_t)ns * top;

@@ -115,6 +115,7 @@ static int gated_step(const Args *a, int ns, bool back, const char *fn) {
     if (a->activation < PTL_GATE_SIGMOID || a->activation > PTL_GATE_RELU) return rows_bad(fn, "unknown activation");
     const bool bias = a->use_biases == 1;
     if (bias && !a->bias) return rows_bad(fn, "use_biases=1 with a null bias blob");
+    if (ns > ROW_MOST) return rows_bad(fn, "more than 2^30 samples");
     if (ns <= 0) return 0;
     auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
     const size_t nx = (size_t)ns * in, ny = (size_t)ns * outs, nw = (size_t)2 * outs * in;

@@ -12,7 +12,7 @@ int rows_int8(RowsArgs &a) {
 template <typename OUT, typename Args>
 static int mm_int8_step(const Args *a, const char *fn) {
     if (!a) return rows_bad(fn, "null argument structure");
-    if (a->N < 0 || a->M <= 0 || a->K <= 0 || a->M > ROW_MOST) return rows_bad(fn, "invalid matrix geometry");
+    if (a->N < 0 || a->N > ROW_MOST || a->M <= 0 || a->K <= 0 || a->M > ROW_MOST) return rows_bad(fn, "invalid matrix geometry");
     if (a->K > 131071) return rows_bad(fn, "sums of more than 131071 products of 8-bit integers do not fit 32 bits");
     const bool bias = a->USE_BIASES == 1;
     if (!a->A || !a->B || !a->C || (bias && !a->bias)) return rows_bad(fn, "null buffer");

@@ -22,6 +22,7 @@ struct NormFw {
     int8_t *q;
     float *scale;
     int rows, dim;
+    int first;  // the launch's first row
     float eps;
 };
 
@@ -50,7 +51,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     constexpr bool SHORT = TPR * NP == 64;  // rows of less than a piece come here too
     __shared__ float red[16][2];
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x;
-    const long row = TPR == 64 ? (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
+    const long row = a.first + (TPR == 64 ? (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x);
     if (row >= a.rows) return;  // (a whole wave, which has no barrier to meet)
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     const size_t at = (size_t)row * dim;
@@ -159,10 +160,15 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
 }
 
 template <typename T, int TPR, int NP>
-static void norm_fw_launch(const NormFw<T> &a) {
-    const dim3 grid(TPR == 64 ? (a.rows + 3) / 4 : a.rows), block(TPR == 64 ? 256 : TPR);
-    if (a.q) hipLaunchKernelGGL((rms_norm_fw_kernel<T, TPR, NP, true>), grid, block, 0, state().stream, a);
-    else hipLaunchKernelGGL((rms_norm_fw_kernel<T, TPR, NP, false>), grid, block, 0, state().stream, a);
+static void norm_fw_launch(NormFw<T> a) {
+    const int all = a.rows, most = (int)(ROW_THREADS / TPR);
+    for (; a.first < all; a.first += most) {
+        const int n = all - a.first < most ? all - a.first : most;
+        a.rows = a.first + n;
+        const dim3 grid(TPR == 64 ? (n + 3) / 4 : n), block(TPR == 64 ? 256 : TPR);
+        if (a.q) hipLaunchKernelGGL((rms_norm_fw_kernel<T, TPR, NP, true>), grid, block, 0, state().stream, a);
+        else hipLaunchKernelGGL((rms_norm_fw_kernel<T, TPR, NP, false>), grid, block, 0, state().stream, a);
+    }
 }
 
 template <typename T>
@@ -191,6 +197,7 @@ struct NormBw {
     float *part;  // of dw: a row for each workgroup (NULL: not wanted)
     float *stat;  // long rows: r and r^3 mean(g s) of each row
     int rows, dim;
+    int first;  // of the rows whose statistics a launch forms
     float eps;
 };
 
@@ -387,7 +394,7 @@ __global__ __launch_bounds__(1024) void rms_norm_stat_kernel(const NormBw<T> a) 
     constexpr int VEC = Piece::VEC;
     __shared__ float red[16][2];
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
-    const size_t at = (size_t)blockIdx.x * dim;
+    const size_t row = (size_t)a.first + blockIdx.x, at = row * dim;
     float v[2] = {0.f, 0.f};
     for (int p = threadIdx.x; p < pieces; p += 1024) {
         Piece s, g, w;
@@ -403,8 +410,8 @@ __global__ __launch_bounds__(1024) void rms_norm_stat_kernel(const NormBw<T> a) 
     row_reduce<1024, 2>(v, red);
     if (threadIdx.x == 0) {
         const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps);
-        a.stat[2 * (size_t)blockIdx.x] = r;
-        a.stat[2 * (size_t)blockIdx.x + 1] = r * r * r * (v[1] / (float)dim);
+        a.stat[2 * row] = r;
+        a.stat[2 * row + 1] = r * r * r * (v[1] / (float)dim);
     }
 }
 template <typename T>
@@ -482,7 +489,9 @@ static int norm_bw(NormBw<T> &a, T *dw) {
     if (!ws) return 2;
     a.stat = ws;
     a.part = dw ? ws + stat : nullptr;
-    hipLaunchKernelGGL((rms_norm_stat_kernel<T>), dim3(a.rows), dim3(1024), 0, state().stream, a);
+    constexpr int most = (int)(ROW_THREADS / 1024);
+    for (a.first = 0; a.first < a.rows; a.first += most)
+        hipLaunchKernelGGL((rms_norm_stat_kernel<T>), dim3(a.rows - a.first < most ? a.rows - a.first : most), dim3(1024), 0, state().stream, a);
     hipLaunchKernelGGL((rms_norm_columns_kernel<T>), dim3((pieces + 255) / 256, shares), dim3(256), 0, state().stream, a);
     if (dw) row_shares<T>(a.part, dw, a.dim, shares);
     return hip_ok(hipGetLastError(), "rms norm launch") ? 0 : 2;
@@ -494,6 +503,7 @@ static int rms_norm_step(const Args *a, int ns, bool back, const char *fn) {
     const int dim = a->input->dim;
     if (dim <= 0 || dim > ROW_MOST) return rows_bad(fn, "invalid tensor geometry");
     if (!(a->eps >= 0.f && a->eps < __builtin_inff())) return rows_bad(fn, "eps is no finite number from 0 on");
+    if (ns > ROW_MOST) return rows_bad(fn, "more than 2^30 samples");
     if (ns <= 0) return 0;
     auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
     T *w = as(a->coeff->data), *sum = as(blob_data(a->sum)), *x = as(a->input->data);

@@ -91,7 +91,8 @@ struct RowPiece {
     }
 };
 
-constexpr int ROW_MOST = 1 << 30;  // elements of a row
+constexpr int ROW_MOST = 1 << 30;  // elements of a row, rows of a call
+constexpr long ROW_THREADS = 1l << 31;  // of a launch (it takes 2^32 - 1; calls with more rows are several launches)
 
 // Sums (and maxima) of N values over the 64 lanes of a wave, the same in every lane.
 __device__ inline float wave_sum(float v) {
@@ -132,7 +133,7 @@ __device__ inline void row_reduce(float (&v)[N], float (*lds)[N]) {
 // flight, so that a few thousand columns fill the chip (1024 shares of 4096: 18 us with 64 columns and 4 shares at a time, 5 so).
 template <typename T>
 __global__ __launch_bounds__(1024) void row_shares_kernel(const float *__restrict__ part, T *__restrict__ out, int dim, int shares) {
-    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, c = blockIdx.x * 32 + o;
+    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, c = (int)(blockIdx.y * gridDim.x + blockIdx.x) * 32 + o;
     LongSum<T> s;
     s.clear();
     if (c < dim) {
@@ -155,7 +156,9 @@ __global__ __launch_bounds__(1024) void row_shares_kernel(const float *__restric
 }
 template <typename T>
 inline void row_shares(const float *part, T *out, int dim, int shares) {
-    hipLaunchKernelGGL((row_shares_kernel<T>), dim3((dim + 31) / 32), dim3(1024), 0, state().stream, part, out, dim, shares);
+    const int groups = (dim + 31) / 32, most = (int)(ROW_THREADS / 1024);  // (the last of several rows of the grid may reach beyond the end)
+    hipLaunchKernelGGL((row_shares_kernel<T>), dim3(groups < most ? groups : most, (groups + most - 1) / most), dim3(1024), 0, state().stream, part, out, dim,
+                       shares);
 }
 
 // A rejected call: its message, as the other entry points give it.

@@ -162,3 +162,22 @@ def test_no_device_is_reported(pkg):
     a, keep = tr.int8_args(pkg, A, A, C)
     assert pkg.load().ptl_mm_int8_fp32(ctypes.byref(a)) == 2
     assert b"no CPU fallback" in pkg.load().ptl_last_error() and (C == 7).all()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+def test_more_samples_than_a_call_takes(pkg, dt):
+    t = np.float32 if dt == "fp32" else np.float16
+    many = 2 ** 30 + 1
+    x, w, y = np.ones((2, 8), t), np.ones(8, t), np.full((2, 8), 7, t)
+    a, keep = tr.norm_args(pkg, 8, x=x, w=w, y=y, dx=y, dw=w, dy=x)
+    refused(pkg, "ptl_rms_norm_%s_fw_batched" % dt, a, many, says="2^30")
+    refused(pkg, "ptl_rms_norm_%s_bw_batched" % dt, a, many, says="2^30")
+    a, keep = tr.gated_args(pkg, 8, 4, 1, x=x, w=x.repeat(4, 0), y=y, h=y)
+    refused(pkg, "ptl_gated_linear_%s_fw_batched" % dt, a, many, says="2^30")
+    refused(pkg, "ptl_gated_linear_%s_bw_batched" % dt, a, many, says="2^30")
+    a, keep = tr.distill_args(pkg, x, y, x, np.zeros((2, 8), np.int32), np.full(2, 7, np.float32), 1.0, 1.0)
+    refused(pkg, "ptl_distill_%s_batched" % dt, a, many, 2, says="2^30")
+    a, keep = tr.int8_args(pkg, np.ones((3, 4), np.int8), np.ones((5, 4), np.int8), y)
+    a.N = many
+    refused(pkg, "ptl_mm_int8_" + dt, a, says="geometry")
+    assert (y == 7).all()
