@@ -34,6 +34,11 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
             const float df = gate.back((float)g.e[i], f);
             og.e[i] = (T)((float)d.e[i] * (float)u.e[i] * df);
             ou.e[i] = (T)((float)d.e[i] * f);
+        }
+        // (the sums are of the values that are stored: formed again for them, with other roundings in between, one in thousands would differ)
+        asm volatile("" : "+v"(og.raw), "+v"(ou.raw));
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
             sum[0][i] += (float)og.e[i];
             sum[1][i] += (float)ou.e[i];
         }

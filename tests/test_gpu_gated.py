@@ -225,3 +225,12 @@ def test_backward_own_products(pkg, gpu, n, n_in, n_out, bias):
     dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, skip_wg=1)
     check_backward("fp16", "silu", x, w, h, dy, dh, dx, None, None)
     assert (dw == 7).all() and (db is None or (db == 7).all())
+
+
+def test_bias_gradients_are_sums_of_what_is_stored(pkg, gpu):
+    """64 tokens, so that a single value rounded another way than it is stored shows in the sum."""
+    n, n_in, n_out = 64, 2048, 1600
+    x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    for act in ("silu", "gelu", "sigmoid", "relu"):
+        check_backward("fp16", act, x, w, h, dy, *backward(pkg, gpu, "fp16", act, x, w, h, dy, 1))
