@@ -10,10 +10,11 @@ int rows_gated(RowsArgs &a) {
 }
 
 // dh = (dy h_up act'(h_gate), dy act(h_gate)): three values read, two written, nothing else (2048 x 5632 in fp16 21 us, 5.5 TB/s).  dh
-// may be h.  part: sums of dh over the rows of a grid row, as it is stored (NULL: not wanted).
+// may be h.  part: sums of dh over the rows of a grid row, as it is stored (NULL: not wanted).  copy: dh in rows of `pitch` values, zeros
+// behind (NULL: not wanted).
 template <typename T>
 __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__restrict__ dy, T *dh, float *__restrict__ part, size_t rows, int outs,
-                                                        int act) {
+                                                        int act, T *__restrict__ copy, int pitch) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC;
     const int pieces = (outs + VEC - 1) / VEC, p = (int)(blockIdx.x * 256 + threadIdx.x);
@@ -44,6 +45,12 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
         }
         og.store(dh + row * 2 * outs, p, outs);
         ou.store(dh + row * 2 * outs + outs, p, outs);
+        if (copy) {
+            T *to = copy + row * pitch;
+            og.store(to, p, outs);
+            ou.store(to + outs, p, outs);
+            for (int i = 2 * outs + p; p < 8 && i < pitch; i += pieces) to[i] = (T)0.f;
+        }
     }
     if (!part) return;
     float *to = part + (size_t)blockIdx.y * 2 * outs;
@@ -58,14 +65,14 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
 static int linear_bw(const ::Linear_args *l, int ns) { return ptl_linear_fp32_bw_batched(l, ns); }
 static int linear_bw(const ::Linear_args_fp16 *l, int ns) { return ptl_linear_fp16_bw_batched(l, ns); }
 
-// Which backward calls have both products made by gated_products(): whole 16-byte pieces, from 1.5 GFLOP on (of 60 layers of 64 to 8192
-// tokens 0.84 to 1.62 times as fast as a dense layer's call, 1.17 in the mean; below, 64 tokens, 512 -> 1408 and 512 tokens, 256 -> 512,
-// 0.91 and 0.82).
+// Which backward calls have both products made by gated_products(): from 1.5 GFLOP on (of 60 layers of 64 to 8192 tokens 0.84 to 1.62
+// times as fast as a dense layer's call, 1.17 in the mean; below, 64 tokens, 512 -> 1408 and 512 tokens, 256 -> 512, 0.91 and 0.82), from
+// 3 where operands have to be copied to rows of whole 16-byte pieces (16 layers 0.93 to 1.99, 1.26 in the mean: 3549 tokens,
+// 1748 -> 1216 198 -> 100 us, 2048 tokens, 2047 -> 5631 390 -> 252; 7 layers below 0.69 to 1.0).
 template <typename T>
-static bool own_products(const T *x, const T *w, const T *dh, int ns, int in, int outs) {
-    const uintptr_t all = (uintptr_t)x | (uintptr_t)w | (uintptr_t)dh | (uintptr_t)in * 2 | (uintptr_t)outs * 4;
+static bool own_products(int ns, int in, int outs, bool copied) {
     const bool fits = in < 1 << 23 && outs < 1 << 22;  // (64 rows of the first operand and 128 of the second within 32 bits)
-    return sizeof(T) == 2 && fits && all % 16 == 0 && 8.0 * ns * in * outs >= 1.5e9 && state().gemm_path == 0;
+    return sizeof(T) == 2 && fits && 8.0 * ns * in * outs >= (copied ? 3e9 : 1.5e9) && state().gemm_path == 0;
 }
 
 template <typename T, typename Linear, typename Args>
@@ -81,7 +88,21 @@ static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool w
         T *dw = wg ? sg.out<T>(as(a->coeff->diff), nw) : nullptr, *dx = ig ? sg.out<T>(as(a->input->diff), nx) : nullptr;
         T *db = wg && bias ? sg.out<T>(as(a->bias->diff), (size_t)2 * outs) : nullptr;
         if (sg.failed()) return 2;
-        const bool own = own_products<T>(x, w, dh, ns, in, outs);
+        // rows that are no whole 16-byte pieces are copied to such; dh is written a second time
+        const int cols = (in + 7) / 8 * 8, pitch = (2 * outs + 7) / 8 * 8;
+        bool copy_x = ((uintptr_t)x | (uintptr_t)w) % 16 || cols != in, copy_dh = (uintptr_t)dh % 16 || pitch != 2 * outs;
+        const bool own = own_products<T>(ns, in, outs, copy_x || copy_dh);
+        copy_x = copy_x && own;
+        copy_dh = copy_dh && own;
+        T *wide_w = nullptr, *wide_x = nullptr, *wide_dh = nullptr;
+        if (copy_x || copy_dh) {
+            const size_t n_w = copy_x && w ? (size_t)2 * outs * cols : 0, n_x = copy_x && x ? (size_t)ns * cols : 0, n_dh = copy_dh ? (size_t)ns * pitch : 0;
+            wide_w = static_cast<T *>(scratch((n_w + n_x + n_dh) * sizeof(T)));
+            if (!wide_w) return 2;
+            wide_x = wide_w + n_w;
+            if (copy_dh) wide_dh = wide_x + n_x;
+            if (n_w + n_x) rows_copy(w, w ? 2 * (size_t)outs : 0, x, x ? ns : 0, wide_w, in * (int)sizeof(T), cols * (int)sizeof(T));
+        }
         const int wide = ((outs + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC + 255) / 256;
         int high = ns < 65535 ? ns : 65535;
         float *part = nullptr;
@@ -90,11 +111,13 @@ static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool w
             high = high < most ? high : most;
             if (!(part = workspace((size_t)high * 2 * outs * sizeof(float)))) return 2;
         }
-        hipLaunchKernelGGL((gate_back_kernel<T>), dim3(wide, high), dim3(256), 0, state().stream, h, dy, dh, part, (size_t)ns, outs, a->activation);
+        hipLaunchKernelGGL((gate_back_kernel<T>), dim3(wide, high), dim3(256), 0, state().stream, h, dy, dh, part, (size_t)ns, outs, a->activation,
+                           wide_dh, pitch);
         if (part) row_shares<T>(part, db, 2 * outs, high);
         int rc = hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
         if constexpr (sizeof(T) == 2) {
-            if (rc == 0 && own && (wg || ig)) rc = gated_products(x, w, dh, dw, dx, ns, in, 2 * outs);
+            if (rc == 0 && own && (wg || ig))
+                rc = gated_products(copy_x ? wide_x : x, copy_x ? wide_w : w, copy_dh ? wide_dh : dh, dw, dx, ns, in, 2 * outs, cols, pitch);
         }
         rc = sg.finish(rc);
         if (rc || own || !(wg || ig)) return rc;

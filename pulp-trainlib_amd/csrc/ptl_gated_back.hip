@@ -10,6 +10,7 @@
 //   * Where that leaves compute units idle k is cut into parts, each with sums of its own in fp32, which another launch adds up.
 // 2048 tokens, 2048 -> 5632: 210 us (900 TFLOP/s; with the gradients of the pre-activations 231), as a dense layer's call 245;
 // 256 tokens of the same layer 58 and 82, 64 tokens 31 and 49.
+// Rows that are no whole 16-byte pieces come as copies (rows_copy(), gate_back_kernel): 2047 -> 5631 252 us with them.
 // Tried: slabs of 32 k, four of them in flight, instead of two of 64: 3 to 8 % longer.
 #include "ptl_rows_mm.inc"
 
@@ -29,6 +30,7 @@ struct GradProd {
     RowsArgs out;       // y, outs (the inputs), tokens (rows of the second operand), tiles; no scales and biases
     const char *f, *s;  // first operand: k rows of outs values; second one: its rows of k values, or k rows of them
     int k, f_b, s_b;    // k, bytes of a row of either
+    int f_n, s_n;       // rows that have values of their own in [k][row] tiles: whole eights
     int parts, chunk;   // k in parts of so many slabs, each with its own sums in fp32 (part) where there are more than one
     float *part;
 };
@@ -54,6 +56,9 @@ __device__ inline uint4 grad_frag(const char *tile, int block, int lane, int chu
     return t.v;
 }
 
+// Floats between the sums of two parts: whole fours.
+__host__ __device__ inline size_t grad_part(int tokens, int outs) { return ((size_t)tokens * outs + 3) & ~(size_t)3; }
+
 // ROWS: the second operand has k along its rows.
 template <bool ROWS>
 __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
@@ -78,14 +83,14 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
         const int k = kk + j * 16;
-        f_off[j] = (unsigned)k * (unsigned)g.f_b + (unsigned)min(at, (a.outs - o0) / 8 - 1) * 16u;
+        f_off[j] = (unsigned)k * (unsigned)g.f_b + (unsigned)min(at, (g.f_n - o0) / 8 - 1) * 16u;
         f_none[j] = k >= tail;
         if constexpr (ROWS) {
             const int r = (j * NT + tid) >> 3, pos = (tid & 7) ^ swz(r);
             s_off[j] = (unsigned)min(r, a.tokens - 1 - t0) * (unsigned)g.s_b + (unsigned)pos * 16u;
             s_none[j] = pos * 8 >= tail;
         } else {
-            s_off[j] = (unsigned)k * (unsigned)g.s_b + (unsigned)min(at, (a.tokens - t0) / 8 - 1) * 16u;
+            s_off[j] = (unsigned)k * (unsigned)g.s_b + (unsigned)min(at, (g.s_n - t0) / 8 - 1) * 16u;
             s_none[j] = k >= tail;
         }
     }
@@ -149,7 +154,7 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
     __syncthreads();
     if (g.parts > 1) {
         RowsArgs p = a;
-        p.y = g.part + (size_t)z * a.tokens * a.outs;
+        p.y = g.part + (size_t)z * grad_part(a.tokens, a.outs);
         rows_behind<P>(p, acc, o0, t0, ww, wt, lane, w_tab, b_tab, x_tab, smem + P::TABLE + wave * 32 * P::PITCH);
     } else {
         rows_behind<C>(a, acc, o0, t0, ww, wt, lane, w_tab, b_tab, x_tab, smem + C::TABLE + wave * 32 * C::PITCH);
@@ -167,7 +172,7 @@ __global__ __launch_bounds__(GradTile<half_t>::NT) void grad_kernel(const GradAr
 struct GradJoin {
     const float *part[2];
     half_t *y[2];
-    size_t n[2];  // values / 4 (0: not in parts)
+    size_t n[2], values[2];  // fours of values (0: not in parts), values
     int parts[2];
 };
 __global__ __launch_bounds__(256) void grad_join_kernel(const GradJoin a) {
@@ -185,7 +190,12 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const GradJoin a) {
         s.w += v.w;
     }
     typedef half_t h4 __attribute__((ext_vector_type(4)));
-    reinterpret_cast<h4 *>(a.y[o])[i] = h4{(half_t)s.x, (half_t)s.y, (half_t)s.z, (half_t)s.w};
+    const h4 v = h4{(half_t)s.x, (half_t)s.y, (half_t)s.z, (half_t)s.w};
+    if (4 * i + 4 <= a.values[o]) {
+        reinterpret_cast<h4 *>(a.y[o])[i] = v;
+    } else {
+        for (int e = 0; 4 * i + e < a.values[o]; ++e) a.y[o][4 * i + e] = v[e];
+    }
 }
 
 // Microseconds of the launch with k of the two products in so many parts: a workgroup takes 0.95 a slab while it shares its compute
@@ -210,7 +220,7 @@ static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const doubl
     return (spread > longest ? spread : longest) + (extra > 0 ? extra + 4.f : 0.f);
 }
 
-int gated_products(const half_t *x, const half_t *w, const half_t *dh, half_t *dw, half_t *dx, int ns, int in, int rows) {
+int gated_products(const half_t *x, const half_t *w, const half_t *dh, half_t *dw, half_t *dx, int ns, int in, int rows, int cols, int pitch) {
     static bool ready = false;
     constexpr int RING = GradTile<half_t>::RING;
     if (!ready) {
@@ -252,11 +262,13 @@ int gated_products(const half_t *x, const half_t *w, const half_t *dh, half_t *d
         p.f = reinterpret_cast<const char *>(i ? x : w);
         p.s = reinterpret_cast<const char *>(dh);
         p.k = k[i];
-        p.f_b = in * 2;
-        p.s_b = rows * 2;
+        p.f_b = cols * 2;
+        p.s_b = pitch * 2;
+        p.f_n = cols;
+        p.s_n = pitch;
         p.chunk = (slabs[i] + parts[i] - 1) / parts[i];
         p.parts = (slabs[i] + p.chunk - 1) / p.chunk;
-        if (p.parts > 1) floats += (size_t)p.parts * n[i] * in;
+        if (p.parts > 1) floats += (size_t)p.parts * grad_part(n[i], in);
     }
     if (floats) {
         float *ws = workspace(floats * sizeof(float));
@@ -266,9 +278,10 @@ int gated_products(const half_t *x, const half_t *w, const half_t *dh, half_t *d
             a.p[i].part = ws;
             j.part[i] = ws;
             j.y[i] = y[i];
-            j.n[i] = (size_t)n[i] * in / 4;
+            j.values[i] = (size_t)n[i] * in;
+            j.n[i] = grad_part(n[i], in) / 4;
             j.parts[i] = a.p[i].parts;
-            ws += (size_t)a.p[i].parts * n[i] * in;
+            ws += (size_t)a.p[i].parts * grad_part(n[i], in);
         }
     }
     a.lead = a.p[0].chunk >= a.p[1].chunk ? 0 : 1;
@@ -280,6 +293,10 @@ int gated_products(const half_t *x, const half_t *w, const half_t *dh, half_t *d
         hipLaunchKernelGGL(grad_join_kernel, dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, state().stream, j);
     }
     return hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
+}
+
+void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, int bytes, int pitch) {
+    rows_copies(static_cast<const char *>(w), n_w, static_cast<const char *>(x), n_x, static_cast<char *>(to), bytes, pitch);
 }
 
 }  // namespace ptl

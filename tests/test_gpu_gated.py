@@ -234,3 +234,40 @@ def test_bias_gradients_are_sums_of_what_is_stored(pkg, gpu):
     h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
     for act in ("silu", "gelu", "sigmoid", "relu"):
         check_backward("fp16", act, x, w, h, dy, *backward(pkg, gpu, "fp16", act, x, w, h, dy, 1))
+
+
+@pytest.mark.parametrize("n,n_in,n_out,bias", [(500, 1100, 2050, 1), (701, 1001, 1003, 1), (3001, 83, 1701, 0), (64, 2045, 3001, 1), (9000, 130, 321, 1)])
+def test_backward_own_products_of_odd_sizes(pkg, gpu, n, n_in, n_out, bias):
+    """Layers from 3 GFLOP on whose rows are no whole 16-byte pieces: the operands as copies, each gradient alone, in place."""
+    x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    full = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias)
+    check_backward("fp16", "silu", x, w, h, dy, *full)
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, over=1)
+    assert all(a is None or torch.equal(a, b) for a, b in zip((dh, dx, dw, db), full))
+    dh, dx, dw, _ = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, skip_wg=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, dx, None, None)
+    assert (dw == 7).all()
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, bias, skip_ig=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, None, dw, db)
+    assert (dx == 7).all()
+
+
+def test_backward_own_products_of_unaligned_tensors(pkg, gpu):
+    """Whole pieces that do not start on 16 bytes; what lies behind the gradients stays as it is."""
+    n, n_in, n_out = 600, 1024, 1024
+    x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+
+    def off(t, fill=None):
+        b = torch.full((t.numel() + 2,), 7, dtype=torch.float16, device="cuda")
+        if fill is None:
+            b[1:-1] = t.flatten().cuda()
+        return b, b[1:-1].view(t.shape)
+    (_, X), (_, W), (_, H), (_, DY) = off(x), off(w), off(h), off(dy)
+    (bx, dx), (bw, dw), (bh, dh) = off(x, 7), off(w, 7), off(h, 7)
+    a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=X, dx=dx, w=W, dw=dw, h=H, dh=dh, dy=DY)
+    pkg.call("ptl_gated_linear_fp16_bw_batched", a, n)
+    assert gpu.ptl_sync() == 0
+    check_backward("fp16", "silu", x, w, h, dy, dh, dx, dw, None)
+    assert all(b[0] == 7 and b[-1] == 7 for b in (bx, bw, bh))
