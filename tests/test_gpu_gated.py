@@ -202,8 +202,8 @@ def test_host_arrays(pkg, gpu):
                                                   ("fp16", 40, 1026, 300, 32032), ("fp16", 700, 512, 600, 64064), ("fp16", 700, 511, 600, 64064),
                                                   ("fp16", 700, 510, 600, 64064), ("fp16", 1500, 1024, 1100, 128128), ("fp16", 2100, 1025, 1500, 128128),
                                                   ("fp16", 2048, 1024, 2100, 256256), ("fp16", 2048, 1021, 2100, 256256), ("fp32", 4, 600, 300, 0),
-                                                  ("fp32", 40, 1024, 100, 32032), ("fp32", 40, 1023, 1000, 32032), ("fp32", 900, 256, 900, 64064),
-                                                  ("fp32", 900, 255, 900, 64064)])
+                                                  ("fp32", 40, 1024, 100, 32032), ("fp32", 40, 1023, 1000, 32032), ("fp32", 900, 256, 900, 32064),
+                                                  ("fp32", 900, 255, 900, 32064), ("fp32", 2000, 600, 900, 64128), ("fp32", 2001, 601, 901, 64128)])
 def test_every_kernel(pkg, gpu, dt, n, n_in, n_out, tile):
     """Each kernel on sizes that it is chosen for, the ones that copy rows first among them (1021 and 1025 inputs)."""
     x, w, b = inputs(n, dt, n, n_in, n_out, 1)
