@@ -7,7 +7,7 @@
 // for the way back: s is read there anyway, and its sum of squares comes with the other sum of the row.
 // A row of up to 2048 bytes (4096 backward, in fp32) has a wave of its own (no barrier), a longer one a workgroup; rows that no workgroup
 // holds (more than 4096 pieces of 16 bytes forward, 16384 values backward) are read twice.  Measured, with the residual's addition: 8192 rows of
-// 4096 fp16 values forward 45 us, 5.9 TB/s (in 8 bits 42 us), backward with the weights' gradient 62 us, 5.4 TB/s of five tensors;
+// 4096 fp16 values forward 45 us, 5.9 TB/s (in 8 bits 42 us), backward with the weights' gradient 62 us, 4.3 TB/s;
 // 8192 x 1024 14 and 23 us; a few rows 3.7 us, which is an empty launch, and backward 4 us for one to three,
 // 7.3 for the two launches of more.
 #include "ptl_rows.hpp"
