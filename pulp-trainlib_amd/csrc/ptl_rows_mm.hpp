@@ -18,6 +18,8 @@ struct RowsArgs {
     const char *zeros;  // 16 zero bytes
     int act;
     int tiles_w, tiles_t;
+    int parts;   // 32 x 32 tiles: workgroups that share a tile's k, each with sums of its own in ...
+    void *part;  // ... parts x tiles x 16 x 64 (the lanes' accumulators)
 };
 
 // The activations of a gated layer, all but the last as m sigmoid(p): silu m = p = x, sigmoid m = 1, p = x, and gelu m = x,

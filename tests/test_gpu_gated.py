@@ -271,3 +271,16 @@ def test_backward_own_products_of_unaligned_tensors(pkg, gpu):
     assert gpu.ptl_sync() == 0
     check_backward("fp16", "silu", x, w, h, dy, dh, dx, dw, None)
     assert all(b[0] == 7 and b[-1] == 7 for b in (bx, bw, bh))
+
+
+@pytest.mark.parametrize("dt,n,n_in,n_out", [("fp32", 16, 3000, 1000), ("fp32", 70, 2001, 35), ("fp32", 500, 4096, 64), ("fp32", 8, 8193, 16), ("fp16", 20, 4097, 300),
+                                             ("fp16", 64, 8192, 1024), ("fp16", 33, 8001, 70)])
+def test_few_outputs_of_long_rows(pkg, gpu, dt, n, n_in, n_out):
+    """k in parts of several workgroups each, with sums that another launch adds up; the same bits in every call."""
+    x, w, b = inputs(n, dt, n, n_in, n_out, 1)
+    y, h = forward(pkg, gpu, dt, "silu", x, w, b)
+    check_forward(dt, "silu", x, w, b, y, h)
+    again, none = forward(pkg, gpu, dt, "silu", x, w, b, keep=0)
+    assert torch.equal(again, y) and none is None
+    y, h = forward(pkg, gpu, dt, "gelu", x, w, None)
+    check_forward(dt, "gelu", x, w, None, y, h)

@@ -113,3 +113,17 @@ def test_every_kernel(pkg, gpu, n, m, k, tile):
     sa, sb = tr.rand(1, n).abs() * 0.001 + 0.0001, tr.rand(2, m).abs() * 0.02 + 0.001
     check(pkg, gpu, "fp16", A, B, sa, sb, tr.rand(3, m, dt="fp16"))
     assert gpu.ptl_last_gemm_tile() == tile
+
+
+@pytest.mark.parametrize("n,m,k", [(64, 2048, 8193), (20, 100, 65537), (8, 256, 131071), (500, 64, 30000)])
+def test_few_outputs_of_long_rows(pkg, gpu, n, m, k):
+    """k in parts of several workgroups each: the sums stay exact."""
+    A, B = ints(n, n, k), ints(m, m, k)
+    check(pkg, gpu, "fp16", A, B, tr.rand(1, n).abs() * 1e-4 + 1e-5, tr.rand(2, m).abs() * 0.02 + 0.001, tr.rand(3, m, dt="fp16"))
+    if n < 100:
+        A, B = torch.full((n, k), -128, dtype=torch.int8), torch.full((m, k), -128, dtype=torch.int8)
+        B[::3, : k // 2] = 127
+        C = check(pkg, gpu, "fp32", A, B, None, None, None)
+        # rows alike: two sums, each formed by hand
+        whole, half = 16384 * k, -128 * 127 * (k // 2) + 16384 * (k - k // 2)
+        assert (C[:, 1::3] == float(torch.tensor(whole).float())).all() and (C[:, ::3] == float(torch.tensor(half).float())).all()
