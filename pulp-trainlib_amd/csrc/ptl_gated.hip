@@ -65,14 +65,18 @@ __global__ __launch_bounds__(256) void gate_back_kernel(const T *h, const T *__r
 static int linear_bw(const ::Linear_args *l, int ns) { return ptl_linear_fp32_bw_batched(l, ns); }
 static int linear_bw(const ::Linear_args_fp16 *l, int ns) { return ptl_linear_fp16_bw_batched(l, ns); }
 
-// Which backward calls have both products made by gated_products(): from 1.5 GFLOP on (of 60 layers of 64 to 8192 tokens 0.84 to 1.62
+// Which backward calls have both products made by gated_products().  fp16: from 1.5 GFLOP on (of 60 layers of 64 to 8192 tokens 0.84 to 1.62
 // times as fast as a dense layer's call, 1.17 in the mean; below, 64 tokens, 512 -> 1408 and 512 tokens, 256 -> 512, 0.91 and 0.82), from
 // 3 where operands have to be copied to rows of whole 16-byte pieces (16 layers 0.93 to 1.99, 1.26 in the mean: 3549 tokens,
-// 1748 -> 1216 198 -> 100 us, 2048 tokens, 2047 -> 5631 390 -> 252; 7 layers below 0.69 to 1.0).
+// 1748 -> 1216 198 -> 100 us, 2048 tokens, 2047 -> 5631 390 -> 252; 7 layers below 0.69 to 1.0).  fp32: from 5 GFLOP on, and with 16 tokens
+// and more where the weights are large (110 layers, copies or not: 52 that qualify 0.9 to 2.1 times as fast, 1.19 in the mean - 111
+// tokens, 3300 -> 6400 370 -> 199 us, 32, 2304 -> 2880 65 -> 41 -, the others 0.66 to 1.39).
 template <typename T>
 static bool own_products(int ns, int in, int outs, bool copied) {
     const bool fits = in < 1 << 23 && outs < 1 << 22;  // (64 rows of the first operand and 128 of the second within 32 bits)
-    return sizeof(T) == 2 && fits && 8.0 * ns * in * outs >= (copied ? 3e9 : 1.5e9) && state().gemm_path == 0;
+    const double flops = 8.0 * ns * in * outs, weights = (double)in * outs;
+    const bool pays = sizeof(T) == 4 ? flops >= 5e9 || (ns >= 16 && weights >= 2.5e6) : flops >= (copied ? 3e9 : 1.5e9);
+    return fits && pays && state().gemm_path == 0;
 }
 
 template <typename T, typename Linear, typename Args>
@@ -89,7 +93,8 @@ static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool w
         T *db = wg && bias ? sg.out<T>(as(a->bias->diff), (size_t)2 * outs) : nullptr;
         if (sg.failed()) return 2;
         // rows that are no whole 16-byte pieces are copied to such; dh is written a second time
-        const int cols = (in + 7) / 8 * 8, pitch = (2 * outs + 7) / 8 * 8;
+        constexpr int VEC = RowPiece<T>::VEC;
+        const int cols = (in + VEC - 1) / VEC * VEC, pitch = (2 * outs + VEC - 1) / VEC * VEC;
         bool copy_x = ((uintptr_t)x | (uintptr_t)w) % 16 || cols != in, copy_dh = (uintptr_t)dh % 16 || pitch != 2 * outs;
         const bool own = own_products<T>(ns, in, outs, copy_x || copy_dh);
         copy_x = copy_x && own;
@@ -115,10 +120,8 @@ static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool w
                            wide_dh, pitch);
         if (part) row_shares<T>(part, db, 2 * outs, high);
         int rc = hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
-        if constexpr (sizeof(T) == 2) {
-            if (rc == 0 && own && (wg || ig))
-                rc = gated_products(copy_x ? wide_x : x, copy_x ? wide_w : w, copy_dh ? wide_dh : dh, dw, dx, ns, in, 2 * outs, cols, pitch);
-        }
+        if (rc == 0 && own && (wg || ig))
+            rc = gated_products<T>(copy_x ? wide_x : x, copy_x ? wide_w : w, copy_dh ? wide_dh : dh, dw, dx, ns, in, 2 * outs, cols, pitch);
         rc = sg.finish(rc);
         if (rc || own || !(wg || ig)) return rc;
     }

@@ -284,3 +284,21 @@ def test_few_outputs_of_long_rows(pkg, gpu, dt, n, n_in, n_out):
     assert torch.equal(again, y) and none is None
     y, h = forward(pkg, gpu, dt, "gelu", x, w, None)
     check_forward(dt, "gelu", x, w, None, y, h)
+
+
+@pytest.mark.parametrize("n,n_in,n_out,bias", [(16, 1600, 1600, 1), (33, 1601, 1601, 1), (153, 1134, 3135, 0), (1024, 640, 960, 1), (5000, 130, 999, 1), (6200, 64, 1700, 0),
+                                               (511, 1027, 1190, 1)])
+def test_backward_own_products_fp32(pkg, gpu, n, n_in, n_out, bias):
+    """fp32 layers with large weights, or from 5 GFLOP on: in parts and not, as they are and as copies, each gradient alone, in place."""
+    x, w, _ = inputs(n, "fp32", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5), tr.rand(n + 6, n, n_out, scale=0.5)
+    full = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, bias)
+    check_backward("fp32", "silu", x, w, h, dy, *full)
+    over = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, bias, over=1)
+    assert all(a is None or torch.equal(a, b) for a, b in zip(over, full))
+    dh, dx, dw, _ = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, bias, skip_wg=1)
+    check_backward("fp32", "silu", x, w, h, dy, dh, dx, None, None)
+    assert (dw == 7).all()
+    dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, bias, skip_ig=1)
+    check_backward("fp32", "silu", x, w, h, dy, dh, None, dw, db)
+    assert (dx == 7).all()
