@@ -80,8 +80,8 @@ int ptl_rms_norm_fp16_bw_batched(const struct RmsNorm_args_fp16 *a, int nsamples
  *   backward: hidden->diff = (output->diff * h_up * act'(h_gate), output->diff * act(h_gate)) from hidden->data;
  *             coeff->diff = hidden->diff^T * input->data (sum over the samples) and, with use_biases, bias->diff = the sum of
  *             hidden->diff, unless skip_wg_grad; input->diff = hidden->diff * coeff unless skip_in_grad.  hidden->diff is
- *             always written and is what the products read, rounded to the tensor type as it is stored; it may be
- *             hidden->data (the pre-activations are lost then). */
+ *             always written and is what the products and sums read, rounded to the tensor type as it is stored (fp16 calls of up
+ *             to two samples or fewer than 16384 values: as it was before that); it may be hidden->data (the pre-activations are lost then). */
 struct GatedLinear_args {
     struct blob *input;
     struct blob *coeff;

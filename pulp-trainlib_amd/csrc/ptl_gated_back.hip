@@ -35,6 +35,8 @@ struct GradProd {
     int k, f_b, s_b;    // k, bytes of a row of either
     int f_n, s_n;       // rows that have values of their own in [k][row] tiles: whole eights
     int parts, chunk;   // k in parts of so many slabs, each with its own sums in fp32 (part) where there are more than one
+    int high;           // parts of s; the others, the same k again, are of `low`
+    const char *low;
     float *part;
 };
 struct GradArgs {
@@ -76,14 +78,14 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
     constexpr int NT = C::NT, ES = (int)sizeof(T), VEC = 16 / ES, KS = ROWB / ES;  // k of a slab
     constexpr int PER = 128 / VEC, XPER = XR / VEC, LX = XR * 8 / NT, FN = C::FN;      // pieces of a k's rows, loads of a thread for the second tile
     const RowsArgs &a = g.out;
-    const int tiles = a.tiles_w * a.tiles_t, z = id / tiles, k0 = z * g.chunk * KS, k_n = min(g.k - k0, g.chunk * KS);
+    const int tiles = a.tiles_w * a.tiles_t, z = id / tiles, k0 = (z < g.high ? z : z - g.high) * g.chunk * KS, k_n = min(g.k - k0, g.chunk * KS);
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave & 1, ww = wave >> 1;
     int tw, tt;
     rows_place(a, id - z * tiles, tw, tt);
     const int o0 = tw * 128, t0 = tt * XR, slabs = (k_n + KS - 1) / KS, tail = k_n - (slabs - 1) * KS;
     const unsigned ring = (unsigned)(uintptr_t)(lds_char *)smem;
     const char *f_ptr = g.f + (long long)o0 * ES + (long long)k0 * g.f_b;
-    const char *s_ptr = ROWS ? g.s + (long long)t0 * g.s_b + (long long)k0 * ES : g.s + (long long)t0 * ES + (long long)k0 * g.s_b;
+    const char *s_ptr = (z < g.high ? g.s : g.low) + (ROWS ? (long long)t0 * g.s_b + (long long)k0 * ES : (long long)t0 * ES + (long long)k0 * g.s_b);
     const long long f_step = (long long)KS * g.f_b, s_step = ROWS ? ROWB : (long long)KS * g.s_b;
     // piece of a [k][row] tile that lies at place q: its k, and its rows as a multiple of VEC behind the tile's first; rows beyond
     // the end repeat the last ones
@@ -189,7 +191,7 @@ struct GradJoin {
     const float *part[2];
     T *y[2];
     size_t n[2], values[2];  // fours of values (0: not in parts), values
-    int parts[2];
+    int parts[2], high[2];
 };
 template <typename T>
 __global__ __launch_bounds__(256) void grad_join_kernel(const GradJoin<T> a) {
@@ -199,13 +201,16 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const GradJoin<T> a) {
     if (i >= a.n[o]) return;
     const float4 *p = reinterpret_cast<const float4 *>(a.part[o]) + i;
     float4 s = p[0];
+    float4 low = make_float4(0.f, 0.f, 0.f, 0.f);
     for (int k = 1; k < a.parts[o]; ++k) {
         const float4 v = p[(size_t)k * a.n[o]];
-        s.x += v.x;
-        s.y += v.y;
-        s.z += v.z;
-        s.w += v.w;
+        float4 &t = k < a.high[o] ? s : low;
+        t.x += v.x;
+        t.y += v.y;
+        t.z += v.z;
+        t.w += v.w;
     }
+    s = make_float4(fmaf(low.x, 1.f / GRAD_LOW, s.x), fmaf(low.y, 1.f / GRAD_LOW, s.y), fmaf(low.z, 1.f / GRAD_LOW, s.z), fmaf(low.w, 1.f / GRAD_LOW, s.w));
     typedef T t4 __attribute__((ext_vector_type(4)));
     const t4 v = t4{(T)s.x, (T)s.y, (T)s.z, (T)s.w};
     if (4 * i + 4 <= a.values[o]) {
@@ -244,7 +249,7 @@ static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const doubl
 }
 
 template <typename T>
-int gated_products(const T *x, const T *w, const T *dh, T *dw, T *dx, int ns, int in, int rows, int cols, int pitch) {
+int gated_products(const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols, int pitch) {
     static bool ready = false;
     constexpr int XR = sizeof(T) == 4 ? 64 : 128, RING = GradTile<T, XR>::RING, KS = ROWB / (int)sizeof(T);
     if (!ready) {
@@ -291,7 +296,9 @@ int gated_products(const T *x, const T *w, const T *dh, T *dw, T *dx, int ns, in
         p.f_n = cols;
         p.s_n = pitch;
         p.chunk = (slabs[i] + parts[i] - 1) / parts[i];
-        p.parts = (slabs[i] + p.chunk - 1) / p.chunk;
+        p.high = (slabs[i] + p.chunk - 1) / p.chunk;
+        p.low = reinterpret_cast<const char *>(low);
+        p.parts = low && y[i] ? 2 * p.high : p.high;
         if (p.parts > 1) floats += (size_t)p.parts * grad_part(n[i], in);
     }
     if (floats) {
@@ -305,6 +312,7 @@ int gated_products(const T *x, const T *w, const T *dh, T *dw, T *dx, int ns, in
             j.values[i] = (size_t)n[i] * in;
             j.n[i] = grad_part(n[i], in) / 4;
             j.parts[i] = a.p[i].parts;
+            j.high[i] = a.p[i].high;
             ws += (size_t)a.p[i].parts * grad_part(n[i], in);
         }
     }
@@ -319,8 +327,8 @@ int gated_products(const T *x, const T *w, const T *dh, T *dw, T *dx, int ns, in
     return hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
 }
 
-template int gated_products<half_t>(const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int, int);
-template int gated_products<float>(const float *, const float *, const float *, float *, float *, int, int, int, int, int);
+template int gated_products<half_t>(const half_t *, const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int, int);
+template int gated_products<float>(const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int);
 
 void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, int bytes, int pitch) {
     rows_copies(static_cast<const char *>(w), n_w, static_cast<const char *>(x), n_x, static_cast<char *>(to), bytes, pitch);

@@ -107,16 +107,19 @@ def check_backward(dt, act, x, w, h, dy, dh, dx, dw, db):
     tol = torch.cat([(d * up).abs() * slope, (d * f).abs() * U * (tr.act_steps(g, act) + 2)], 1)
     tr.within(dh, ref, tol + tr.step(ref, dt), "dh")
     got = dh.double().cpu()  # what the products read
+    off = torch.zeros_like(got)
+    if dt == "fp16" and (n <= 2 or 2 * n * n_out < 16384):  # ... few of them: before they are rounded, in two halves of 11 bits; the second in steps of 2^-24 / 2048
+        got, off = ref, tol + ref.abs() * 2.0 ** -22 + 2.0 ** -36
     x, w = x.double(), w.double()
     if dx is not None:
         ref = got @ w
-        tr.within(dx, ref, U * (2 * n_out + 4) * (got.abs() @ w.abs()) + tr.step(ref, dt), "dx")
+        tr.within(dx, ref, U * (4 * n_out + 8) * (got.abs() @ w.abs()) + off @ w.abs() + tr.step(ref, dt), "dx")
     if dw is not None:
         ref = got.t() @ x
-        tr.within(dw, ref, U * (n + 4) * (got.abs().t() @ x.abs()) + tr.step(ref, dt), "dw")
+        tr.within(dw, ref, U * (2 * n + 8) * (got.abs().t() @ x.abs()) + off.t() @ x.abs() + tr.step(ref, dt), "dw")
     if db is not None:
         ref = got.sum(0)
-        tr.within(db, ref, U * (n + 4) * got.abs().sum(0) + tr.step(ref, dt), "db")
+        tr.within(db, ref, U * (n + 4) * got.abs().sum(0) + off.sum(0) + tr.step(ref, dt), "db")
 
 
 @pytest.mark.parametrize("dt", ["fp32", "fp16"])
@@ -302,3 +305,36 @@ def test_backward_own_products_fp32(pkg, gpu, n, n_in, n_out, bias):
     dh, dx, dw, db = backward(pkg, gpu, "fp32", "silu", x, w, h, dy, bias, skip_ig=1)
     check_backward("fp32", "silu", x, w, h, dy, dh, None, dw, db)
     assert (dx == 7).all()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,n_in,n_out", [(1, 1, 1), (1, 3, 5), (1, 9, 700), (2, 2954, 67), (3, 64, 64), (4, 1001, 333), (5, 130, 257), (7, 515, 40), (8, 600, 1000),
+                                          (1, 2000, 9000), (2, 4101, 2000), (12, 333, 600), (100, 77, 50)])
+def test_backward_of_few_tokens(pkg, gpu, dt, n, n_in, n_out):
+    """Layers whose whole backward pass is one kernel and its sums, and small ones in two halves: all parts, each gradient alone, in place."""
+    x, w, _ = inputs(n, dt, n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt=dt), tr.rand(n + 6, n, n_out, scale=0.5, dt=dt)
+    for act in ("silu", "gelu", "sigmoid", "relu"):
+        full = backward(pkg, gpu, dt, act, x, w, h, dy, 1)
+        check_backward(dt, act, x, w, h, dy, *full)
+    over = backward(pkg, gpu, dt, act, x, w, h, dy, 1, over=1)
+    assert all(torch.equal(a, b) for a, b in zip(over, full))
+    dh, dx, dw, _ = backward(pkg, gpu, dt, act, x, w, h, dy, 1, skip_wg=1)
+    check_backward(dt, act, x, w, h, dy, dh, dx, None, None)
+    assert (dw == 7).all()
+    dh, dx, dw, db = backward(pkg, gpu, dt, act, x, w, h, dy, 1, skip_ig=1)
+    check_backward(dt, act, x, w, h, dy, dh, None, dw, db)
+    assert (dx == 7).all()
+
+
+def test_backward_of_few_tokens_with_infinities(pkg, gpu):
+    """A gradient beyond the largest half number is infinite in hidden->diff and in what depends on it, nowhere else."""
+    for n in (1, 20):
+        n_in, n_out = 40, 30
+        x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+        h, dy = torch.ones(n, 2 * n_out, dtype=torch.float16), torch.ones(n, n_out, dtype=torch.float16)
+        h[0, n_out + 3], dy[0, 3] = 60000, 60000
+        dh, dx, dw, db = backward(pkg, gpu, "fp16", "relu", x, w, h, dy, 1)
+        assert torch.isinf(dh[0, 3]) and torch.isfinite(dh[0, :3]).all() and torch.isinf(db[3])
+        assert not torch.isfinite(dw[3]).any() and torch.isfinite(dw[:3]).all() and not torch.isfinite(dx[0]).any()
+        assert n == 1 or torch.isfinite(dx[1:]).all()
