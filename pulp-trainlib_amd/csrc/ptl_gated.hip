@@ -222,11 +222,12 @@ static bool few_gradients(int ns, int in, int outs) {
     return sizeof(T) == 2 && in < 1 << 23 && (double)ns * 2 * outs < 16384 && state().gemm_path == 0;
 }
 // Which calls gate_few() takes: in halves the same 1.1 to 4 times as long; against a dense layer's call one and two tokens 0.92 to 1.37 times
-// as fast, in fp32 three and four 0.9 to 1.15 (in fp16 0.76 to 0.98).
+// as fast, in fp32 three and four 0.9 to 1.15 up to 7 million weights of either half (beyond, in rows that are no whole pieces, 0.82 to 0.9;
+// in fp16 0.75 to 1.1).
 template <typename T>
 static bool few_tokens(int ns, int in, int outs) {
     const bool fits = (double)ns * in < ROW_MOST && outs < GATE_HIGH * 32000;  // (columns of a sum of shares, groups of rows)
-    const bool pays = ns <= 2 || (sizeof(T) == 4 && ns <= 4) || (ns <= 8 && few_gradients<T>(ns, in, outs));
+    const bool pays = ns <= 2 || (sizeof(T) == 4 && ns <= 4 && (double)in * outs <= 7e6) || (ns <= 8 && few_gradients<T>(ns, in, outs));
     return fits && pays && state().gemm_path == 0;
 }
 
