@@ -294,7 +294,7 @@ __device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first
         RowPiece<T> o;
         if (some) {
 #pragma unroll
-            for (int i = 0; i < RowPiece<T>::VEC; ++i) o.e[i] = (T)(e(z[j].e[i]) * f);
+            for (int i = 0; i < RowPiece<T>::VEC; ++i) o.e[i] = row_round<T>(e(z[j].e[i]) * f);
         } else {
             o.raw = row_u4{0, 0, 0, 0};
         }

@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256) void gate_few_kernel(const GateFew<T> a) {
                     float f = v[0] * (float)x[0].e[i];
 #pragma unroll
                     for (int t = 1; t < NS; ++t) f = fmaf(v[t], (float)x[t].e[i], f);
-                    o.e[i] = (T)f;
+                    o.e[i] = row_round<T>(f);
                 }
                 o.template put<true>(a.dw + (size_t)(r0 + r + 4 * u) * in, p, in);
             }

@@ -128,12 +128,12 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
         };
         if (a.skip) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = (T)f[i];
+            for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(f[i]);
             out(a.sum + at);
         }
         if (a.y) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = (T)(f[i] * r * (float)w.e[i]);
+            for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(f[i] * r * (float)w.e[i]);
             out(a.y + at);
         }
         if constexpr (Q8) {
@@ -316,7 +316,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
             Piece o;
 #pragma unroll
             for (int i = 0; i < VEC; ++i)
-                o.e[i] = (T)norm_dx((float)x.s[j].e[i], (float)x.g[j].e[i] * (float)wj.e[i], a.add ? (float)d.e[i] : 0.f, r, m);
+                o.e[i] = row_round<T>(norm_dx((float)x.s[j].e[i], (float)x.g[j].e[i] * (float)wj.e[i], a.add ? (float)d.e[i] : 0.f, r, m));
             const int cut = LATE ? Piece::cut(p, dim) : 0;
             if (cut) {  // (a.add, read late, may be in the place of dx: another thread's elements are left to it)
 #pragma unroll
@@ -369,7 +369,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
             gather(j);
             Piece o;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = (T)dw[LATE ? 0 : j][i];
+            for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(dw[LATE ? 0 : j][i]);
             o.template put<SHORT>(a.dw, j * TPR + t, dim);
         }
     } else {

@@ -91,6 +91,15 @@ struct RowPiece {
     }
 };
 
+// A value as it is stored.  It is rounded to fp32 first, in every place alike: left to itself the compiler joins the last operation and the
+// rounding to fp16 for some values of a piece and not for others, which gives another value in one of thousands, and the values that
+// two pieces share (RowPiece::put) would depend on which is written last.
+template <typename T>
+__device__ inline T row_round(float f) {
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(f));
+    return (T)f;
+}
+
 constexpr int ROW_MOST = 1 << 30;  // elements of a row, rows of a call
 constexpr long ROW_THREADS = 1l << 31;  // of a launch (it takes 2^32 - 1; calls with more rows are several launches)
 

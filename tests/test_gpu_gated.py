@@ -338,3 +338,20 @@ def test_backward_of_few_tokens_with_infinities(pkg, gpu):
         assert torch.isinf(dh[0, 3]) and torch.isfinite(dh[0, :3]).all() and torch.isinf(db[3])
         assert not torch.isfinite(dw[3]).any() and torch.isfinite(dw[:3]).all() and not torch.isfinite(dx[0]).any()
         assert n == 1 or torch.isfinite(dx[1:]).all()
+
+
+def test_backward_of_few_tokens_is_the_same_in_every_call(pkg, gpu):
+    """The piece that ends a row is another workgroup's and shares values with the one before: they are the same values."""
+    n, n_in, n_out = 2, 2561, 3000
+    x, w, _ = inputs(n, "fp16", n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    X, W, H, DY = (tr.dev(t) for t in (x, w, h, dy))
+    dx, dw, dh = torch.empty_like(X), torch.empty_like(W), torch.empty_like(H)
+    a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=X, dx=dx, w=W, dw=dw, h=H, dh=dh, dy=DY)
+    first = None
+    for _ in range(100):
+        dw.fill_(7)
+        pkg.call("ptl_gated_linear_fp16_bw_batched", a, n)
+        assert gpu.ptl_sync() == 0
+        first = first or [t.clone() for t in (dh, dx, dw)]
+        assert all(torch.equal(p, q) for p, q in zip(first, (dh, dx, dw)))
