@@ -175,3 +175,46 @@ def test_values_in_rows_that_no_workgroup_holds(pkg, gpu, dt, n, v):
     assert torch.isnan(loss[3]) and torch.isnan(grad[3]).all()
     again, over = run(pkg, gpu, dt, z, teacher, classes, in_place=True)
     assert torch.equal(again[keep], loss[keep]) and torch.equal(over[keep], grad[keep])
+
+
+def case_at(seed, n, v, k, dt, temperature, far, spread):
+    """Logits around `far`, a teacher whose logits differ by some temperatures."""
+    z, _, classes = case(seed, n, v, k, dt)
+    z = (z.double() * spread / 2 + far).to(z.dtype)
+    top = z.float().topk(min(k, 3), dim=1).indices  # the first entries name the largest classes
+    classes[:, : top.shape[1]] = top.to(torch.int32)
+    return z, tr.rand(seed + 1, n, k, scale=2.0 * temperature, dt=dt), classes
+
+
+def check_at(dt, z, teacher, classes, loss, grad, temperature, weight):
+    """Temperature and weight are fp32 numbers here.  log p and log q are differences from the row's largest logit, 4 u of themselves off
+    (the difference, 1 / T, the product), less the log of a sum, which is c u off, and rounded; p and the terms follow from them."""
+    ref_loss, _, _ = tr.distill64(z, teacher, classes, temperature, weight)
+    v, k = z.shape[1], classes.shape[1]
+    at = torch.where((classes >= 0) & (classes < v), classes, torch.zeros_like(classes)).long()
+    there = (classes >= 0) & (classes < v)
+    zz = (z.double().amax(1, keepdim=True) - z.double().gather(1, at)) / temperature
+    u = torch.where(there, teacher.double() / temperature, torch.tensor(-math.inf, dtype=torch.float64))
+    uu = torch.where(there, u.amax(1, keepdim=True) - u, torch.zeros_like(u))
+    log_q = torch.log_softmax(z.double() / temperature, 1).gather(1, at)
+    log_p = torch.where(there, torch.log_softmax(torch.where(there, u, torch.full_like(u, -1e300)), 1), torch.zeros_like(u))
+    p = torch.where(there, log_p.exp(), torch.zeros_like(u))
+    c = 128 + 21 + v / 1024 + 16
+    off = p * (4 * zz + 4 * uu + 2 * c + (log_p.abs() + log_q.abs()) * (c + 4 * uu + k + 30))
+    tr.within(loss, ref_loss, abs(weight) * U * off.sum(1) + 2.0 ** -140, "loss")
+    check(dt, z, teacher, classes, None, grad, temperature, weight)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n,v,k", [(3, 3000, 40), (1030, 300, 9), (3, 40001, 40), (130, 131075, 20)])
+def test_low_temperatures_and_far_logits(pkg, gpu, dt, n, v, k):
+    """Rows by the workgroup, by the wave, in parts and walked.  A class' probability follows from its distance from the largest logit,
+    however far from 0 both lie in units of the temperature."""
+    cases = ((0.05, 0, 2), (0.05, 1000, 2), (0.01, 100, 1), (1e-3, 5, 5), (1e-3, -1, 0.01), (1e-4, 0, 100), (1e-5, 100, 1), (1e-6, 0, 5), (1e-6, 0, 2000),
+             (1.0, 30000, 20), (2.0, -60000, 40))
+    for temperature, far, spread in cases if n < 100 else cases[1::3]:
+        temperature = float(torch.tensor(temperature, dtype=torch.float32))
+        weight = float(torch.tensor(3 * temperature, dtype=torch.float32))
+        z, teacher, classes = case_at(n + v, n, v, k, dt, temperature, far, spread)
+        loss, grad = run(pkg, gpu, dt, z, teacher, classes, temperature, weight)
+        check_at(dt, z, teacher, classes, loss, grad, temperature, weight)
