@@ -58,7 +58,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };  // (pieces that no thread has; half of them someone has)
     float s[HELD][VEC];
     Piece w[HELD];
-    float v[2] = {0.f, 0.f};  // sum of squares, largest |s w|
+    float v[2] = {0.f, 0.f};  // sum of squares, largest |s w| (NaN where one is)
     auto join = [&](const Piece &x, const Piece &k, float (&f)[VEC]) {
 #pragma unroll
         for (int i = 0; i < VEC; ++i) f[i] = a.skip ? (float)x.e[i] + (float)k.e[i] : (float)x.e[i];
@@ -73,7 +73,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
         }
         if constexpr (Q8) {
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) v[1] = fmaxf(v[1], fabsf(f[i] * (float)w.e[i]));
+            for (int i = 0; i < VEC; ++i) v[1] = nan_max(v[1], fabsf(f[i] * (float)w.e[i]));
         }
     };
     // (rows that are walked: a thread reads behind the barrier what another may have written over by then, so each has its own elements)
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
             put(p, s[0], w[0]);
         }
     }
-    // infinities and NaN: v[0] is then no finite number, and neither is the scale
+    // infinities and NaN: v[0] or (of the weights) v[1] is then no finite number, and neither is the scale
     if (Q8 && t == 0) a.scale[row] = v[0] < __builtin_inff() ? v[1] * r / 127.f : __builtin_nanf("");
 }
 

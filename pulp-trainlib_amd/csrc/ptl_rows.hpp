@@ -114,13 +114,20 @@ __device__ inline float wave_max(float v) {
     for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off));
     return v;
 }
+// The larger value, or NaN where either is none (one instruction takes three of them).
+__device__ inline float nan_max(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+__device__ inline float wave_nan_max(float v) {
+#pragma unroll
+    for (int off = 32; off > 0; off >>= 1) v = nan_max(v, __shfl_xor(v, off));
+    return v;
+}
 
 // ... over the TPR threads that have a row: one wave, or a workgroup (a float per wave and value in `lds`, which the caller
 // does not use again without a barrier).
-template <int TPR, int N, bool MAX1 = false>  // MAX1: the second value is a maximum
+template <int TPR, int N, bool MAX1 = false>  // MAX1: the second value is a maximum that keeps NaN
 __device__ inline void row_reduce(float (&v)[N], float (*lds)[N]) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) v[i] = MAX1 && i == 1 ? wave_max(v[i]) : wave_sum(v[i]);
+    for (int i = 0; i < N; ++i) v[i] = MAX1 && i == 1 ? wave_nan_max(v[i]) : wave_sum(v[i]);
     if constexpr (TPR > 64) {
         const int wave = threadIdx.x >> 6;
         if ((threadIdx.x & 63) == 0) {
@@ -132,7 +139,7 @@ __device__ inline void row_reduce(float (&v)[N], float (*lds)[N]) {
         for (int i = 0; i < N; ++i) {
             float s = lds[0][i];
 #pragma unroll
-            for (int w = 1; w < TPR / 64; ++w) s = MAX1 && i == 1 ? fmaxf(s, lds[w][i]) : s + lds[w][i];
+            for (int w = 1; w < TPR / 64; ++w) s = MAX1 && i == 1 ? nan_max(s, lds[w][i]) : s + lds[w][i];
             v[i] = s;
         }
     }

@@ -246,3 +246,21 @@ def test_rows_that_end_inside_a_piece(pkg, gpu, dt, n, dim):
     pkg.call("ptl_rms_norm_%s_bw_batched" % dt, a, n)
     check_backward(dt, x, dy, None, w, big[1:n + 1], None, None)
     assert (big[0] == 7).all() and (big[n + 1] == 7).all()
+
+
+# rows of a wave, of a workgroup with one and several pieces a thread, and rows that are walked
+VARIANTS = [5, 100, 1001, 4096, 9001, 40001]
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("dim", VARIANTS)
+def test_no_numbers_among_the_weights_in_8_bits(pkg, gpu, dt, dim):
+    """NaN or an infinity in coeff, also one that meets a 0: every row has a value that is no finite number, and so is its scale."""
+    x = tr.rand(1, 6, dim, dt=dt)
+    x[3, dim // 2] = 0
+    for bad in ("nan", "inf", "-inf"):
+        w = 1 + tr.rand(2, dim, scale=0.2, dt=dt)
+        w[dim // 2] = float(bad)
+        _, Y, _, C = forward(pkg, gpu, dt, x, None, w)
+        assert not torch.isfinite(Y[:, dim // 2]).any() and not torch.isfinite(C).any(), bad
+        assert torch.isfinite(torch.cat([Y[:, : dim // 2], Y[:, dim // 2 + 1:]], 1)).all()
