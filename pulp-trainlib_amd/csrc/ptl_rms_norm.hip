@@ -118,7 +118,9 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
     row_reduce<TPR, 2, true>(v, red);
     const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps);
     // (a row of zeros: all zeros; otherwise the largest value becomes 127 to within a rounding of the product)
-    const float unit = v[1] > 0.f ? 127.f / v[1] : 0.f;
+    // (fp32: 127 / v[1] is infinite from 3.7e-37 down, and products there lose their bits: such rows are worked on 2^100 times as large)
+    const float lift = sizeof(T) == 4 && v[1] < 0x1p-100f ? 0x1p100f : 1.f;
+    const float unit = v[1] > 0.f ? 127.f / (v[1] * lift) : 0.f;
     auto put = [&](int p, const float (&f)[VEC], const Piece &w) {
         if (p >= pieces) return;
         Piece o;
@@ -139,7 +141,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
         if constexpr (Q8) {
             int q[VEC];
 #pragma unroll
-            for (int i = 0; i < VEC; ++i) q[i] = (int)fminf(fmaxf(rintf(f[i] * (float)w.e[i] * unit), -127.f), 127.f);
+            for (int i = 0; i < VEC; ++i) q[i] = (int)fminf(fmaxf(rintf((sizeof(T) == 4 ? f[i] * lift : f[i]) * (float)w.e[i] * unit), -127.f), 127.f);
             put_q<VEC, (NP > 0 && !SHORT)>(a.q + at, p * VEC - (NP > 0 ? Piece::cut(p, dim) : 0), dim, q);
         }
     };

@@ -264,3 +264,21 @@ def test_no_numbers_among_the_weights_in_8_bits(pkg, gpu, dt, dim):
         _, Y, _, C = forward(pkg, gpu, dt, x, None, w)
         assert not torch.isfinite(Y[:, dim // 2]).any() and not torch.isfinite(C).any(), bad
         assert torch.isfinite(torch.cat([Y[:, : dim // 2], Y[:, dim // 2 + 1:]], 1)).all()
+
+
+@pytest.mark.parametrize("dim", VARIANTS)
+def test_tiny_rows_in_8_bits(pkg, gpu, dim):
+    """Rows whose largest |s w| is at the end of fp32's range: zeros stay zeros and the largest value becomes 127.  A value that is no
+    normal number is off by up to 2^-150, which is 127 * 2^-150 / max|y| of the unit."""
+    x, w = tr.rand(1, 5, dim).double(), 1 + tr.rand(2, dim, scale=0.2)
+    x[:, ::3] = 0
+    x = (x * torch.tensor([1.0, 1e-36, 2e-38, 1e-40, 1e-42], dtype=torch.float64)[:, None]).float()
+    _, _, Q, C = forward(pkg, gpu, "fp32", x, None, w, y=False)
+    v = x.double() * w.double()
+    ref = tr.norm64(x.double(), w.double(), EPS)
+    amax = v.abs().amax(1, keepdim=True)
+    off = (Q.cpu().double() - v * 127 / amax).abs()
+    assert (off <= 0.5 + 127 * (6 * U + 2.0 ** -149 / amax)).all()
+    assert (Q.cpu()[x == 0] == 0).all() and (Q.abs().amax(1) == 127).all()
+    amax = ref.abs().amax(1)
+    tr.within(C, amax / 127, amax / 127 * U * (chain(dim) / 2 + 10) + 2.0 ** -148 * (1 + amax / v.abs().amax(1)))
