@@ -23,6 +23,7 @@ extern "C" {
 
 /* Root-mean-square normalisation of rows, behind a residual's addition.
  *   forward:  s = input [+ skip];  r = 1 / sqrt(mean(s^2) + eps);  y = s * r * coeff
+ *     With eps = 0 a row of zeros (one whose squares are all 0 in fp32) has r = 0: y is 0, and backward it takes no part.
  *     sum->data    (needed with skip, else NULL or not read) receives s, rounded to the tensor type
  *     output->data (output or its data may be NULL) receives y
  *     q_data, q_scale (both or neither): y in 8 bits, q = y / scale rounded to the nearest (ties to even), with one scale

@@ -26,6 +26,13 @@ struct NormFw {
     float eps;
 };
 
+// 1 / sqrt(mean + eps) of a row's sum of squares; 0 where both are 0 (a row of zeros, or of values so small that their squares are, with
+// eps = 0): such a row has zeros, and the gradient reaches it along the residual only.
+__device__ inline float norm_r(float sum, int dim, float eps) {
+    const float q = sum / (float)dim + eps;
+    return q == 0.f ? 0.f : 1.f / sqrtf(q);
+}
+
 // The eight-bit integers of VEC values, from element `at` on: one store of VEC bytes where the row has all of them (WHOLE: it has).
 template <int VEC, bool WHOLE>
 __device__ inline void put_q(int8_t *row, int at, int dim, const int (&q)[VEC]) {
@@ -116,11 +123,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_fw_kernel(cons
         }
     }
     row_reduce<TPR, 2, true>(v, red);
-    const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps);
+    const float r = norm_r(v[0], dim, a.eps);
     // (a row of zeros: all zeros; otherwise the largest value becomes 127 to within a rounding of the product)
     // (fp32: 127 / v[1] is infinite from 3.7e-37 down, and products there lose their bits: such rows are worked on 2^100 times as large)
     const float lift = sizeof(T) == 4 && v[1] < 0x1p-100f ? 0x1p100f : 1.f;
-    const float unit = v[1] > 0.f ? 127.f / (v[1] * lift) : 0.f;
+    const float unit = v[1] > 0.f && r > 0.f ? 127.f / (v[1] * lift) : 0.f;
     auto put = [&](int p, const float (&f)[VEC], const Piece &w) {
         if (p >= pieces) return;
         Piece o;
@@ -300,7 +307,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
         }
         row_reduce<TPR, 2>(v, red[turn]);
         turn ^= 1;
-        const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps), m = r * r * r * (v[1] / (float)dim);
+        const float r = norm_r(v[0], dim, a.eps), m = r * r * r * (v[1] / (float)dim);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
@@ -411,7 +418,7 @@ __global__ __launch_bounds__(1024) void rms_norm_stat_kernel(const NormBw<T> a) 
     }
     row_reduce<1024, 2>(v, red);
     if (threadIdx.x == 0) {
-        const float r = 1.f / sqrtf(v[0] / (float)dim + a.eps);
+        const float r = norm_r(v[0], dim, a.eps);
         a.stat[2 * row] = r;
         a.stat[2 * row + 1] = r * r * r * (v[1] / (float)dim);
     }

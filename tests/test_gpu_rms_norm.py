@@ -282,3 +282,22 @@ def test_tiny_rows_in_8_bits(pkg, gpu, dim):
     assert (Q.cpu()[x == 0] == 0).all() and (Q.abs().amax(1) == 127).all()
     amax = ref.abs().amax(1)
     tr.within(C, amax / 127, amax / 127 * U * (chain(dim) / 2 + 10) + 2.0 ** -148 * (1 + amax / v.abs().amax(1)))
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("dim", VARIANTS)
+def test_rows_of_zeros_without_eps(pkg, gpu, dt, dim):
+    """eps = 0: a row of zeros has zeros, the scale 0 and no gradient but the one along the residual; the other rows are as always."""
+    x, w = tr.rand(1, 4, dim, dt=dt), 1 + tr.rand(2, dim, scale=0.2, dt=dt)
+    x[1] = 0
+    _, Y, Q, C = forward(pkg, gpu, dt, x, None, w, eps=0.0)
+    assert (Y[1] == 0).all() and (Q[1] == 0).all() and C[1] == 0
+    check_forward(dt, x[[0, 2, 3]], None, w, None, Y[[0, 2, 3]], Q[[0, 2, 3]], C[[0, 2, 3]], eps=0.0)
+    dy, add = tr.rand(3, 4, dim, scale=0.5, dt=dt), tr.rand(4, 4, dim, dt=dt)
+    DX, _, DW = backward(pkg, gpu, dt, x, dy, add, w, 1, eps=0.0)
+    assert torch.equal(DX[1].cpu(), add[1])
+    rest = [0, 2, 3]
+    A, _, B = backward(pkg, gpu, dt, x[rest], dy[rest], add[rest], w, 1, eps=0.0)
+    assert torch.equal(DX[rest], A)
+    t = (dy.double() * x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True)))[rest]
+    tr.within(DW, t.sum(0), t.abs().sum(0) * U * (chain(dim) / 2 + 12) + tr.step(t.sum(0), dt), "dw")
