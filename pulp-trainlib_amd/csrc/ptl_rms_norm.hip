@@ -204,13 +204,16 @@ struct NormBw {
     T *dx, *dx2;  // (NULL: not wanted)
     T *dw;        // where one workgroup has all the rows (else NULL)
     float *part;  // of dw: a row for each workgroup (NULL: not wanted)
-    float *stat;  // long rows: r and r^3 mean(g s) of each row
+    float *stat;  // long rows: r and r^2 mean(g s) of each row
     int rows, dim;
     int first;  // of the rows whose statistics a launch forms
     float eps;
 };
 
-__device__ inline float norm_dx(float s, float g, float add, float r, float m) { return fmaf(r, g, fmaf(-m, s, add)); }
+// r (g - s m) + add with m = r^2 mean(g s), formed as r (r mean): each step is of the size of r or of g, where r^3 leaves fp32's range from
+// rows of 1e-13 down and from 1e13 up.
+__device__ inline float norm_m(float r, float sum, int dim) { return r * (r * (sum / (float)dim)); }
+__device__ inline float norm_dx(float s, float g, float add, float r, float m) { return fmaf(r, fmaf(-m, s, g), add); }
 
 // Whether registers hold two rows.
 template <typename T, int TPR, int NP>
@@ -307,7 +310,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void rms_norm_bw_kernel(cons
         }
         row_reduce<TPR, 2>(v, red[turn]);
         turn ^= 1;
-        const float r = norm_r(v[0], dim, a.eps), m = r * r * r * (v[1] / (float)dim);
+        const float r = norm_r(v[0], dim, a.eps), m = norm_m(r, v[1], dim);
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
@@ -420,7 +423,7 @@ __global__ __launch_bounds__(1024) void rms_norm_stat_kernel(const NormBw<T> a) 
     if (threadIdx.x == 0) {
         const float r = norm_r(v[0], dim, a.eps);
         a.stat[2 * row] = r;
-        a.stat[2 * row + 1] = r * r * r * (v[1] / (float)dim);
+        a.stat[2 * row + 1] = norm_m(r, v[1], dim);
     }
 }
 template <typename T>

@@ -301,3 +301,21 @@ def test_rows_of_zeros_without_eps(pkg, gpu, dt, dim):
     assert torch.equal(DX[rest], A)
     t = (dy.double() * x.double() / torch.sqrt((x.double() ** 2).mean(1, keepdim=True)))[rest]
     tr.within(DW, t.sum(0), t.abs().sum(0) * U * (chain(dim) / 2 + 12) + tr.step(t.sum(0), dt), "dw")
+
+
+@pytest.mark.parametrize("dim", VARIANTS)
+def test_backward_of_very_small_and_very_large_rows(pkg, gpu, dim):
+    """Gradients of the size of 1 / rms, which fp32 holds where (1 / rms)^3 is infinite or subnormal."""
+    n = 5
+    for size, eps in ((1e14, EPS), (3e14, EPS), (1e-14, 0.0), (1e-16, 0.0)):
+        s = (tr.rand(1, n, dim).double() * size).float()
+        dy, w = tr.rand(2, n, dim, scale=0.5), 1 + tr.rand(3, dim, scale=0.2)
+        DX, _, DW = backward(pkg, gpu, "fp32", s, dy, None, w, 0, eps=eps)
+        s64, g = s.double(), dy.double() * w.double()
+        r = 1 / torch.sqrt((s64 * s64).mean(1, keepdim=True) + eps)
+        ref = r * (g - s64 * r * r * (g * s64).mean(1, keepdim=True))
+        c = U * (chain(dim) + 16)
+        tol = c * ((r * g).abs() + r ** 3 * (g * s64).abs().mean(1, keepdim=True) * s64.abs()) + 2 * U * ref.abs() + 2.0 ** -149
+        tr.within(DX, ref, tol, "dx of rows of %g" % size)
+        t = dy.double() * s64 * r
+        tr.within(DW, t.sum(0), t.abs().sum(0) * U * (chain(dim) / 2 + 8 + n), "dw")
