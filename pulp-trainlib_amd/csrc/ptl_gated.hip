@@ -180,6 +180,9 @@ __global__ __launch_bounds__(256) void gate_few_kernel(const GateFew<T> a) {
 }
 template <typename T>
 static int gate_few(GateFew<T> a) {
+    const size_t n_h = (size_t)a.ns * 2 * a.outs * sizeof(T);
+    T *copy = nullptr;  // of h, where dh takes its place: workgroups read what others write over
+    if (a.h == a.dh && !(copy = static_cast<T *>(scratch(n_h + 16)))) return 2;
     const int rows = 2 * a.outs, wide = ((a.in + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC + 63) / 64, cu = state().num_cu;
     // four workgroups a compute unit, of sixteen rows and more (2 tokens, 4096 -> 8000 in fp16 with two, four, six 95, 65 and 67 us)
     int high = (int)((long)rows * wide / (4 * cu));
@@ -188,6 +191,10 @@ static int gate_few(GateFew<T> a) {
     const int groups = (rows + high - 1) / high;
     T *dx = a.dx;
     if (dx && groups > 1 && !(a.part = workspace((size_t)groups * a.ns * a.in * sizeof(float)))) return 2;
+    if (copy) {
+        rows_copy(a.h, 1, nullptr, 0, copy, (int)n_h, (int)((n_h + 15) / 16 * 16));
+        a.h = copy;
+    }
     const dim3 grid(wide, groups);
     if (a.ns == 1) hipLaunchKernelGGL((gate_few_kernel<T, 1>), grid, dim3(256), 0, state().stream, a);
     else if (a.ns == 2) hipLaunchKernelGGL((gate_few_kernel<T, 2>), grid, dim3(256), 0, state().stream, a);
@@ -231,77 +238,106 @@ static bool few_tokens(int ns, int in, int outs) {
     return fits && pays && state().gemm_path == 0;
 }
 
+// What the sums of a dense layer's backward call take at most: of each product its outputs, in rows of whole pieces whichever operand goes
+// first, and the bias' sums for every part of k, none of which is shorter than 256 bytes; or the bias' shares, one for every 128 tokens.
+template <typename T>
+static size_t dense_workspace(int ns, int in, int out) {
+    constexpr size_t KS = 256 / sizeof(T);
+    auto parts = [](size_t k) { return (k + KS - 1) / KS; };
+    return sizeof(float) * (parts(ns) * ((size_t)out + 8) * ((size_t)in + 16) + parts(out) * ((size_t)ns + 8) * ((size_t)in + 16) + (size_t)(ns / 128 + 1) * out);
+}
+
 template <typename T, typename Linear, typename Args>
 static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool wg, bool ig) {
     auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
     const size_t nx = (size_t)ns * in, ny = (size_t)ns * outs, nw = (size_t)2 * outs * in;
-    {
-        Stager sg;
-        const T *h = sg.in<T>(as(a->hidden->data), 2 * ny), *dy = sg.in<T>(as(a->output->diff), ny);
-        T *dh = sg.out<T>(as(a->hidden->diff), 2 * ny);
-        if (sg.failed()) return 2;
-        const T *x = wg ? sg.in<T>(as(a->input->data), nx) : nullptr, *w = ig ? sg.in<T>(as(a->coeff->data), nw) : nullptr;
-        T *dw = wg ? sg.out<T>(as(a->coeff->diff), nw) : nullptr, *dx = ig ? sg.out<T>(as(a->input->diff), nx) : nullptr;
-        T *db = wg && bias ? sg.out<T>(as(a->bias->diff), (size_t)2 * outs) : nullptr;
-        if (sg.failed()) return 2;
-        if ((wg || ig) && few_tokens<T>(ns, in, outs)) {
-            if (h == dh) {  // workgroups read what others write over
-                T *copy = static_cast<T *>(scratch(2 * ny * sizeof(T) + 16));
-                if (!copy) return 2;
-                rows_copy(h, 1, nullptr, 0, copy, (int)(2 * ny * sizeof(T)), (int)((2 * ny * sizeof(T) + 15) / 16 * 16));
-                h = copy;
-            }
-            GateFew<T> k = {};
-            k.h = h;
-            k.dy = dy;
-            k.x = x;
-            k.w = w;
-            k.dh = dh;
-            k.dw = dw;
-            k.dx = dx;
-            k.db = db;
-            k.ns = ns;
-            k.in = in;
-            k.outs = outs;
-            k.act = a->activation;
-            return sg.finish(gate_few(k));
-        }
-        // rows that are no whole 16-byte pieces are copied to such; dh is written a second time
-        constexpr int VEC = RowPiece<T>::VEC;
-        const int cols = (in + VEC - 1) / VEC * VEC, pitch = (2 * outs + VEC - 1) / VEC * VEC;
-        bool copy_x = ((uintptr_t)x | (uintptr_t)w) % 16 || cols != in, copy_dh = (uintptr_t)dh % 16 || pitch != 2 * outs;
-        const bool few = few_gradients<T>(ns, in, outs) && (wg || ig), own = few || own_products<T>(ns, in, outs, copy_x || copy_dh);
-        copy_x = copy_x && own;
-        copy_dh = copy_dh && own;
-        T *wide_w = nullptr, *wide_x = nullptr, *wide_dh = nullptr, *low = nullptr;
-        if (copy_x || copy_dh || few) {
-            const size_t n_w = copy_x && w ? (size_t)2 * outs * cols : 0, n_x = copy_x && x ? (size_t)ns * cols : 0, n_dh = copy_dh ? (size_t)ns * pitch : 0, n_low = few ? (size_t)ns * pitch : 0;
-            wide_w = static_cast<T *>(scratch((n_w + n_x + n_dh + n_low) * sizeof(T)));
-            if (!wide_w) return 2;
-            wide_x = wide_w + n_w;
-            if (copy_dh) wide_dh = wide_x + n_x;
-            if (few) low = wide_x + n_x + n_dh;
-            if (n_w + n_x) rows_copy(w, w ? 2 * (size_t)outs : 0, x, x ? ns : 0, wide_w, in * (int)sizeof(T), cols * (int)sizeof(T));
-        }
-        const int wide = ((outs + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC + 255) / 256;
-        int high = ns < 65535 ? ns : 65535;
-        float *part = nullptr;
-        if (own && db) {  // its sums come with the gradients of the pre-activations: eight workgroups a compute unit
+    Stager sg;
+    const T *h = sg.in<T>(as(a->hidden->data), 2 * ny), *dy = sg.in<T>(as(a->output->diff), ny);
+    T *dh = sg.out<T>(as(a->hidden->diff), 2 * ny);
+    if (sg.failed()) return 2;
+    const T *x = wg ? sg.in<T>(as(a->input->data), nx) : nullptr, *w = ig ? sg.in<T>(as(a->coeff->data), nw) : nullptr;
+    T *dw = wg ? sg.out<T>(as(a->coeff->diff), nw) : nullptr, *dx = ig ? sg.out<T>(as(a->input->diff), nx) : nullptr;
+    T *db = wg && bias ? sg.out<T>(as(a->bias->diff), (size_t)2 * outs) : nullptr;
+    if (sg.failed()) return 2;
+    if ((wg || ig) && few_tokens<T>(ns, in, outs)) {
+        GateFew<T> k = {};
+        k.h = h;
+        k.dy = dy;
+        k.x = x;
+        k.w = w;
+        k.dh = dh;
+        k.dw = dw;
+        k.dx = dx;
+        k.db = db;
+        k.ns = ns;
+        k.in = in;
+        k.outs = outs;
+        k.act = a->activation;
+        return sg.finish(gate_few(k));
+    }
+    // rows that are no whole 16-byte pieces are copied to such; dh is written a second time
+    constexpr int VEC = RowPiece<T>::VEC;
+    const int cols = (in + VEC - 1) / VEC * VEC, pitch = (2 * outs + VEC - 1) / VEC * VEC;
+    bool copy_x = ((uintptr_t)x | (uintptr_t)w) % 16 || cols != in, copy_dh = (uintptr_t)dh % 16 || pitch != 2 * outs;
+    const bool few = few_gradients<T>(ns, in, outs) && (wg || ig), own = few || own_products<T>(ns, in, outs, copy_x || copy_dh);
+    copy_x = copy_x && own;
+    copy_dh = copy_dh && own;
+    // All the memory comes before the first launch: a call that cannot have it leaves the pre-activations as they are, also where the
+    // gradients take their place.
+    T *wide_w = nullptr, *wide_x = nullptr, *wide_dh = nullptr, *low = nullptr;
+    const size_t n_w = copy_x && w ? (size_t)2 * outs * cols : 0, n_x = copy_x && x ? (size_t)ns * cols : 0, n_dh = copy_dh ? (size_t)ns * pitch : 0, n_low = few ? (size_t)ns * pitch : 0;
+    if (copy_x || copy_dh || few) {
+        wide_w = static_cast<T *>(scratch((n_w + n_x + n_dh + n_low) * sizeof(T)));
+        if (!wide_w) return 2;
+        wide_x = wide_w + n_w;
+        if (copy_dh) wide_dh = wide_x + n_x;
+        if (few) low = wide_x + n_x + n_dh;
+    }
+    const int wide = ((outs + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC + 255) / 256;
+    int high = ns < 65535 ? ns : 65535;
+    float *part = nullptr, *ws = nullptr;
+    GradParts plan = {};
+    if (own) {
+        size_t need = 0;
+        if (db) {  // its sums come with the gradients of the pre-activations: eight workgroups a compute unit
             const int most = (8 * state().num_cu + wide - 1) / wide;
             high = high < most ? high : most;
-            if (!(part = workspace((size_t)high * 2 * outs * sizeof(float)))) return 2;
+            need = (size_t)high * 2 * outs * sizeof(float);
         }
-        hipLaunchKernelGGL((gate_back_kernel<T>), dim3(wide, high), dim3(256), 0, state().stream, h, dy, dh, part, (size_t)ns, outs, a->activation,
+        if (int rc = gated_products_plan<T>(plan, wg, ig, few, ns, in, 2 * outs)) return rc;
+        // (the parts of the products' sums lie where the bias' were: they are added up by then)
+        need = need > plan.bytes ? need : plan.bytes;
+        if (need && !(ws = workspace(need))) return 2;
+        if (db) part = ws;
+    }
+    // A dense layer's call asks for its memory itself.  Where the gradients take the pre-activations' place, either there is as much as it
+    // can ask for, or it reads them from a place of their own and they are formed again over the pre-activations once it went well (64
+    // tokens, 512 -> 1408 in fp16 14.5 and 17.9 us).
+    const bool dense = !own && (wg || ig);
+    T *to = dh;
+    if (dense && h == dh) {
+        const size_t most = dense_workspace<T>(ns, in, 2 * outs);
+        const bool there = most <= ((size_t)64 << 20) && workspace_if(most);
+        if (!there && !(to = static_cast<T *>(scratch(2 * ny * sizeof(T))))) return 2;
+    }
+    auto gate_back = [&](T *out) {
+        hipLaunchKernelGGL((gate_back_kernel<T>), dim3(wide, high), dim3(256), 0, state().stream, h, dy, out, part, (size_t)ns, outs, a->activation,
                            wide_dh, low, pitch);
         if (part) row_shares<T>(part, db, 2 * outs, high);
-        int rc = hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
-        if (rc == 0 && own && (wg || ig))
-            rc = gated_products<T>(copy_x ? wide_x : x, copy_x ? wide_w : w, copy_dh ? wide_dh : dh, low, dw, dx, ns, in, 2 * outs, cols, pitch);
+        return hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
+    };
+    if (n_w + n_x) rows_copy(w, w ? 2 * (size_t)outs : 0, x, x ? ns : 0, wide_w, in * (int)sizeof(T), cols * (int)sizeof(T));
+    int rc = gate_back(to);
+    if (rc == 0 && own && (wg || ig))
+        rc = gated_products<T>(plan, ws, copy_x ? wide_x : x, copy_x ? wide_w : w, copy_dh ? wide_dh : dh, low, dw, dx, ns, in, 2 * outs, cols, pitch);
+    if (to == dh) {
         rc = sg.finish(rc);
-        if (rc || own || !(wg || ig)) return rc;
+        if (rc || !dense) return rc;
     }
+    if (rc) return rc;
     auto out = *a->hidden;  // a dense layer of 2 n_out outputs
     out.dim = 2 * outs;
+    if (to != dh) out.diff = reinterpret_cast<decltype(out.diff)>(to);
     Linear l = {};
     l.input = a->input;
     l.coeff = a->coeff;
@@ -310,7 +346,9 @@ static int gated_back(const Args *a, int ns, int in, int outs, bool bias, bool w
     l.skip_wg_grad = a->skip_wg_grad;
     l.skip_in_grad = a->skip_in_grad;
     l.use_biases = a->use_biases;
-    return linear_bw(&l, ns);
+    rc = linear_bw(&l, ns);
+    if (to == dh) return rc;
+    return sg.finish(rc ? rc : gate_back(dh));
 }
 
 template <typename T, typename Linear, typename Args>

@@ -249,37 +249,65 @@ static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const doubl
 }
 
 template <typename T>
-int gated_products(const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols, int pitch) {
+struct GradSizes {
+    static constexpr int XR = sizeof(T) == 4 ? 64 : 128, RING = GradTile<T, XR>::RING, KS = ROWB / (int)sizeof(T);
+};
+// Slabs of k of product i, of a part, and parts.
+template <typename T>
+static void grad_cut(int i, int parts, int ns, int rows, int &chunk, int &high) {
+    const int slabs = ((i ? ns : rows) + GradSizes<T>::KS - 1) / GradSizes<T>::KS;
+    chunk = (slabs + parts - 1) / parts;
+    high = (slabs + chunk - 1) / chunk;
+}
+
+template <typename T>
+int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in, int rows) {
+    constexpr int XR = GradSizes<T>::XR, KS = GradSizes<T>::KS;
     static bool ready = false;
-    constexpr int XR = sizeof(T) == 4 ? 64 : 128, RING = GradTile<T, XR>::RING, KS = ROWB / (int)sizeof(T);
     if (!ready) {
-        if (!hip_ok(hipFuncSetAttribute(reinterpret_cast<const void *>(grad_kernel<T, XR>), hipFuncAttributeMaxDynamicSharedMemorySize, RING), "hipFuncSetAttribute"))
+        if (!hip_ok(hipFuncSetAttribute(reinterpret_cast<const void *>(grad_kernel<T, XR>), hipFuncAttributeMaxDynamicSharedMemorySize, GradSizes<T>::RING),
+                    "hipFuncSetAttribute"))
             return 2;
         ready = true;
     }
-    GradArgs a = {};
-    T *y[2] = {dx, dw};
+    const bool wanted[2] = {dx, dw};
     const int n[2] = {ns, rows}, k[2] = {rows, ns};
-    int tiles[2], slabs[2], parts[2] = {1, 1};
+    int tiles[2], slabs[2];
     double values[2];
     for (int i = 0; i < 2; ++i) {
-        tiles[i] = y[i] ? (in + 127) / 128 * ((n[i] + XR - 1) / XR) : 0;
+        tiles[i] = wanted[i] ? (in + 127) / 128 * ((n[i] + XR - 1) / XR) : 0;
         slabs[i] = (k[i] + KS - 1) / KS;
         values[i] = (double)n[i] * in;
     }
+    p = {{1, 1}, 0};
     float best = 1e30f;
     for (int u = 1; u <= 32 && (u == 1 || (tiles[0] && u * 4 <= slabs[0])); u *= 2)
         for (int v = 1; v <= 32 && (v == 1 || (tiles[1] && v * 4 <= slabs[1])); v *= 2) {
-            const int p[2] = {u, v};
-            const float c = grad_cost(tiles, slabs, values, p, sizeof(T) == 4);
+            const int parts[2] = {u, v};
+            const float c = grad_cost(tiles, slabs, values, parts, sizeof(T) == 4);
             if (c < best) {
                 best = c;
-                parts[0] = u;
-                parts[1] = v;
+                p.parts[0] = u;
+                p.parts[1] = v;
             }
         }
+    for (int i = 0; i < 2; ++i) {
+        int chunk, high;
+        grad_cut<T>(i, p.parts[i], ns, rows, chunk, high);
+        const size_t parts = low && wanted[i] ? 2 * high : high;
+        if (parts > 1) p.bytes += parts * grad_part(n[i], in) * sizeof(float);
+    }
+    return 0;
+}
+
+template <typename T>
+int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols,
+                   int pitch) {
+    constexpr int XR = GradSizes<T>::XR, RING = GradSizes<T>::RING;
+    GradArgs a = {};
+    T *y[2] = {dx, dw};
+    const int n[2] = {ns, rows}, k[2] = {rows, ns};
     GradJoin<T> j = {};
-    size_t floats = 0;
     for (int i = 0; i < 2; ++i) {
         GradProd &p = a.p[i];
         p.out.y = y[i];
@@ -295,40 +323,36 @@ int gated_products(const T *x, const T *w, const T *dh, const T *low, T *dw, T *
         p.s_b = pitch * (int)sizeof(T);
         p.f_n = cols;
         p.s_n = pitch;
-        p.chunk = (slabs[i] + parts[i] - 1) / parts[i];
-        p.high = (slabs[i] + p.chunk - 1) / p.chunk;
+        grad_cut<T>(i, parts.parts[i], ns, rows, p.chunk, p.high);
         p.low = reinterpret_cast<const char *>(low);
         p.parts = low && y[i] ? 2 * p.high : p.high;
-        if (p.parts > 1) floats += (size_t)p.parts * grad_part(n[i], in);
-    }
-    if (floats) {
-        float *ws = workspace(floats * sizeof(float));
-        if (!ws) return 2;
-        for (int i = 0; i < 2; ++i) {
-            if (a.p[i].parts == 1) continue;
-            a.p[i].part = ws;
-            j.part[i] = ws;
-            j.y[i] = y[i];
-            j.values[i] = (size_t)n[i] * in;
-            j.n[i] = grad_part(n[i], in) / 4;
-            j.parts[i] = a.p[i].parts;
-            j.high[i] = a.p[i].high;
-            ws += (size_t)a.p[i].parts * grad_part(n[i], in);
-        }
+        if (p.parts == 1) continue;
+        p.part = ws;
+        j.part[i] = ws;
+        j.y[i] = y[i];
+        j.values[i] = (size_t)n[i] * in;
+        j.n[i] = grad_part(n[i], in) / 4;
+        j.parts[i] = p.parts;
+        j.high[i] = p.high;
+        ws += (size_t)p.parts * grad_part(n[i], in);
     }
     a.lead = a.p[0].chunk >= a.p[1].chunk ? 0 : 1;
-    const int groups[2] = {tiles[0] * a.p[0].parts, tiles[1] * a.p[1].parts};
+    int groups[2];
+    for (int i = 0; i < 2; ++i) groups[i] = y[i] ? a.p[i].out.tiles_w * a.p[i].out.tiles_t * a.p[i].parts : 0;
     a.first = groups[a.lead];
     hipLaunchKernelGGL((grad_kernel<T, XR>), dim3(groups[0] + groups[1]), dim3(GradTile<T, XR>::NT), RING, state().stream, a);
-    if (floats) {
+    if (parts.bytes) {
         const size_t fours = j.n[0] + j.n[1];
         hipLaunchKernelGGL((grad_join_kernel<T>), dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, state().stream, j);
     }
     return hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
 }
 
-template int gated_products<half_t>(const half_t *, const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int, int);
-template int gated_products<float>(const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int);
+template int gated_products_plan<half_t>(GradParts &, bool, bool, bool, int, int, int);
+template int gated_products_plan<float>(GradParts &, bool, bool, bool, int, int, int);
+template int gated_products<half_t>(const GradParts &, float *, const half_t *, const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int,
+                                    int);
+template int gated_products<float>(const GradParts &, float *, const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int);
 
 void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, int bytes, int pitch) {
     rows_copies(static_cast<const char *>(w), n_w, static_cast<const char *>(x), n_x, static_cast<char *>(to), bytes, pitch);

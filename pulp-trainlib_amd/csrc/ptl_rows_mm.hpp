@@ -62,10 +62,18 @@ struct Gate {
 
 // Both products behind the gradients of a gated layer's pre-activations (dw or dx NULL: not wanted).  x and w have rows of `cols` values
 // (in and more), dh of `pitch` (rows and more), all of whole 16-byte pieces; what dh has beyond `rows` is 0.  low: what dh lost when it was
-// rounded, GRAD_LOW times, in the same layout (NULL: the products are of dh as it is).
+// rounded, GRAD_LOW times, in the same layout (NULL: the products are of dh as it is).  The plan comes first: it says in how many parts k of
+// dx and of dw is taken and what workspace their sums need, `ws`, which a call has in hand before its first launch.
 constexpr float GRAD_LOW = 2048.f;
+struct GradParts {
+    int parts[2];
+    size_t bytes;
+};
 template <typename T>
-int gated_products(const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols, int pitch);
+int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in, int rows);
+template <typename T>
+int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols,
+                   int pitch);
 // Copies of n_x rows of x and n_w rows of w (either may be 0), whose rows have `bytes`, to rows of `pitch` bytes (in whole 16-byte pieces)
 // with zeros behind them, one behind the other.
 void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, int bytes, int pitch);

@@ -273,3 +273,53 @@ def test_growth_is_refused_in_a_capture(gpu, what):
     code = "import sys; sys.path[:0] = [%r, %r]; import test_gpu_transformer_block as t; t.growth_in_a_capture(%r)" % (here, os.path.dirname(here), what)
     r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
     assert r.returncode == 0 and "finished" in r.stdout, r.stdout + r.stderr
+
+
+def refused_in_place(sizes):
+    """In a process of its own: a gated layer's way back in a capture whose workspace (whose copies' memory is there) may not grow,
+    hidden->diff in the place of hidden->data.  The refused call leaves the pre-activations as they are, also when what was captured is
+    replayed, and an eager call behind it has its results."""
+    import __graft_entry__ as ge
+    pkg = ge.load_package()
+    gpu = pkg.load()
+    assert gpu.ptl_init(0) == 0
+    dt, n, i, o, path, bias = sizes
+    r = lambda s, *sh: tr.dev(tr.rand(s, *sh, dt=dt))  # noqa: E731
+    x, w, h, dy = r(1, n, i), r(2, 2 * o, i), r(3, n, 2 * o), r(4, n, o)
+    dx, dw, db = torch.full_like(x, 7), torch.full_like(w, 7), torch.full((2 * o,), 7, dtype=x.dtype, device="cuda") if bias else None
+    a, keep = tr.gated_args(pkg, i, o, 1, x=x, dx=dx, w=w, dw=dw, db=db, h=h, dh=h, dy=dy)
+    call = lambda: getattr(gpu, "ptl_gated_linear_%s_bw_batched" % dt)(ctypes.byref(a), n)  # noqa: E731
+    gpu.ptl_set_gemm_path(path)
+    assert gpu.ptl_reserve(0, 256 << 20) == 0
+    ws = ctypes.c_size_t(1)
+    before, after, side, graph = h.clone(), torch.zeros(1, device="cuda"), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    gpu.ptl_set_stream(ctypes.c_void_p(side.cuda_stream))
+    with torch.cuda.graph(graph, stream=side):
+        rc, text = call(), gpu.ptl_last_error().decode()
+        after.add_(1)
+    assert rc == 2 and "ptl_reserve" in text, (rc, text)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert float(after) == 1 and torch.equal(h, before)
+    assert call() == 0 and gpu.ptl_sync() == 0
+    gpu.ptl_reserved(ctypes.byref(ws), None)
+    assert ws.value > 0
+    over = [t.clone() for t in (h, dx, dw) + ((db,) if bias else ())]
+    h2, dh = before.clone(), torch.full_like(before, 7)
+    a, keep = tr.gated_args(pkg, i, o, 1, x=x, dx=dx, w=w, dw=dw, db=db, h=h2, dh=dh, dy=dy)
+    assert call() == 0 and gpu.ptl_sync() == 0
+    assert all(torch.equal(p, q) for p, q in zip(over, (dh, dx, dw) + ((db,) if bias else ())))
+    gpu.ptl_set_stream(None)
+    gpu.ptl_set_gemm_path(0)
+    print("finished", flush=True)
+
+
+# both products in one launch, in parts; as copies, with the sums of the bias; in two halves; a dense layer's call, by three of its routes; one kernel
+@pytest.mark.parametrize("sizes", [("fp16", 256, 2048, 2048, 0, 0), ("fp16", 257, 2045, 2047, 0, 1), ("fp16", 20, 1000, 400, 0, 0), ("fp32", 40, 300, 2000, 0, 0),
+                                   ("fp32", 200, 300, 2000, 1, 1), ("fp16", 64, 512, 1408, 0, 0), ("fp32", 2, 300, 2000, 0, 1)])
+def test_a_refused_call_leaves_what_it_reads(gpu, sizes):
+    here = os.path.dirname(os.path.abspath(__file__))
+    code = "import sys; sys.path[:0] = [%r, %r]; import test_gpu_transformer_block as t; t.refused_in_place(%r)" % (here, os.path.dirname(here), sizes)
+    r = subprocess.run([sys.executable, "-c", code], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "finished" in r.stdout, r.stdout + r.stderr
