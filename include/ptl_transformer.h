@@ -66,7 +66,7 @@ int ptl_rms_norm_fp32_bw_batched(const struct RmsNorm_args *a, int nsamples);
 int ptl_rms_norm_fp16_fw_batched(const struct RmsNorm_args_fp16 *a, int nsamples);
 int ptl_rms_norm_fp16_bw_batched(const struct RmsNorm_args_fp16 *a, int nsamples);
 
-/* Activation of a gated layer's first half. */
+/* Activation of a gated layer's first half.  Infinities have the activation's and its slope's limits (0 at -inf). */
 #define PTL_GATE_SIGMOID 0 /* 1 / (1 + exp(-x)) */
 #define PTL_GATE_SILU 1    /* x / (1 + exp(-x)) */
 #define PTL_GATE_GELU 2    /* x (1 + tanh(sqrt(2 / pi) (x + 0.044715 x^3))) / 2 */

@@ -27,10 +27,10 @@ struct RowsArgs {
 // selects, not branches: a tile has 32768 outputs a compute unit, at expf(), a division and a branch each 10 us of 200 (4096 tokens,
 // 2048 -> 5632 in fp16), this way 2.
 struct Gate {
-    float k1, k3;  // p = x (k1 + k3 x^2)
-    bool one, relu;
+    float k1, k3;  // gelu: p = x (k1 + k3 x^2)
+    bool one, relu, gelu;
     __device__ inline Gate(int act) {
-        const bool gelu = act == GATE_GELU;
+        gelu = act == GATE_GELU;
         k1 = gelu ? 1.5957691216057308f : 1.f;
         k3 = gelu ? 0.07135481627260025f : 0.f;  // 0.044715 k1
         one = act == GATE_SIGMOID;
@@ -44,16 +44,26 @@ struct Gate {
         rest = p < 0.f ? r : s;
         return p < 0.f ? s : r;
     }
+    // Infinities take the limits: the product that gives gelu's p would be 0 times infinity in the others, and at -inf the sigmoid's 0
+    // meets the lowest finite value.  GELU: 0 or 1 where it is known which, -1 otherwise.
+    template <int GELU>
+    __device__ inline float power(float x) const {
+        if constexpr (GELU == 0) return x;
+        const float p = x * fmaf(k3 * x, x, k1);
+        return GELU == 1 || gelu ? p : x;
+    }
+    __device__ inline float factor(float x) const { return one ? 1.f : fmaxf(x, -3.402823466e38f); }
+    template <int GELU = -1>
     __device__ inline float act(float x) const {
         float rest;
-        const float s = sigmoid(x * fmaf(k3 * x, x, k1), rest), f = (one ? 1.f : x) * s;
+        const float s = sigmoid(power<GELU>(x), rest), f = factor(x) * s;
         return relu ? (x < 0.f ? 0.f : x) : f;
     }
     // The derivative; f: the activation itself.
     __device__ inline float back(float x, float &f) const {
         float rest;
-        const float s = sigmoid(x * fmaf(k3 * x, x, k1), rest), slope = s * rest;  // of sigmoid, to p
-        f = relu ? (x < 0.f ? 0.f : x) : (one ? 1.f : x) * s;
+        const float s = sigmoid(power<-1>(x), rest), slope = s * rest;  // of sigmoid, to p
+        f = relu ? (x < 0.f ? 0.f : x) : factor(x) * s;
         // d p / d x = k1 + 3 k3 x^2; far from 0 the slope is 0, whatever that grows to
         const float d = slope > 0.f ? slope * (one ? 1.f : x * fmaf(3.f * k3 * x, x, k1)) : (x != x ? x : 0.f);
         return relu ? (x > 0.f ? 1.f : x != x ? x : 0.f) : one ? d : s + d;

@@ -355,3 +355,40 @@ def test_backward_of_few_tokens_is_the_same_in_every_call(pkg, gpu):
         assert gpu.ptl_sync() == 0
         first = first or [t.clone() for t in (dh, dx, dw)]
         assert all(torch.equal(p, q) for p, q in zip(first, (dh, dx, dw)))
+
+
+LIMITS = {"silu": (float("inf"), 0.0), "gelu": (float("inf"), 0.0), "relu": (float("inf"), 0.0), "sigmoid": (1.0, 0.0)}  # at +inf, at -inf
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n", [1, 3, 70, 700])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+def test_infinite_gates(pkg, gpu, dt, n, act):
+    """A gate of +-inf (of a bias, forward; as an overflow of fp16 is kept, backward) takes the activation's limit and the slope's, and
+    a NaN stays one."""
+    n_in, n_out = 33, 40
+    x, w, b = inputs(5, dt, n, n_in, n_out, 1)
+    b[3], b[4], b[5] = float("inf"), -float("inf"), float("nan")
+    y, h = forward(pkg, gpu, dt, act, x, w, b)
+    up = (x.double() @ w.double().t() + b.double())[:, n_out:]
+    high, low = LIMITS[act]
+    got = y.double().cpu()
+    if high == 1:
+        off = U * (n_in + 2) * (x.double().abs() @ w.double().abs().t() + b.double().abs())[:, n_out + 3] + tr.step(up[:, 3], dt) + 4 * U * up[:, 3].abs()
+        tr.within(got[:, 3], up[:, 3], off)
+    else:
+        assert torch.equal(got[:, 3], torch.sign(up[:, 3]) * high)
+    assert (got[:, 4] == low).all() and torch.isnan(got[:, 5]).all() and torch.isfinite(torch.cat([got[:, :3], got[:, 6:]], 1)).all()
+    dy = tr.rand(6, n, n_out, scale=0.5, dt=dt)
+    hidden = h.cpu()
+    dh = backward(pkg, gpu, dt, act, x, w, hidden, dy, 1)[0].double().cpu()
+    d, u = dy.double(), hidden[:, n_out:].double()
+    slope = 0.0 if act == "sigmoid" else 1.0
+    want = d[:, 3] * u[:, 3] * slope
+    tr.within(dh[:, 3], want, tr.step(want, dt) + 4 * U * want.abs())
+    assert (dh[:, 4] == 0).all()
+    if high == 1:
+        tr.within(dh[:, n_out + 3], d[:, 3], tr.step(d[:, 3], dt) + 4 * U * d[:, 3].abs())
+    else:
+        assert torch.equal(dh[:, n_out + 3], torch.sign(d[:, 3]) * high)
+    assert (dh[:, n_out + 4] == 0).all() and torch.isnan(dh[:, [5, n_out + 5]]).all()
