@@ -54,3 +54,35 @@ def test_more_outputs_than_a_call_forms(pkg, gpu):
     a.N = 2 ** 24 + 3
     assert gpu.ptl_mm_int8_fp16(ctypes.byref(a)) == 0 and gpu.ptl_sync() == 0
     assert bool((C[:a.N] == 1).all()) and bool((C[a.N:] == 7).all())
+
+
+def test_norm_backward(pkg, gpu):
+    """The gradients of all rows, of two values each, and the weights' gradient, a sum over all rows, against the sum in 64 bits (formed on the device, in parts)."""
+    g = torch.Generator(device="cuda").manual_seed(3)
+    for dt in ("fp16", "fp32"):
+        t = tr.t_dtype(dt)
+        s, dy = (torch.randn(N, 2, dtype=t, device="cuda", generator=g) for _ in range(2))
+        dy = (s + dy * 0.3) * 5e-4  # (so that the weights' gradient is as large as its terms' sum, and no infinity in fp16)
+        w = torch.tensor([1.5, -0.75], dtype=t, device="cuda")
+        dx, dw = torch.full_like(s, 7), torch.full_like(w, 7)
+        a, keep = tr.norm_args(pkg, 2, x=s, dx=dx, w=w, dw=dw, dy=dy, eps=1e-5)
+        pkg.call("ptl_rms_norm_%s_bw_batched" % dt, a, N)
+        assert gpu.ptl_sync() == 0
+        total, size, off = torch.zeros(2, dtype=torch.float64), torch.zeros(2, dtype=torch.float64), 0.0
+        for at in range(0, N, 1 << 22):
+            part = slice(at, min(at + (1 << 22), N))
+            x, d = s[part].double(), dy[part].double()
+            r = 1 / torch.sqrt((x * x).mean(1, keepdim=True) + 1e-5)
+            v = d * x * r
+            total += v.sum(0).cpu()
+            size += v.abs().sum(0).cpu()
+            h = d * w.double()
+            ref = r * (h - x * r * r * (h * x).mean(1, keepdim=True))
+            # sums of two terms and a dozen roundings of either term, and the result's own
+            tol = 32 * tr.U * ((r * h).abs() + (x * r).abs() * r * (h * x * r).abs().mean(1, keepdim=True)) + (ref.abs() * 2.0 ** -11 + 2.0 ** -25 if dt == "fp16" else 0)
+            off = max(off, float(((dx[part].double() - ref).abs() - tol).max()))
+        assert off <= 0, dt
+        # a wave's chain: N rows over the waves of at most sqrt(72 N sizeof) workgroups of four; fp16: the workgroups' sums in 32 chains
+        groups = int((72.0 * N * s.element_size()) ** 0.5)
+        c = N / (4 * groups) + 16 + (groups / 32 + 32 if dt == "fp16" else 0)
+        tr.within(dw, total, size * tr.U * c + tr.step(total, dt), "dw " + dt)
