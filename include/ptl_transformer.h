@@ -7,10 +7,13 @@
  * Conventions are those of ptl_api.h, which includes this file: blobs describe ONE sample (a token) of `dim` elements,
  * sample n lies at data + n * dim; pointers may be host or device pointers; the calls return 0, 1 after rejecting their
  * arguments (message printed, outputs untouched) or 2 where a HIP call failed, and run on the library's stream.
- * nsamples <= 0 is an empty batch: nothing is read or written, 0 is returned.  A call takes at most 2^30 samples, and a
- * product as many outputs as 2^31 threads form (some 4 * 10^9 and more; 33 million outputs of a few tokens); larger ones
- * are rejected.  Tensors a call writes must not overlap
- * those it reads or the other ones it writes except where a comment says so.
+ * nsamples <= 0 is an empty batch: nothing is read or written, 0 is returned.  A call takes at most 2^30 samples of at most
+ * 2^30 elements, a gated layer at most 2^27 inputs and fewer than 2^29 outputs, its backward call tensors of less than 2^31
+ * elements (samples times elements, and the weights), and a product as many outputs as 2^31 threads form (some 4 * 10^9 and
+ * more; 33 million outputs of a few tokens); larger ones are rejected.  Tensors a call writes must not overlap those it reads
+ * or the other ones it writes except where a comment says so.  A call that gets no memory (status 2) leaves what it reads as
+ * it was, also a tensor that its results would have replaced; other outputs may be written in part.  Sums and products in fp32
+ * that leave its range count as infinite.
  */
 #ifndef PTL_TRANSFORMER_H
 #define PTL_TRANSFORMER_H
@@ -82,7 +85,8 @@ int ptl_rms_norm_fp16_bw_batched(const struct RmsNorm_args_fp16 *a, int nsamples
  *             coeff->diff = hidden->diff^T * input->data (sum over the samples) and, with use_biases, bias->diff = the sum of
  *             hidden->diff, unless skip_wg_grad; input->diff = hidden->diff * coeff unless skip_in_grad.  hidden->diff is
  *             always written and is what the products and sums read, rounded to the tensor type as it is stored (fp16 calls of up
- *             to two samples or fewer than 16384 values: as it was before that); it may be hidden->data (the pre-activations are lost then). */
+ *             to two samples or fewer than 16384 values: as it was before that, unless ptl_set_gemm_path() asks for another way); it
+ *             may be hidden->data (the pre-activations are lost then). */
 struct GatedLinear_args {
     struct blob *input;
     struct blob *coeff;
@@ -147,7 +151,7 @@ int ptl_mm_int8_fp16(const struct matMul_int8_args_fp16 *a);
  *   p = softmax over the row's entries of teacher / temperature;  q = softmax over all classes of output / temperature
  *   wr_loss[row] = weight * sum p (log p - log q);   output->diff = weight / temperature * (q * sum p - p)
  * A row without entries (or whose entries are all -inf) has loss 0 and gradient 0.  Logits of -inf (classes that are masked
- * out) are allowed.  temperature: 1e-6 .. 1e6.  step: 0 the losses, 1 the gradient, 2 both in one pass.  output->diff may be output->data. */
+ * out) are allowed; a row in which all are has no probabilities, and NaN for what an entry asks of it.  temperature: 1e-6 .. 1e6.  step: 0 the losses, 1 the gradient, 2 both in one pass.  output->diff may be output->data. */
 struct distill_args {
     struct blob *output;
     float *teacher;

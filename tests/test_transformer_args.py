@@ -181,3 +181,18 @@ def test_more_samples_than_a_call_takes(pkg, dt):
     a.N = many
     refused(pkg, "ptl_mm_int8_" + dt, a, says="geometry")
     assert (y == 7).all()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+def test_larger_layers_than_a_call_takes(pkg, dt):
+    t = np.float32 if dt == "fp32" else np.float16
+    x, y = np.ones((2, 8), t), np.full((2, 8), 7, t)
+    for step in ("fw", "bw"):
+        name = "ptl_gated_linear_%s_%s_batched" % (dt, step)
+        for n_in, n_out in ((2 ** 27 + 1, 4), (8, 2 ** 29)):
+            a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=x, dx=y, w=x, dw=y, h=x, dh=y, y=y, dy=x)
+            refused(pkg, name, a, 2, says="geometry")
+    for n, n_in, n_out in ((2 ** 10, 2 ** 21, 1), (2 ** 10, 1, 2 ** 20), (1, 2 ** 20, 2 ** 10)):  # inputs, pre-activations, weights of 2^31
+        a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=x, dx=y, w=x, dw=y, h=x, dh=y, y=y, dy=x)
+        refused(pkg, name, a, n, says="2^31")
+    assert (y == 7).all() and (x == 1).all()
