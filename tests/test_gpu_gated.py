@@ -392,3 +392,26 @@ def test_infinite_gates(pkg, gpu, dt, n, act):
     else:
         assert torch.equal(dh[:, n_out + 3], torch.sign(d[:, 3]) * high)
     assert (dh[:, n_out + 4] == 0).all() and torch.isnan(dh[:, [5, n_out + 5]]).all()
+
+
+@pytest.mark.parametrize("dt,n,n_in,n_out,path", [("fp32", 1000, 512, 1000, 0), ("fp16", 2000, 512, 1000, 1), ("fp32", 1001, 513, 999, 1)])
+def test_backward_in_place_with_gradients_of_their_own(pkg, gpu, dt, n, n_in, n_out, path):
+    """Layers whose gradients are a dense layer's call that could ask for more than 64 MB: it reads the pre-activations' gradients from a
+    place of their own, and they take the pre-activations' place behind it.  Tensors of the device and of the host, each gradient alone."""
+    x, w, _ = inputs(n, dt, n, n_in, n_out, 0)
+    h, dy = tr.rand(n + 5, n, 2 * n_out, scale=1.5, dt=dt), tr.rand(n + 6, n, n_out, scale=0.5, dt=dt)
+    gpu.ptl_set_gemm_path(path)
+    try:
+        for more in ({}, {"skip_wg": 1}, {"skip_ig": 1}):
+            full = backward(pkg, gpu, dt, "silu", x, w, h, dy, 1, **more)
+            over = backward(pkg, gpu, dt, "silu", x, w, h, dy, 1, over=1, **more)
+            assert all(torch.equal(a, b) for a, b in zip(over, full)), more
+        want = backward(pkg, gpu, dt, "silu", x, w, h, dy, 1)
+        z = lambda *s: torch.full(s, 7, dtype=x.dtype).numpy()  # noqa: E731
+        dx, dw, db, hh = z(n, n_in), z(2 * n_out, n_in), z(2 * n_out), h.numpy().copy()
+        a, keep = tr.gated_args(pkg, n_in, n_out, 1, x=x.numpy(), dx=dx, w=w.numpy(), dw=dw, db=db, h=hh, dh=hh, dy=dy.numpy())
+        pkg.call("ptl_gated_linear_%s_bw_batched" % dt, a, n)
+        for got, ref in zip((hh, dx, dw, db), want):
+            assert torch.equal(torch.from_numpy(got), ref.cpu())
+    finally:
+        gpu.ptl_set_gemm_path(0)

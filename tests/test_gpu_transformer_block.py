@@ -306,6 +306,17 @@ def refused_in_place(sizes):
     gpu.ptl_reserved(ctypes.byref(ws), None)
     assert ws.value > 0
     over = [t.clone() for t in (h, dx, dw) + ((db,) if bias else ())]
+    again = torch.cuda.CUDAGraph()  # with what the eager call has left reserved it is captured
+    with torch.cuda.graph(again, stream=side):
+        assert call() == 0, gpu.ptl_last_error()
+    for _ in range(3):
+        h.copy_(before)
+        for t in (dx, dw):
+            t.fill_(7)
+        torch.cuda.synchronize()
+        again.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(over, (h, dx, dw)))
     h2, dh = before.clone(), torch.full_like(before, 7)
     a, keep = tr.gated_args(pkg, i, o, 1, x=x, dx=dx, w=w, dw=dw, db=db, h=h2, dh=dh, dy=dy)
     assert call() == 0 and gpu.ptl_sync() == 0
