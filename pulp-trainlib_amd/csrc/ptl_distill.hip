@@ -7,8 +7,8 @@
 // into parts of a workgroup each: one launch leaves every part's maximum and sum, the next one joins them and writes.
 // The teacher's entries (tens to hundreds) are worked on by the same workgroup once the row's sum is known: the gradient of
 // a class that is named is written a second time, behind a barrier, by the first entry that names it.
-// Measured, loss and gradient: 2048 rows of 32000 classes in fp16 60 us (4.4 TB/s), in fp32 111 (4.7); 256 rows of 131072 29 us, in
-// fp32 (read twice) 76; 4 rows of 50000 8.4 us in two launches; a few short rows 4 us.
+// Measured, loss and gradient: 2048 rows of 32000 classes in fp16 60 us (4.4 TB/s), in fp32 111 (4.7); 256 rows of 131072 34 us, in
+// fp32 (read twice) 76; 4 rows of 50000 8.7 us in two launches; a few short rows 4 us.
 #include "ptl_rows.hpp"
 #include "ptl_transformer.h"
 

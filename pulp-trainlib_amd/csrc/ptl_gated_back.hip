@@ -11,7 +11,7 @@
 //     slower).  The two products' tiles differ in length (2 n_out against the number of tokens): the longer ones come first in the grid and the
 //     shorter ones fill up behind them.
 //   * Where that leaves compute units idle k is cut into parts, each with sums of its own in fp32, which another launch adds up.
-// fp16, 2048 tokens, 2048 -> 5632: 205 us (920 TFLOP/s; with the gradients of the pre-activations 227 to 233), as a dense layer's call 245;
+// fp16, 2048 tokens, 2048 -> 5632: 205 us (920 TFLOP/s; with the gradients of the pre-activations 226 to 235), as a dense layer's call 245;
 // 256 tokens of the same layer 58 and 82, 64 tokens 31 and 49.  fp32, 2048 tokens, 1024 -> 2816: 391 us (121 TFLOP/s) and 461.
 // Rows that are no whole 16-byte pieces come as copies (rows_copy(), gate_back_kernel): fp16, 2047 -> 5631 252 us with them.
 // Tried: slabs of 32 k, four of them in flight, instead of two of 64: 3 to 8 % longer.
