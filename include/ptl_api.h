@@ -26,6 +26,7 @@
 
 #include "ptl_structs.h"
 #include "ptl_transformer.h"
+#include "ptl_tuning.h"
 
 #ifdef __cplusplus
 extern "C" {

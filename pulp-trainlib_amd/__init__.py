@@ -123,6 +123,13 @@ ROW_ENTRY_POINTS = ["ptl_%s_%s_%s_batched" % (n, dt, step) for n in ("rms_norm",
 INT8_ENTRY_POINTS = ["ptl_mm_int8_fp32", "ptl_mm_int8_fp16"]
 DISTILL_ENTRY_POINTS = ["ptl_distill_fp32_batched", "ptl_distill_fp16_batched"]
 
+# include/ptl_tuning.h: `int f(const args *, int nsamples)`, `int f(const args *, int nsamples, int step)`,
+# `int f(const adamw_args *list, int count, const adamw_step *)`
+TUNING_ENTRY_POINTS = ["ptl_%s_%s_%s_batched" % (n, dt, step) for n in ("act_linear", "norm_join") for dt in ("fp32", "fp16")
+                       for step in ("fw", "bw")]
+POLICY_ENTRY_POINTS = ["ptl_policy_loss_fp32_batched", "ptl_policy_loss_fp16_batched"]
+ADAMW_ENTRY_POINTS = ["ptl_adamw_fp32_multi", "ptl_adamw_fp16_multi"]
+
 OTHER_ENTRY_POINTS = ["ptl_init", "ptl_last_error", "ptl_last_status", "ptl_set_stream", "ptl_sync", "ptl_set_gemm_path",
                       "ptl_last_conv_direct", "ptl_last_gemm_streamed", "ptl_last_conv_resident", "ptl_last_gemm_tile", "ptl_last_gemm_form", "ptl_staging_copies", "ptl_timer_begin", "ptl_timer_end_ms", "ptl_mm_fp32", "ptl_mm_fp16", "ptl_copy_bytes",
                       "ptl_reserve", "ptl_reserved", "ptl_probe_mfma_fp16"]
@@ -141,17 +148,21 @@ def load():
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p]
         f.restype = None
-    for name in BATCHED_ENTRY_POINTS + ROW_ENTRY_POINTS:
+    for name in BATCHED_ENTRY_POINTS + ROW_ENTRY_POINTS + TUNING_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p, ctypes.c_int]
         f.restype = ctypes.c_int
-    for name in STEP_ENTRY_POINTS + DISTILL_ENTRY_POINTS:
+    for name in STEP_ENTRY_POINTS + DISTILL_ENTRY_POINTS + POLICY_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_int]
         f.restype = ctypes.c_int
     for name in PLAIN_ENTRY_POINTS + INT8_ENTRY_POINTS:
         f = getattr(lib, name)
         f.argtypes = [ctypes.c_void_p]
+        f.restype = ctypes.c_int
+    for name in ADAMW_ENTRY_POINTS:
+        f = getattr(lib, name)
+        f.argtypes = [ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p]
         f.restype = ctypes.c_int
     for name in FUSED_NORM_ENTRY_POINTS:
         f = getattr(lib, name)

@@ -9,7 +9,7 @@
 // a class that is named is written a second time, behind a barrier, by the first entry that names it.
 // Measured, loss and gradient: 2048 rows of 32000 classes in fp16 60 us (4.4 TB/s), in fp32 111 (4.7); 256 rows of 131072 34 us, in
 // fp32 (read twice) 76; 4 rows of 50000 8.7 us in two launches; a few short rows 4 us.
-#include "ptl_rows.hpp"
+#include "ptl_soft_rows.hpp"
 #include "ptl_transformer.h"
 
 namespace ptl {
@@ -25,7 +25,7 @@ struct DistillEntry {
     float pad[3];
 };
 template <typename T>
-struct DistillArgs {
+struct DistillArgs : SoftScale {
     const T *z, *u;
     const int *at;
     T *grad;      // (NULL: not wanted)
@@ -33,80 +33,8 @@ struct DistillArgs {
     float2 *part;  // of each part of a row: its largest logit, the sum of exponentials relative to that
     struct DistillEntry *entry;  // of each row, behind those: what the first launch finds out about the teacher's entries
     int rows, first, dim, top, parts, per_part;  // first: the launch's first row; per_part: pieces
-    float inv_t, hi, lo, least;  // 1 / T; log2(e) / T as the sum of two floats above 0; z - m from which on exp((z - m) / T) is 0
     float weight, scale;  // scale = weight / T
 };
-
-// exp((z - m) / T) of an entry: the exponent as the sum of two floats, the second of which corrects the result.
-template <typename T>
-__device__ inline float distill_exp(float z, float m, const DistillArgs<T> &a) {
-    float d = z - m;
-    d = d < a.least ? a.least : d;  // (0 from there on, -inf too; NaN stays)
-    const float y = d * a.hi, r = fmaf(d, a.hi, -y) + d * a.lo, e = __builtin_amdgcn_exp2f(y);
-    return fmaf(e, r * 0.693147181f, e);
-}
-// ... and of all the classes.  fp32: the exponent is rounded to 2^-24 of itself, which reaches steps of the result only in classes far
-// below the largest (corrected as well: 2048 rows of 32000 124 us, 111 so).  fp16: a fused multiply-add on the value as it was read, less
-// m / T rounded to fp32, and what that rounding took away: it is the same for the whole row, but as large as 2^-24 of m / T, and the
-// loss and the classes that the teacher names compare the sum with logits relative to m (2048 rows of 32000: 59.7 us, 58.7 without it, 60.7
-// with m subtracted first, 75 in the form of fp32; the walks over a row are bound by their instructions).
-template <typename T>
-struct DistillExp {
-    float m, rest;
-    const DistillArgs<T> &a;
-    __device__ inline DistillExp(float max, const DistillArgs<T> &a) : a(a) {
-        if constexpr (sizeof(T) == 4) {
-            m = max;
-        } else {  // (an infinite maximum gives NaN in every class, as z - m does)
-            m = -max * a.hi;
-            rest = fmaf(-max, a.hi, -m);
-        }
-    }
-    __device__ inline float operator()(T z) const {
-        if constexpr (sizeof(T) == 4) {
-            const float d = z - m;
-            return __builtin_amdgcn_exp2f(fmaf(d, a.hi, d * a.lo));
-        } else {
-            return __builtin_amdgcn_exp2f(fmaf((float)z, a.hi, m) + rest);
-        }
-    }
-};
-
-// NT threads have a row: a workgroup, or (64) one wave of a workgroup of four, which needs no barriers.
-template <int NT>
-__device__ inline int row_thread() { return NT == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x; }
-template <int NT>
-__device__ inline void row_sync() {
-    if constexpr (NT == 64) {
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-    } else {
-        __syncthreads();
-    }
-}
-template <int NT>
-__device__ inline void row_sync_wave() {  // where a reduction follows, which is a barrier for a workgroup
-    if constexpr (NT == 64) row_sync<NT>();
-}
-// Two values over them.  `lds` holds two floats per wave and is not written again before another barrier.
-template <int NT, bool MAX>
-__device__ inline void group_reduce(float (&v)[2], float *lds) {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) v[i] = MAX ? wave_max(v[i]) : wave_sum(v[i]);
-    if constexpr (NT == 64) return;
-    if ((threadIdx.x & 63) == 0) *reinterpret_cast<float2 *>(lds + 2 * (threadIdx.x >> 6)) = make_float2(v[0], v[1]);
-    __syncthreads();
-    const float2 r = *reinterpret_cast<const float2 *>(lds + 2 * (threadIdx.x & (NT / 64 - 1)));
-    v[0] = r.x;
-    v[1] = r.y;
-#pragma unroll
-    for (int off = NT / 128; off > 0; off >>= 1)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            const float o = __shfl_xor(v[i], off);
-            v[i] = MAX ? fmaxf(v[i], o) : v[i] + o;
-        }
-}
 
 // In LDS: room for three reductions, then `top` (in whole fours) each of classes, logits of the teacher (later probabilities) and
 // of the student (later gradients).
@@ -175,7 +103,7 @@ template <typename T, int NT>
 __device__ inline float distill_total(const DistillArgs<T> &a, const DistillTop &t, float &um) {
     if (um == -__builtin_inff()) um = 0.f;
     float s = 0.f;
-    for (int i = row_thread<NT>(); i < a.top; i += NT) s += distill_exp(t.p[i], um, a);
+    for (int i = row_thread<NT>(); i < a.top; i += NT) s += soft_exp(t.p[i], um, a);
     return s;
 }
 
@@ -184,7 +112,7 @@ template <typename T, int NT, typename F>
 __device__ inline void distill_probabilities(const DistillArgs<T> &a, const DistillTop &t, float um, float total, F f) {
     const float inv_total = total != 0.f ? 1.f / total : 0.f;
     for (int i = row_thread<NT>(); i < a.top; i += NT) {
-        const float u = t.p[i], p = distill_exp(u, um, a) * inv_total;
+        const float u = t.p[i], p = soft_exp(u, um, a) * inv_total;
         f(i, p, u - um);
         t.p[i] = p;
     }
@@ -222,94 +150,6 @@ __device__ inline float distill_term(float p, float log_p, float zc, float m, fl
     return p != 0.f ? p * (log_p - ((zc - m) * a.inv_t - log_sum)) : 0.f;
 }
 
-// NP pieces of logits in each of NT threads, from piece `first` on.  MINE: each piece has its own classes only, and what the row does
-// not have is -inf; else a thread may have classes that are another's too (RowPiece::cut), which only the sum has to know.
-template <typename T, int NT, int NP, bool MINE>
-__device__ inline void distill_hold(RowPiece<T> (&z)[NP], const T *row, int first, int end, int dim) {
-    constexpr int VEC = RowPiece<T>::VEC;
-    constexpr bool SHORT = NP == 1;  // rows of less than a piece: one piece a thread
-    if (!MINE && !(SHORT && dim < VEC)) {
-#pragma unroll
-        for (int j = 0; j < NP; ++j) z[j].template hold<false>(row, first + j * NT + row_thread<NT>(), dim);
-        return;
-    }
-#pragma unroll
-    for (int j = 0; j < NP; ++j) z[j].fetch(row, min(first + j * NT + row_thread<NT>(), end - 1), dim);
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int p = first + j * NT + row_thread<NT>();
-        z[j].trim(min(p, end - 1), dim);
-        if (!__any(p >= end || (p + 1) * VEC > dim)) continue;
-#pragma unroll
-        for (int i = 0; i < VEC; ++i)
-            if (p >= end || p * VEC + i >= dim) z[j].e[i] = (T)-__builtin_inff();
-    }
-}
-// Between two walks over the registers: what one converted is not kept for the next (fp16: twice the registers).
-template <typename T, int NP>
-__device__ inline void distill_as_read(RowPiece<T> (&z)[NP]) {
-#pragma unroll
-    for (int j = 0; j < NP; ++j) asm volatile("" : "+v"(z[j].raw));
-}
-template <typename T, int NP>
-__device__ inline float distill_max(const RowPiece<T> (&z)[NP]) {
-    if constexpr (sizeof(T) == 2) {  // (two at a time)
-        typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-        h2 m = {(T)-__builtin_inff(), (T)-__builtin_inff()};
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const unsigned w[4] = {z[j].raw.x, z[j].raw.y, z[j].raw.z, z[j].raw.w};
-#pragma unroll
-            for (int i = 0; i < 4; ++i) m = __builtin_elementwise_max(m, __builtin_bit_cast(h2, w[i]));
-        }
-        return fmaxf((float)m.x, (float)m.y);
-    } else {
-        float m = -__builtin_inff();
-#pragma unroll
-        for (int j = 0; j < NP; ++j)
-#pragma unroll
-            for (int i = 0; i < RowPiece<T>::VEC; ++i) m = fmaxf(m, (float)z[j].e[i]);
-        return m;
-    }
-}
-template <typename T, int NT, int NP, bool MINE>
-__device__ inline float distill_sum(const RowPiece<T> (&z)[NP], const DistillExp<T> &e, int dim) {
-    float s = 0.f;
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int cut = MINE ? 0 : RowPiece<T>::cut(j * NT + row_thread<NT>(), dim);
-        if (!MINE && __any(cut)) {
-#pragma unroll
-            for (int i = 0; i < RowPiece<T>::VEC; ++i) s += i < cut ? 0.f : e(z[j].e[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < RowPiece<T>::VEC; ++i) s += e(z[j].e[i]);
-        }
-    }
-    return s;
-}
-// The gradient of the classes that are held.
-template <typename T, int NT, int NP, bool MINE>
-__device__ inline void distill_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const DistillExp<T> &e, float f, bool some, int dim) {
-    int mine = first + row_thread<NT>();
-    asm volatile("" : "+v"(mine));  // (the loads' addresses are not kept for the stores)
-#pragma unroll
-    for (int j = 0; j < NP; ++j) {
-        const int p = mine + j * NT;
-        RowPiece<T> o;
-        if (some) {
-#pragma unroll
-            for (int i = 0; i < RowPiece<T>::VEC; ++i) o.e[i] = row_round<T>(e(z[j].e[i]) * f);
-        } else {
-            o.raw = row_u4{0, 0, 0, 0};
-        }
-        if (MINE) {
-            if (p < end) o.store(row, p, dim);
-        } else {
-            o.template put<NP == 1>(row, p, dim);
-        }
-    }
-}
 // NP = 0: the row is read twice.
 template <typename T, int NT, int NP>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_row_kernel(const DistillArgs<T> a) {
@@ -326,33 +166,33 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_row_kernel(const 
     RowPiece<T> z[HELD];
     float top[2], own = 0.f, sum[2] = {0.f, 0.f};  // of the student, of the teacher
     if constexpr (NP > 0) {
-        distill_hold<T, NT, HELD, MINE>(z, zr, 0, pieces, a.dim);
+        soft_hold<T, NT, HELD, MINE>(z, zr, 0, pieces, a.dim);
         top[1] = distill_fetch<T, NT>(a, row, t);
-        top[0] = distill_max<T>(z);
+        top[0] = soft_max<T>(z);
     } else {
         // maximum and sum in one walk: a thread's sum is to its own largest logit so far
         top[1] = distill_fetch<T, NT>(a, row, t);
         top[0] = -__builtin_inff();
         for (int p = 0; p < pieces; p += NT * HELD) {
-            distill_hold<T, NT, HELD, MINE>(z, zr, p, pieces, a.dim);
-            const float m = fmaxf(top[0], distill_max<T>(z));
+            soft_hold<T, NT, HELD, MINE>(z, zr, p, pieces, a.dim);
+            const float m = fmaxf(top[0], soft_max<T>(z));
             // (as long as all are -inf: sums of 0, and of NaN, which is no maximum)
-            const float part = distill_sum<T, NT, HELD, MINE>(z, DistillExp<T>(m == -__builtin_inff() ? 0.f : m, a), a.dim);
-            sum[0] = part + (top[0] == -__builtin_inff() ? sum[0] : sum[0] * distill_exp(top[0], m, a));
+            const float part = soft_sum<T, NT, HELD, MINE>(z, SoftExp<T>(m == -__builtin_inff() ? 0.f : m, a), a.dim);
+            sum[0] = part + (top[0] == -__builtin_inff() ? sum[0] : sum[0] * soft_exp(top[0], m, a));
             top[0] = m;
         }
         own = top[0];
     }
     row_sync_wave<NT>();
     group_reduce<NT, true>(top, t.red);
-    const DistillExp<T> e(top[0], a);
+    const SoftExp<T> e(top[0], a);
     distill_insert<T, NT>(a, t);
     if constexpr (NP > 0) {
-        distill_as_read<T>(z);
-        sum[0] = distill_sum<T, NT, HELD, MINE>(z, e, a.dim);
-        distill_as_read<T>(z);
+        soft_as_read<T>(z);
+        sum[0] = soft_sum<T, NT, HELD, MINE>(z, e, a.dim);
+        soft_as_read<T>(z);
     } else {
-        if (own != -__builtin_inff()) sum[0] *= distill_exp(own, top[0], a);
+        if (own != -__builtin_inff()) sum[0] *= soft_exp(own, top[0], a);
     }
     sum[1] = distill_total<T, NT>(a, t, top[1]);
     row_sync_wave<NT>();
@@ -372,17 +212,17 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void distill_row_kernel(const 
     distill_merge<T, NT>(a, t, twice);
     const float f = a.scale / sum[0];
     if constexpr (NP > 0) {
-        distill_put<T, NT, HELD, MINE>(z, gr, 0, pieces, e, f, some, a.dim);
+        soft_put<T, NT, HELD, MINE>(z, gr, 0, pieces, e, f, some, a.dim);
     } else {
         for (int p = 0; p < pieces; p += NT * HELD) {
-            distill_hold<T, NT, HELD, MINE>(z, zr, p, pieces, a.dim);
-            distill_put<T, NT, HELD, MINE>(z, gr, p, pieces, e, f, some, a.dim);
+            soft_hold<T, NT, HELD, MINE>(z, zr, p, pieces, a.dim);
+            soft_put<T, NT, HELD, MINE>(z, gr, p, pieces, e, f, some, a.dim);
         }
     }
     row_sync<NT>();  // behind all of those, the classes that the entries name
     for (int i = row_thread<NT>(); i < a.top; i += NT) {
         const int c = t.to[i];
-        if (c >= 0) gr[c] = some ? (T)(a.scale * (distill_exp(t.zc[i], top[0], a) / sum[0] - t.sum[i])) : (T)0.f;
+        if (c >= 0) gr[c] = some ? (T)(a.scale * (soft_exp(t.zc[i], top[0], a) / sum[0] - t.sum[i])) : (T)0.f;
     }
 }
 
@@ -419,12 +259,12 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_part_kernel(const DistillA
     const int part = (int)blockIdx.x - 1;
     const int pieces = (a.dim + VEC - 1) / VEC, first = part * a.per_part, end = min(first + a.per_part, pieces);
     RowPiece<T> z[NP];
-    distill_hold<T, NT, NP, true>(z, a.z + row * a.dim, first, end, a.dim);
-    float m[2] = {distill_max<T>(z), 0.f}, s[2] = {0.f, 0.f};
+    soft_hold<T, NT, NP, true>(z, a.z + row * a.dim, first, end, a.dim);
+    float m[2] = {soft_max<T>(z), 0.f}, s[2] = {0.f, 0.f};
     group_reduce<NT, true>(m, t.red);
     // (a part of nothing but -inf adds nothing to a row that has more; a NaN among them is no maximum, but in the sum)
-    const DistillExp<T> e(m[0] == -__builtin_inff() ? 0.f : m[0], a);
-    s[0] = distill_sum<T, NT, NP, true>(z, e, a.dim);
+    const SoftExp<T> e(m[0] == -__builtin_inff() ? 0.f : m[0], a);
+    s[0] = soft_sum<T, NT, NP, true>(z, e, a.dim);
     group_reduce<NT, false>(s, t.red + 32);
     if (threadIdx.x == 0) a.part[row * (a.parts + 1) + part] = make_float2(m[0], s[0]);
 }
@@ -438,14 +278,14 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_join_kernel(const DistillA
     const float2 *part = a.part + row * (a.parts + 1);
     const DistillEntry *entry = a.entry + row * a.top;
     RowPiece<T> z[NP];
-    if (a.grad) distill_hold<T, NT, NP, true>(z, a.z + row * a.dim, first, end, a.dim);
+    if (a.grad) soft_hold<T, NT, NP, true>(z, a.z + row * a.dim, first, end, a.dim);
     const bool some = part[a.parts].x != 0.f;
     float top[2] = {-__builtin_inff(), 0.f}, sum[2] = {0.f, 0.f};
     for (int i = threadIdx.x; i < a.parts; i += NT) top[0] = fmaxf(top[0], part[i].x);
     group_reduce<NT, true>(top, red);
     for (int i = threadIdx.x; i < a.parts; i += NT) {
         const float2 v = part[i];
-        sum[0] += v.x == -__builtin_inff() ? v.y : v.y * distill_exp(v.x, top[0], a);
+        sum[0] += v.x == -__builtin_inff() ? v.y : v.y * soft_exp(v.x, top[0], a);
     }
     group_reduce<NT, false>(sum, red + 32);
     if (a.loss && blockIdx.x == 0) {
@@ -457,12 +297,12 @@ __global__ __launch_bounds__(DISTILL_NT) void distill_join_kernel(const DistillA
     }
     if (!a.grad) return;
     T *gr = a.grad + row * a.dim;
-    distill_put<T, NT, NP, true>(z, gr, first, end, DistillExp<T>(top[0], a), a.scale / sum[0], some, a.dim);
+    soft_put<T, NT, NP, true>(z, gr, first, end, SoftExp<T>(top[0], a), a.scale / sum[0], some, a.dim);
     __syncthreads();  // behind all of those, the classes among them that the entries name
     const int lo = first * VEC, hi = end == pieces ? a.dim : end * VEC;
     for (int i = threadIdx.x; i < a.top; i += NT) {
         const DistillEntry e = entry[i];
-        if (e.to >= lo && e.to < hi) gr[e.to] = some ? (T)(a.scale * (distill_exp(e.zc, top[0], a) / sum[0] - e.sum)) : (T)0.f;
+        if (e.to >= lo && e.to < hi) gr[e.to] = some ? (T)(a.scale * (soft_exp(e.zc, top[0], a) / sum[0] - e.sum)) : (T)0.f;
     }
 }
 
@@ -551,12 +391,7 @@ static int distill_step(const Args *a, int ns, int step, const char *fn) {
     d.rows = ns;
     d.dim = dim;
     d.top = top;
-    const double log2e = 1.4426950408889634074 / a->temperature;
-    d.inv_t = 1.f / a->temperature;
-    d.hi = (float)log2e;
-    if ((double)d.hi >= log2e) d.hi = nextafterf(d.hi, 0.f);
-    d.lo = (float)(log2e - (double)d.hi);  // above 0: a difference of -inf gives -inf from both
-    d.least = (float)(-150. / log2e);
+    static_cast<SoftScale &>(d) = SoftScale(a->temperature);
     d.weight = a->weight;
     d.scale = a->weight / a->temperature;
     return sg.finish(distill_launch<T>(d, ns));

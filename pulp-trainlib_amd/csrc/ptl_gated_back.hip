@@ -23,7 +23,8 @@ template <typename OUT, int XR>  // tiles of 128 inputs by XR rows of the other 
 struct GradTile {
     typedef OUT Out;
     typedef f32x16 Acc;
-    static constexpr bool GATE = false;
+    static constexpr RowsAfter AFTER_SUMS = ROWS_SCALED;
+    static constexpr bool GATED = false;
     static constexpr int ROWS_W = 128, ROWS_X = XR, WM = 64, WN = XR / 2, FM = 2, FN = XR / 64, OC = 64, PITCH = OC * (int)sizeof(OUT) + 16, GROUPS = 1;
     static constexpr int NT = 256, TILE = 128 * ROWB, STAGE = TILE + XR * ROWB, RING = 2 * STAGE, TABLE = (2 * ROWS_W + ROWS_X) * 4;
     static_assert(TABLE + 4 * 32 * PITCH <= RING, "what follows the sums fits the ring");

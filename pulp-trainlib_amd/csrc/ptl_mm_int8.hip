@@ -6,7 +6,7 @@ namespace ptl {
 
 template <typename OUT>
 int rows_int8(RowsArgs &a) {
-    return rows_product<int8_t, OUT, false>(a);
+    return rows_product<int8_t, OUT, ROWS_SCALED>(a);
 }
 
 template <typename OUT, typename Args>

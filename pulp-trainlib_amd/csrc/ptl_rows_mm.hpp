@@ -1,18 +1,21 @@
 // Products of two operands that both hold the contraction along their rows, with what a layer does to its sums behind them: the
-// gated dense layer and the product of 8-bit integers (ptl_rows_mm.inc).
+// gated dense layer, the dense layer with activation and residual, and the product of 8-bit integers (ptl_rows_mm.inc).
 #pragma once
 #include "ptl_common.hpp"
 
 namespace ptl {
 
-enum GateAct : int { GATE_SIGMOID = 0, GATE_SILU = 1, GATE_GELU = 2, GATE_RELU = 3 };
+enum GateAct : int { GATE_SIGMOID = 0, GATE_SILU = 1, GATE_GELU = 2, GATE_RELU = 3, GATE_NONE = 4 };
+// What follows the sums: scales, act(one half) * the other, act(all) + a residual.
+enum RowsAfter : int { ROWS_SCALED, ROWS_GATED, ROWS_ACT };
 
 struct RowsArgs {
     const char *w, *x;  // rows of weights, rows of tokens
     int row_b;          // bytes of a row of either
     int outs, tokens;   // gated: 2 x outs rows of weights
     void *y;            // tokens x outs
-    void *hidden;       // gated: tokens x 2 outs (NULL: not wanted)
+    void *hidden;       // gated: tokens x 2 outs, with a residual: tokens x outs (NULL: not wanted)
+    const void *skip;   // the residual, tokens x outs (NULL: none)
     const void *bias;   // of the weights' rows (NULL: none)
     const float *w_scale, *x_scale;  // integers: of the weights' rows, of the tokens (NULL: 1)
     const char *zeros;  // 16 zero bytes
@@ -91,6 +94,8 @@ void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, i
 // 0: launched, 2: HIP error.
 template <typename T>
 int rows_gated(RowsArgs &a);  // T: tensors and products
+template <typename T>
+int rows_act(RowsArgs &a);
 template <typename OUT>
 int rows_int8(RowsArgs &a);
 

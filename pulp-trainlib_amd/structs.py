@@ -212,7 +212,39 @@ class DistillArgs(C.Structure):
                 ("weight", C.c_float), ("wr_loss", P)]
 
 
-GATE_SIGMOID, GATE_SILU, GATE_GELU, GATE_RELU = 0, 1, 2, 3
+# include/ptl_tuning.h
+
+class ActLinearArgs(C.Structure):
+    _fields_ = [("input", BlobP), ("coeff", BlobP), ("bias", BlobP), ("hidden", BlobP), ("skip", BlobP), ("output", BlobP),
+                ("activation", I), ("skip_wg_grad", I), ("skip_in_grad", I), ("use_biases", I)]
+
+
+class NormJoinArgs(C.Structure):
+    _fields_ = [("input", BlobP), ("skip", BlobP), ("gate", BlobP), ("coeff_post", BlobP), ("coeff_pre", BlobP), ("sum", BlobP),
+                ("output", BlobP), ("skip_scale", C.c_float), ("eps", C.c_float), ("rows_per_gate", I), ("skip_wg_grad", I),
+                ("skip_in_grad", I)]
+
+
+class PolicyLossArgs(C.Structure):
+    _fields_ = [("output", BlobP), ("actions", P), ("old_logp", P), ("ref_logp", P), ("advantages", P), ("row_weight", P),
+                ("clip_low", C.c_float), ("clip_high", C.c_float), ("beta", C.c_float), ("temperature", C.c_float),
+                ("weight", C.c_float), ("wr_loss", P), ("wr_logp", P)]
+
+
+class AdamwState(C.Structure):
+    _fields_ = [("m", P), ("v", P), ("m_root", P), ("v_root", P), ("m_scale", P), ("v_scale", P), ("master", P)]
+
+
+class AdamwArgs(C.Structure):
+    _fields_ = [("weights", BlobP), ("updated", BlobP), ("state", C.POINTER(AdamwState)), ("new_state", C.POINTER(AdamwState)),
+                ("learning_rate", C.c_float), ("weight_decay", C.c_float)]
+
+
+class AdamwStep(C.Structure):
+    _fields_ = [("beta1", C.c_float), ("beta2", C.c_float), ("eps", C.c_float), ("step", I), ("step_data", P), ("grad_factor", P)]
+
+
+GATE_SIGMOID, GATE_SILU, GATE_GELU, GATE_RELU, ACT_NONE = 0, 1, 2, 3, 4
 LAYER_CONV2D, LAYER_DW_CONV, LAYER_PW_CONV, LAYER_LINEAR = 0, 1, 2, 3
 STEP_FW, STEP_WGT_GRAD, STEP_IN_GRAD = 0, 1, 2
 
