@@ -3,8 +3,12 @@
 //   ds = ds_in + r2 (dy w_pre - s r2^2 mean(dy w_pre s));  dx = alpha ds;  k = gate w_post b
 //   db = r1 (gate w_post ds - b r1^2 mean(k ds));  P = sum ds b r1:  dgate = w_post P,  dw_post = gate P;  dw_pre = sum dy s r2
 // Both passes move bytes and little else.  A row is read once, into the registers of a wave or a workgroup, which walks over
-// neighbouring rows and keeps weights and gates, and backward its share of the three sums over rows.  Backward all of a row's sums come
-// from one reduction: mean(k ds) needs r2, but the sums of k ds_in, k dy w_pre and k s do not.
+// rows in turn and keeps weights and gates, and backward its share of the sums over rows.  Backward all of a row's sums come
+// from one reduction: mean(k ds) needs r2, but the sums of k ds_in, k dy w_pre and k s do not.  What is written, and backward what is read,
+// passes by the caches (8192 x 4096 fp16: forward 51.7 -> 48.6 us, backward 90 -> 82; forward the block's output is often still there).
+// Measured: 8192 x 4096 fp16 forward 48.6 us (5.5 TB/s), backward with eight gates 82 us (4.9 TB/s), with one 79; 8192 x 1024 12.8 and 28;
+// one row 3.4 us, which is an empty launch.  Large copies reach 5.0 TB/s on the same card.
+#include "ptl_row_sums.hpp"
 #include "ptl_rows.hpp"
 #include "ptl_tuning.h"
 
@@ -16,7 +20,7 @@ template <typename T>
 struct JoinFw {
     const T *b, *x, *gate, *w_post, *w_pre;  // gate, w_pre: NULL where there is none
     T *s, *y;
-    int rows, dim, per, chunk;  // per: rows of a gate (all of them: rows); chunk: rows of a walker
+    int rows, dim, per, walkers;  // per: rows of a gate (all of them: rows); walker w has rows w, w + walkers, ...
     float alpha, eps;
 };
 
@@ -32,23 +36,36 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC, HELD = NP ? NP : 1;
     constexpr bool SHORT = TPR * NP == 64;  // rows of less than a piece come here too
-    constexpr bool AHEAD = NP > 0 && NP * VEC <= 16;
-    __shared__ float red[2][16][1];
+    __shared__ float red[2][ROW_SUMS<TPR, 1>];
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x;
     const long walker = TPR == 64 ? (long)blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : blockIdx.x;
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
-    const long first = walker * a.chunk, end = min(first + a.chunk, (long)a.rows);
-    if (first >= end) return;  // (a whole wave, which has no barrier to meet)
+    const long first = walker, end = a.rows, step = a.walkers;
+    if (first >= min(end, step)) return;  // (a whole wave, which has no barrier to meet)
     auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };  // (pieces that no thread has; half of them someone has)
     if constexpr (NP > 0) {
-        Piece post[HELD], pre[HELD], gate[HELD];
+        Piece pre[HELD];
+        float w[HELD][VEC];  // w_post times the gate
         int of = -1;
+        auto weights = [&](int gate) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            if (none(j)) break;
-            post[j].template hold<SHORT>(a.w_post, j * TPR + t, dim);
-            if (a.w_pre) pre[j].template hold<SHORT>(a.w_pre, j * TPR + t, dim);
+            for (int j = 0; j < NP; ++j) {
+                if (none(j)) break;
+                Piece p, g;
+                p.template hold<SHORT>(a.w_post, j * TPR + t, dim);
+                if (a.gate) g.template hold<SHORT>(a.gate + (size_t)gate * dim, j * TPR + t, dim);
+#pragma unroll
+                for (int i = 0; i < VEC; ++i) w[j][i] = a.gate ? (float)p.e[i] * (float)g.e[i] : (float)p.e[i];
+            }
+        };
+        if (a.w_pre) {
+#pragma unroll
+            for (int j = 0; j < NP; ++j) {
+                if (none(j)) break;
+                pre[j].template hold<SHORT>(a.w_pre, j * TPR + t, dim);
+            }
         }
+        if (!a.gate) weights(0);
         struct Row {
             Piece b[HELD], x[HELD];
         };
@@ -74,11 +91,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
             const size_t at = (size_t)row * dim;
             if (a.gate && (int)row / a.per != of) {
                 of = (int)row / a.per;
-#pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    if (none(j)) break;
-                    gate[j].template hold<SHORT>(a.gate + (size_t)of * dim, j * TPR + t, dim);
-                }
+                weights(of);
             }
             float v[1] = {0.f};
 #pragma unroll
@@ -89,7 +102,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
                 for (int i = 0; i < VEC; ++i) f[i] = (float)r.b[j].e[i];
                 squares(f, Piece::cut(j * TPR + t, dim), v[0]);
             }
-            row_reduce<TPR, 1>(v, red[0]);
+            row_sums<TPR, 1>(v, red[0]);
             const float r1 = join_r(v[0], dim, a.eps);
             float s[HELD][VEC];
             v[0] = 0.f;
@@ -97,21 +110,18 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
             for (int j = 0; j < NP; ++j) {
                 if (none(j)) break;
 #pragma unroll
-                for (int i = 0; i < VEC; ++i) {
-                    const float u = (float)r.b[j].e[i] * r1 * (float)post[j].e[i];
-                    s[j][i] = fmaf(a.alpha, (float)r.x[j].e[i], a.gate ? u * (float)gate[j].e[i] : u);
-                }
+                for (int i = 0; i < VEC; ++i) s[j][i] = fmaf(a.alpha, (float)r.x[j].e[i], (float)r.b[j].e[i] * r1 * w[j][i]);
                 if (a.w_pre) squares(s[j], Piece::cut(j * TPR + t, dim), v[0]);
             }
             // (behind the second reduction's barrier no wave reads the first one's sums any more, and the other way round)
-            if (a.w_pre || TPR > 64) row_reduce<TPR, 1>(v, red[1]);
+            if (a.w_pre || TPR > 64) row_sums<TPR, 1>(v, red[1]);
 #pragma unroll
             for (int j = 0; j < NP; ++j) {
                 if (none(j)) break;
                 Piece o;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(s[j][i]);
-                o.template put<SHORT>(a.s + at, j * TPR + t, dim);
+                o.template put<SHORT, true>(a.s + at, j * TPR + t, dim);
             }
             if (!a.w_pre) return;
             const float r2 = join_r(v[0], dim, a.eps);
@@ -121,29 +131,16 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
                 Piece o;
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(s[j][i] * r2 * (float)pre[j].e[i]);
-                o.template put<SHORT>(a.y + at, j * TPR + t, dim);
+                o.template put<SHORT, true>(a.y + at, j * TPR + t, dim);
             }
         };
-        if constexpr (AHEAD) {
-            Row x, y;
-            long row = first;
+        Row x;
+        for (long row = first; row < end; row += step) {
             fetch(row, x);
-            for (; row < end; row += 2) {
-                if (row + 1 < end) fetch(row + 1, y);
-                work(row, x);
-                if (row + 1 >= end) break;
-                if (row + 2 < end) fetch(row + 2, x);
-                work(row + 1, y);
-            }
-        } else {
-            Row x;
-            for (long row = first; row < end; ++row) {
-                fetch(row, x);
-                work(row, x);
-            }
+            work(row, x);
         }
     } else {
-        for (long row = first; row < end; ++row) {
+        for (long row = first; row < end; row += step) {
             const size_t at = (size_t)row * dim;
             const T *gates = a.gate ? a.gate + (size_t)((int)row / a.per) * dim : nullptr;
             float v[1] = {0.f};
@@ -153,7 +150,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
 #pragma unroll
                 for (int i = 0; i < VEC; ++i) v[0] = fmaf((float)b.e[i], (float)b.e[i], v[0]);
             }
-            row_reduce<TPR, 1>(v, red[0]);
+            row_sums<TPR, 1>(v, red[0]);
             const float r1 = join_r(v[0], dim, a.eps);
             auto join = [&](int p, float (&s)[VEC]) {
                 Piece b, x, post, gate;
@@ -176,7 +173,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
                     for (int i = 0; i < VEC; ++i) v[0] = fmaf(s[i], s[i], v[0]);
                 }
             }
-            row_reduce<TPR, 1>(v, red[1]);
+            row_sums<TPR, 1>(v, red[1]);
             const float r2 = join_r(v[0], dim, a.eps);
             for (int p = t; p < pieces; p += TPR) {  // (each thread writes over its own elements only)
                 float s[VEC];
@@ -198,11 +195,11 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_fw_kernel(const Jo
 template <typename T, int TPR, int NP>
 static void join_fw_launch(JoinFw<T> a) {
     constexpr int per = TPR == 64 ? 4 : 1, waves = TPR / 64;
-    // walkers that fill the chip twice over: 32 waves a compute unit
-    const long most = (long)state().num_cu * 32 / waves;
-    a.chunk = (int)((a.rows + most - 1) / most);
-    const int walkers = (a.rows + a.chunk - 1) / a.chunk;
-    hipLaunchKernelGGL((join_fw_kernel<T, TPR, NP>), dim3((walkers + per - 1) / per), dim3(TPR == 64 ? 256 : TPR), 0, state().stream, a);
+    // 64 waves a compute unit, twice what it holds: rows of 4096 fp16 values, 8192 of them, 47.8 us; 32 waves 51.7, a workgroup for every row,
+    // which reads the weights again for each, 49.9
+    const long most = (long)state().num_cu * 64 / waves;
+    a.walkers = a.rows < most ? a.rows : (int)most;
+    hipLaunchKernelGGL((join_fw_kernel<T, TPR, NP>), dim3((a.walkers + per - 1) / per), dim3(TPR == 64 ? 256 : TPR), 0, state().stream, a);
 }
 
 template <typename T>
@@ -213,42 +210,52 @@ static void join_fw(const JoinFw<T> &a) {
     if (pieces <= 256) return join_fw_launch<T, 256, 1>(a);
     if (pieces <= 512) return join_fw_launch<T, 256, 2>(a);
     if (pieces <= 1024) return join_fw_launch<T, 512, 2>(a);
-    if (pieces <= 2048) return join_fw_launch<T, 512, 4>(a);
+    if (pieces <= 2048) return join_fw_launch<T, 1024, 2>(a);
+    if (sizeof(T) == 4 && pieces <= 4096) return join_fw_launch<T, 1024, 4>(a);
     join_fw_launch<T, 1024, 0>(a);
 }
 
 // ---- backward --------------------------------------------------------------------------------------------------------
 
-// Walkers (waves or workgroups) have neighbouring rows: with one gate for all `chunk` rows each.  Otherwise a walker has one of
-// `parts` parts (of `chunk` rows) of a gate's rows, or, where there are more gates than walkers, `gates` whole ones.
+// Waves or workgroups ("walkers") take rows in turn, so that what runs together reads neighbouring rows.  With several gates a workgroup has
+// every `parts`-th row of one (GATES == 1), or, where there are more gates than workgroups, a walker every `walkers`-th gate's rows (GATES == 2).
 template <typename T>
 struct JoinBw {
     const T *b, *s, *dy, *ds, *gate, *w_post, *w_pre;  // s, dy, w_pre NULL: no second norm; ds, gate: may be NULL
-    T *dx, *db;                       // (NULL: not wanted)
-    T *dgate, *dw_post, *dw_pre;      // what a walker writes itself: gates that it has all rows of; in a grid of one also the weights'
-    float *part, *part_gate;          // of the workgroups: sums over rows, P or dw_post and (with the second norm) dw_pre; of the walkers: P of a gate's part
-    float *stat;                      // long rows: r1, m1, r2, m2 of each
-    int rows, dim, per, chunk, parts, gates, walkers, first;
+    T *dx, *db;                   // (NULL: not wanted)
+    T *dgate, *dw_post, *dw_pre;  // what a walker writes itself: gates that it has all rows of; in a grid of one also the weights'
+    float *part;                  // of the workgroups, sums over their rows: P (GATES == 2: of dw_post) and, with the second norm, of dw_pre
+    float *stat;                  // long rows: r1, m1, r2, m2 of each
+    int rows, dim, per, parts, walkers, first;
     float alpha, eps;
     bool sums;
 };
-struct JoinSpan {
-    long first, end;
-};
-template <typename T>
-__device__ inline JoinSpan join_span(const JoinBw<T> &a, long walker, bool groups) {
-    JoinSpan s;
-    if (groups && a.parts > 1) {
-        const long g = walker / a.parts, z = walker - g * a.parts;
-        s.first = g * a.per + z * a.chunk;
-        s.end = min(min(s.first + a.chunk, (g + 1) * a.per), (long)a.rows);
-    } else {
-        const long rows = groups ? (long)a.gates * a.per : a.chunk;
-        s.first = walker * rows;
-        s.end = min(s.first + rows, (long)a.rows);
+template <typename T, int GATES>
+struct JoinRows {
+    int first, end, step, gate;
+    const JoinBw<T> &a;
+    // Of walker `at` of `of` in workgroup `group`.
+    __device__ inline JoinRows(const JoinBw<T> &a, int group, int at, int of) : end(a.rows), gate(0), a(a) {
+        const int walker = group * of + at;
+        if (GATES == 0) {
+            first = walker;
+            step = a.walkers;
+        } else if (GATES == 1) {
+            gate = group / a.parts;
+            first = gate * a.per + (group - gate * a.parts) * of + at;
+            end = (int)min((long)(gate + 1) * a.per, (long)a.rows);
+            step = a.parts * of;
+        } else {
+            first = walker < a.walkers ? walker * a.per : a.rows;
+            step = 1;
+        }
     }
-    return s;
-}
+    __device__ inline bool has(long row) const { return row < end; }
+    __device__ inline long next(long row) const {
+        if (GATES == 2) return (int)(row + 1) % a.per == 0 ? row + 1 + (a.walkers - 1) * (long)a.per : row + 1;
+        return row + step;
+    }
+};
 // The scalars of a row, from its six sums: s^2, dy w_pre s, b^2, k ds_in, k dy w_pre, k s.  Each step is of the size of r or of a gradient.
 struct JoinScalars {
     float r1, m1, r2, m2;
@@ -262,57 +269,87 @@ struct JoinScalars {
     __device__ inline float ds(float in, float s, float g) const { return fmaf(r2, fmaf(-m2, s, g), in); }
 };
 
-// GROUPS: several gates.
-template <typename T, int TPR, int NP, bool GROUPS>
+// A thread's sums over rows, P and Q: in registers, or (KEEP) in its own places of LDS, where those do not suffice.
+template <int N, int NT, bool KEEP>
+struct JoinSumsOf {
+    float v[2][N];
+    __device__ inline void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[0][i] = v[1][i] = 0.f;
+    }
+    __device__ inline float get(int k, int i) const { return v[k][i]; }
+    __device__ inline void set(int k, int i, float f) { v[k][i] = f; }
+};
+template <int N, int NT>
+struct JoinSumsOf<N, NT, true> {
+    __device__ static inline float *at(int k, int i) {
+        extern __shared__ __attribute__((aligned(16))) float join_lds[];
+        return join_lds + (k * N + i) * NT + threadIdx.x;
+    }
+    __device__ inline void clear() {
+#pragma unroll
+        for (int i = 0; i < N; ++i) *at(0, i) = *at(1, i) = 0.f;
+    }
+    __device__ inline float get(int k, int i) const { return *at(k, i); }
+    __device__ inline void set(int k, int i, float f) { *at(k, i) = f; }
+};
+
+template <typename T, int TPR, int NP, int GATES, bool KEEP>
 __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const JoinBw<T> a) {
     typedef RowPiece<T> Piece;
-    constexpr int VEC = Piece::VEC;
-    constexpr bool AHEAD = NP * VEC <= 8, SHORT = TPR * NP == 64;
-    __shared__ float red[2][16][6];
+    constexpr int VEC = Piece::VEC, NT = TPR == 64 ? 256 : TPR;
+    constexpr bool AHEAD = NP * VEC <= 8 && TPR < 1024, SHORT = TPR * NP == 64;  // AHEAD: registers hold two rows
+    __shared__ float red[2][ROW_SUMS<TPR, 6>];
     const int t = TPR == 64 ? (threadIdx.x & 63) : threadIdx.x, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const long walker = TPR == 64 ? (long)blockIdx.x * 4 + wave : blockIdx.x;
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     auto none = [&](int j) { return j > NP / 2 && j * TPR >= pieces; };
-    const JoinSpan span = join_span(a, walker, GROUPS);
-    Piece post[NP], pre[NP], gate[NP];
-    float P[NP][VEC], Q[NP][VEC], D[GROUPS ? NP : 1][VEC];
+    const JoinRows<T, GATES> rows(a, blockIdx.x, TPR == 64 ? wave : 0, TPR == 64 ? 4 : 1);
+    // w_post times the gate; the sums over rows, of which D, with several gates, only changes where one ends: it is in LDS (a thread's own)
+    Piece pre[NP];
+    float w[NP][VEC];
+    JoinSumsOf<NP * VEC, NT, KEEP> sums;
+    __shared__ float D[GATES == 2 ? NP * VEC : 1][NT];
+    auto weights = [&](int gate) {
+#pragma unroll
+        for (int j = 0; j < NP; ++j) {
+            if (none(j)) break;
+            Piece p, g;
+            p.template hold<SHORT>(a.w_post, j * TPR + t, dim);
+            if (a.gate) g.template hold<SHORT>(a.gate + (size_t)gate * dim, j * TPR + t, dim);
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) w[j][i] = a.gate ? (float)p.e[i] * (float)g.e[i] : (float)p.e[i];
+        }
+    };
+    sums.clear();
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
-        post[j].template hold<SHORT>(a.w_post, j * TPR + t, dim);
-        pre[j].raw = gate[j].raw = row_u4{0, 0, 0, 0};
+        pre[j].raw = row_u4{0, 0, 0, 0};
         if (a.w_pre) pre[j].template hold<SHORT>(a.w_pre, j * TPR + t, dim);
-        if (!GROUPS && a.gate) gate[j].template hold<SHORT>(a.gate, j * TPR + t, dim);
+        if constexpr (GATES == 2) {
 #pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            P[j][i] = Q[j][i] = 0.f;
-            if constexpr (GROUPS) D[j][i] = 0.f;
+            for (int i = 0; i < VEC; ++i) D[j * VEC + i][threadIdx.x] = 0.f;
         }
     }
+    if (GATES < 2) weights(rows.gate);
     int of = -1;
-    // Of a gate whose rows are done: its gradient (or this walker's part of it), and its share of the weights'.
+    // Of a gate whose rows are done: its gradient, and its share of the weights'.
     auto close = [&]() {
-        if (!a.sums || (of < 0 && (a.parts == 1 || walker >= a.walkers))) return;  // (a part that no row is left for: zeros)
+        if (!a.sums || of < 0) return;
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
             const int p = j * TPR + t;
-            if (a.parts == 1) {
-                Piece o;
-#pragma unroll
-                for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(P[j][i] * (float)post[j].e[i]);
-                o.template put<SHORT>(a.dgate + (size_t)of * dim, p, dim);
-            } else if (p < pieces) {
-                float *to = a.part_gate + (size_t)walker * dim;
-                const int cut = Piece::cut(p, dim);
-#pragma unroll
-                for (int i = 0; i < VEC; ++i)
-                    if (i >= cut && p * VEC - cut + i < dim) to[p * VEC - cut + i] = P[j][i];
-            }
+            Piece gate, o, post;
+            gate.template hold<SHORT>(a.gate + (size_t)of * dim, p, dim);
+            post.template hold<SHORT>(a.w_post, p, dim);
 #pragma unroll
             for (int i = 0; i < VEC; ++i) {
-                if constexpr (GROUPS) D[j][i] = fmaf((float)gate[j].e[i], P[j][i], D[j][i]);
-                P[j][i] = 0.f;
+                const float P = sums.get(0, j * VEC + i);
+                o.e[i] = row_round<T>(P * (float)post.e[i]);
+                D[GATES == 2 ? j * VEC + i : 0][threadIdx.x] = fmaf((float)gate.e[i], P, D[GATES == 2 ? j * VEC + i : 0][threadIdx.x]);
+                sums.set(0, j * VEC + i, 0.f);
             }
+            o.template put<SHORT>(a.dgate + (size_t)of * dim, p, dim);
         }
     };
     struct Row {
@@ -323,37 +360,32 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const Jo
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
-            r.b[j].template hold<SHORT>(a.b + at, j * TPR + t, dim);
+            r.b[j].template hold<SHORT, true>(a.b + at, j * TPR + t, dim);
             r.s[j].raw = r.g[j].raw = r.d[j].raw = row_u4{0, 0, 0, 0};
             if (a.w_pre) {
-                r.s[j].template hold<SHORT>(a.s + at, j * TPR + t, dim);
-                r.g[j].template hold<SHORT>(a.dy + at, j * TPR + t, dim);
+                r.s[j].template hold<SHORT, true>(a.s + at, j * TPR + t, dim);
+                r.g[j].template hold<SHORT, true>(a.dy + at, j * TPR + t, dim);
             }
-            if (a.ds) r.d[j].template hold<SHORT>(a.ds + at, j * TPR + t, dim);
+            if (a.ds) r.d[j].template hold<SHORT, true>(a.ds + at, j * TPR + t, dim);
         }
     };
     int turn = 0;
     auto work = [&](long row, const Row &x) {
         const size_t at = (size_t)row * dim;
-        if constexpr (GROUPS) {
+        if constexpr (GATES == 2) {
             if ((int)row / a.per != of) {
                 close();
                 of = (int)row / a.per;
-#pragma unroll
-                for (int j = 0; j < NP; ++j) {
-                    if (none(j)) break;
-                    gate[j].template hold<SHORT>(a.gate + (size_t)of * dim, j * TPR + t, dim);
-                }
+                weights(of);
             }
         }
-        auto weight = [&](int j, int i) { return a.gate ? (float)post[j].e[i] * (float)gate[j].e[i] : (float)post[j].e[i]; };
         float v[6] = {};
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             if (none(j)) break;
             const int cut = Piece::cut(j * TPR + t, dim);
             auto add = [&](int i) {
-                const float b = (float)x.b[j].e[i], s = (float)x.s[j].e[i], g = (float)x.g[j].e[i] * (float)pre[j].e[i], k = weight(j, i) * b;
+                const float b = (float)x.b[j].e[i], s = (float)x.s[j].e[i], g = (float)x.g[j].e[i] * (float)pre[j].e[i], k = w[j][i] * b;
                 v[0] = fmaf(s, s, v[0]);
                 v[1] = fmaf(g, s, v[1]);
                 v[2] = fmaf(b, b, v[2]);
@@ -370,7 +402,7 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const Jo
                 for (int i = 0; i < VEC; ++i) add(i);
             }
         }
-        row_reduce<TPR, 6>(v, red[turn]);
+        row_sums<TPR, 6>(v, red[turn]);
         turn ^= 1;
         const JoinScalars c(v, dim, a.eps);
 #pragma unroll
@@ -382,36 +414,38 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const Jo
             for (int i = 0; i < VEC; ++i) {
                 const float b = (float)x.b[j].e[i], s = (float)x.s[j].e[i], dy = (float)x.g[j].e[i];
                 const float ds = c.ds((float)x.d[j].e[i], s, dy * (float)pre[j].e[i]);
-                P[j][i] = fmaf(ds, b * c.r1, P[j][i]);
-                Q[j][i] = fmaf(dy, s * c.r2, Q[j][i]);
+                sums.set(0, j * VEC + i, fmaf(ds, b * c.r1, sums.get(0, j * VEC + i)));
+                sums.set(1, j * VEC + i, fmaf(dy, s * c.r2, sums.get(1, j * VEC + i)));
                 ox.e[i] = row_round<T>(a.alpha * ds);
-                ob.e[i] = row_round<T>(c.r1 * fmaf(-c.m1, b, weight(j, i) * ds));
+                ob.e[i] = row_round<T>(c.r1 * fmaf(-c.m1, b, w[j][i] * ds));
             }
             if (!a.dx) continue;
-            ox.template put<SHORT>(a.dx + at, p, dim);
-            ob.template put<SHORT>(a.db + at, p, dim);
+            ox.template put<SHORT, true>(a.dx + at, p, dim);
+            ob.template put<SHORT, true>(a.db + at, p, dim);
         }
     };
     if constexpr (AHEAD) {
         Row x, y;
-        long row = span.first;
-        if (row < span.end) fetch(row, x);
-        for (; row < span.end; row += 2) {
-            if (row + 1 < span.end) fetch(row + 1, y);
+        long row = rows.first;
+        if (rows.has(row)) fetch(row, x);
+        while (rows.has(row)) {
+            const long second = rows.next(row), third = rows.next(second);
+            if (rows.has(second)) fetch(second, y);
             work(row, x);
-            if (row + 1 >= span.end) break;
-            if (row + 2 < span.end) fetch(row + 2, x);
-            work(row + 1, y);
+            if (!rows.has(second)) break;
+            if (rows.has(third)) fetch(third, x);
+            work(second, y);
+            row = third;
         }
     } else {
         Row x;
-        for (long row = span.first; row < span.end; ++row) {
+        for (long row = rows.first; rows.has(row); row = rows.next(row)) {
             fetch(row, x);
             work(row, x);
         }
     }
     if (!a.sums) return;
-    if constexpr (GROUPS) close();
+    if constexpr (GATES == 2) close();
     auto out = [&](int c, float p, float q) {  // (a column's sums over the rows of the workgroup)
         if (a.part) {
             float *part = a.part + (size_t)blockIdx.x * (a.w_pre ? 2 : 1) * dim;
@@ -419,14 +453,14 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const Jo
             if (a.w_pre) part[dim + c] = q;
             return;
         }
-        if (!GROUPS && a.gate) {
+        if (GATES == 0 && a.gate) {
             a.dgate[c] = row_round<T>(p * (float)a.w_post[c]);
             p *= (float)a.gate[c];
         }
         a.dw_post[c] = row_round<T>(p);
         if (a.w_pre) a.dw_pre[c] = row_round<T>(q);
     };
-    auto S = [&](int j, int i) { if constexpr (GROUPS) return D[j][i]; else return P[j][i]; };
+    auto S = [&](int j, int i) { return GATES == 2 ? D[GATES == 2 ? j * VEC + i : 0][threadIdx.x] : sums.get(0, j * VEC + i); };
     if constexpr (TPR == 64) {  // the four waves' shares as one
         __shared__ float all[4][2][64 * NP * VEC];
 #pragma unroll
@@ -436,33 +470,31 @@ __global__ __launch_bounds__(TPR == 64 ? 256 : TPR) void join_bw_kernel(const Jo
                 const int p = j * 64 + t, cut = Piece::cut(p, dim), c = p * VEC - cut + i;
                 if (i >= cut && c < dim) {
                     all[wave][0][c] = S(j, i);
-                    all[wave][1][c] = Q[j][i];
+                    all[wave][1][c] = sums.get(1, j * VEC + i);
                 }
             }
         __syncthreads();
         for (int c = threadIdx.x; c < dim; c += 256)
             out(c, all[0][0][c] + all[1][0][c] + (all[2][0][c] + all[3][0][c]), all[0][1][c] + all[1][1][c] + (all[2][1][c] + all[3][1][c]));
-    } else if (a.part) {
-        float *part = a.part + (size_t)blockIdx.x * (a.w_pre ? 2 : 1) * dim;
-#pragma unroll
-        for (int j = 0; j < NP; ++j) {
-            const int p = j * TPR + t;
-            if (p >= pieces) continue;
-            float *to = part + p * VEC - Piece::cut(p, dim);
-#pragma unroll
-            for (int i = 0; i < VEC; i += 4) {
-                *reinterpret_cast<row_u4 *>(to + i) = __builtin_bit_cast(row_u4, row_f4{S(j, i), S(j, i + 1), S(j, i + 2), S(j, i + 3)});
-                if (a.w_pre) *reinterpret_cast<row_u4 *>(to + dim + i) = __builtin_bit_cast(row_u4, row_f4{Q[j][i], Q[j][i + 1], Q[j][i + 2], Q[j][i + 3]});
-            }
-        }
     } else {
 #pragma unroll
         for (int j = 0; j < NP; ++j) {
             const int p = j * TPR + t, cut = Piece::cut(p, dim);
             if (p >= pieces) continue;
+            if (a.part) {
+                float *to = a.part + (size_t)blockIdx.x * (a.w_pre ? 2 : 1) * dim + p * VEC - cut;
 #pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (i >= cut) out(p * VEC - cut + i, S(j, i), Q[j][i]);
+                for (int i = 0; i < VEC; i += 4) {
+                    *reinterpret_cast<row_u4 *>(to + i) = __builtin_bit_cast(row_u4, row_f4{S(j, i), S(j, i + 1), S(j, i + 2), S(j, i + 3)});
+                    if (a.w_pre)
+                        *reinterpret_cast<row_u4 *>(to + dim + i) = __builtin_bit_cast(
+                            row_u4, row_f4{sums.get(1, j * VEC + i), sums.get(1, j * VEC + i + 1), sums.get(1, j * VEC + i + 2), sums.get(1, j * VEC + i + 3)});
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < VEC; ++i)
+                    if (i >= cut) out(p * VEC - cut + i, S(j, i), sums.get(1, j * VEC + i));
+            }
         }
     }
 }
@@ -472,7 +504,7 @@ template <typename T>
 __global__ __launch_bounds__(1024) void join_stat_kernel(const JoinBw<T> a) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC;
-    __shared__ float red[16][6];
+    __shared__ float red[ROW_SUMS<1024, 6>];
     const int dim = a.dim, pieces = (dim + VEC - 1) / VEC;
     const size_t row = (size_t)a.first + blockIdx.x, at = row * dim;
     const T *gates = a.gate ? a.gate + (row / a.per) * dim : nullptr;
@@ -501,47 +533,40 @@ __global__ __launch_bounds__(1024) void join_stat_kernel(const JoinBw<T> a) {
             v[5] = fmaf(k, fs, v[5]);
         }
     }
-    row_reduce<1024, 6>(v, red);
+    row_sums<1024, 6>(v, red);
     if (threadIdx.x == 0) {
         const JoinScalars c(v, dim, a.eps);
         reinterpret_cast<float4 *>(a.stat)[row] = make_float4(c.r1, c.m1, c.r2, c.m2);
     }
 }
-template <typename T, bool GROUPS>
+template <typename T, int GATES>
 __global__ __launch_bounds__(256) void join_columns_kernel(const JoinBw<T> a) {
     typedef RowPiece<T> Piece;
     constexpr int VEC = Piece::VEC;
     const int dim = a.dim, p = (int)blockIdx.x * 256 + (int)threadIdx.x;
     if (p * (long)VEC >= dim) return;
-    const JoinSpan span = join_span(a, blockIdx.y, GROUPS);
+    const JoinRows<T, GATES> rows(a, blockIdx.y, 0, 1);
     Piece post, pre, gate;
-    pre.raw = gate.raw = row_u4{0, 0, 0, 0};
+    pre.raw = row_u4{0, 0, 0, 0};
     post.load(a.w_post, p, dim);
     if (a.w_pre) pre.load(a.w_pre, p, dim);
-    if (!GROUPS && a.gate) gate.load(a.gate, p, dim);
+    if (GATES < 2 && a.gate) gate.load(a.gate + (size_t)rows.gate * dim, p, dim);
     float P[VEC] = {}, Q[VEC] = {}, D[VEC] = {};
     int of = -1;
     auto close = [&]() {
-        if (!a.sums || (of < 0 && a.parts == 1)) return;  // (a part that no row is left for: zeros)
-        if (a.parts == 1) {
-            Piece o;
-#pragma unroll
-            for (int i = 0; i < VEC; ++i) o.e[i] = row_round<T>(P[i] * (float)post.e[i]);
-            o.store(a.dgate + (size_t)of * dim, p, dim);
-        } else {
-#pragma unroll
-            for (int i = 0; i < VEC; ++i)
-                if (p * VEC + i < dim) a.part_gate[(size_t)blockIdx.y * dim + p * VEC + i] = P[i];
-        }
+        if (!a.sums || of < 0) return;
+        Piece o;
 #pragma unroll
         for (int i = 0; i < VEC; ++i) {
+            o.e[i] = row_round<T>(P[i] * (float)post.e[i]);
             D[i] = fmaf((float)gate.e[i], P[i], D[i]);
             P[i] = 0.f;
         }
+        o.store(a.dgate + (size_t)of * dim, p, dim);
     };
-    for (long row = span.first; row < span.end; ++row) {
+    for (long row = rows.first; rows.has(row); row = rows.next(row)) {
         const size_t at = (size_t)row * dim;
-        if (GROUPS && (int)row / a.per != of) {
+        if (GATES == 2 && (int)row / a.per != of) {
             close();
             of = (int)row / a.per;
             gate.load(a.gate + (size_t)of * dim, p, dim);
@@ -569,118 +594,138 @@ __global__ __launch_bounds__(256) void join_columns_kernel(const JoinBw<T> a) {
         ob.store(a.db + at, p, dim);
     }
     if (!a.sums) return;
-    if (GROUPS) close();
+    if (GATES == 2) close();
     float *part = a.part + (size_t)blockIdx.y * (a.w_pre ? 2 : 1) * dim;
 #pragma unroll
     for (int i = 0; i < VEC; ++i)
         if (p * VEC + i < dim) {
-            part[p * VEC + i] = GROUPS ? D[i] : P[i];
+            part[p * VEC + i] = GATES == 2 ? D[i] : P[i];
             if (a.w_pre) part[dim + p * VEC + i] = Q[i];
         }
 }
 
-// Sums over shares: of column c of group z (blockIdx.y) those of part[(z * shares + share) * width + c]; 32 columns (a 128-byte line) a
-// workgroup, 32 shares at a time with four loads in flight.
-struct JoinSums {
-    const float *part;
-    int width, shares;
-};
-template <typename T, typename F>
-__device__ inline void join_sums(const JoinSums &a, F put) {
-    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, c = (int)blockIdx.x * 32 + o;
-    const float *part = a.part + (size_t)blockIdx.y * a.shares * a.width;
+// The workgroups' shares added up, 32 columns (a 128-byte line) a workgroup, 32 shares at a time with four loads in flight: the first
+// w_blocks workgroups have the columns of dw_post (GATES == 0: of P, of which dw_post and the one gate's gradient are made; GATES == 1: of P times its
+// gate) and behind them those of dw_pre; with GATES == 1 the others have the gates', whose shares lie side by side.
+template <typename T, int GATES>
+__global__ __launch_bounds__(1024) void join_sums_kernel(const JoinBw<T> a, int shares, int w_blocks) {
+    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, width = a.dim * (a.w_pre ? 2 : 1);
+    const bool gates = GATES == 1 && (int)blockIdx.x >= w_blocks;
+    const int per = (a.dim + 31) / 32, z0 = gates ? ((int)blockIdx.x - w_blocks) / per : 0;
+    const int c = (gates ? (int)blockIdx.x - w_blocks - z0 * per : (int)blockIdx.x) * 32 + o, most = gates ? a.dim : width;
+    const int first = gates ? z0 * a.parts : 0, end = gates ? first + a.parts : shares;
+    const bool scaled = GATES == 1 && !gates && c < a.dim;
     LongSum<T> s;
     s.clear();
-    if (c < a.width) {
-        int z = g;
-        for (; z + 96 < a.shares; z += 128) {
+    if (c < most) {
+        auto value = [&](int z) { return a.part[(size_t)z * width + c] * (scaled ? (float)a.gate[(size_t)(z / a.parts) * a.dim + c] : 1.f); };
+        int z = first + g;
+        for (; z + 96 < end; z += 128) {
             float v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(z + 32 * u) * a.width + c];
+            for (int u = 0; u < 4; ++u) v[u] = value(z + 32 * u);
 #pragma unroll
             for (int u = 0; u < 4; ++u) s.add(v[u]);
         }
-        for (; z < a.shares; z += 32) s.add(part[(size_t)z * a.width + c]);
+        for (; z < end; z += 32) s.add(value(z));
     }
     __shared__ LongSum<T> red[32][32];
     red[g][o] = s;
     __syncthreads();
-    if (g != 0 || c >= a.width) return;
+    if (g != 0 || c >= most) return;
     for (int k = 1; k < 32; ++k) s.add(red[k][o]);
-    put(c, s.value());
-}
-// ... of the weights (and the one gate's, where `gate` is given: its sums are P)
-template <typename T>
-__global__ __launch_bounds__(1024) void join_weights_kernel(const JoinSums a, const JoinBw<T> b, const T *gate) {
-    join_sums<T>(a, [&](int c, float v) {
-        if (c >= b.dim) {
-            b.dw_pre[c - b.dim] = row_round<T>(v);
-            return;
+    float v = s.value();
+    if (gates) {
+        a.dgate[(size_t)z0 * a.dim + c] = row_round<T>(v * (float)a.w_post[c]);
+    } else if (c >= a.dim) {
+        a.dw_pre[c - a.dim] = row_round<T>(v);
+    } else {
+        if (GATES == 0 && a.gate) {
+            a.dgate[c] = row_round<T>(v * (float)a.w_post[c]);
+            v *= (float)a.gate[c];
         }
-        if (gate) {
-            b.dgate[c] = row_round<T>(v * (float)b.w_post[c]);
-            v *= (float)gate[c];
-        }
-        b.dw_post[c] = row_round<T>(v);
-    });
-}
-// ... of gates whose rows several walkers have
-template <typename T>
-__global__ __launch_bounds__(1024) void join_gates_kernel(const JoinSums a, const JoinBw<T> b) {
-    join_sums<T>(a, [&](int c, float v) { b.dgate[(size_t)blockIdx.y * b.dim + c] = row_round<T>(v * (float)b.w_post[c]); });
+        a.dw_post[c] = row_round<T>(v);
+    }
 }
 
-// How the rows are dealt to about `want` walkers; returns how many there are.
+// How the rows are dealt to about `want` workgroups of `of` walkers each: their number, and which kernel (GATES).
 template <typename T>
-static int join_deal(JoinBw<T> &a, bool groups, int want) {
-    a.parts = a.gates = 1;
-    if (!groups) {
-        a.chunk = (a.rows + want - 1) / want;
-        return a.walkers = (a.rows + a.chunk - 1) / a.chunk;
-    }
+static int join_deal(JoinBw<T> &a, bool groups, int want, int of, int &gates) {
     const int all = (a.rows + a.per - 1) / a.per;
-    if (want >= 2 * all) {
-        int parts = want / all;
-        a.chunk = (a.per + parts - 1) / parts;
-        a.parts = (a.per + a.chunk - 1) / a.chunk;
-        return a.walkers = all * a.parts;
+    a.parts = 1;
+    gates = !groups ? 0 : want >= 2 * all && a.per >= 2 * of ? 1 : 2;
+    if (gates == 1) {
+        const int most = (a.per + of - 1) / of;
+        a.parts = want / all < most ? want / all : most;
+        return all * a.parts;
     }
-    a.gates = (all + want - 1) / want;
-    return a.walkers = (all + a.gates - 1) / a.gates;
+    const long units = gates == 0 ? a.rows : all, groups_of = (units + of - 1) / of;
+    const int grid = (int)(want < groups_of ? want : groups_of);
+    a.walkers = (int)((long)grid * of < units ? (long)grid * of : units);
+    return grid;
 }
 
 template <typename T>
-static int join_finish(const JoinBw<T> &a, bool groups, int shares) {
+static int join_finish(const JoinBw<T> &a, int gates, int shares) {
     if (a.part) {
-        const JoinSums s = {a.part, a.dim * (a.w_pre ? 2 : 1), shares};
-        hipLaunchKernelGGL((join_weights_kernel<T>), dim3((s.width + 31) / 32), dim3(1024), 0, state().stream, s, a, groups ? nullptr : a.gate);
-    }
-    if (a.part_gate) {
-        const JoinSums s = {a.part_gate, a.dim, a.parts};
-        hipLaunchKernelGGL((join_gates_kernel<T>), dim3((a.dim + 31) / 32, (a.rows + a.per - 1) / a.per), dim3(1024), 0, state().stream, s, a);
+        const int w_blocks = (a.dim * (a.w_pre ? 2 : 1) + 31) / 32, z_blocks = gates == 1 ? (a.dim + 31) / 32 * ((a.rows + a.per - 1) / a.per) : 0;
+        const dim3 grid(w_blocks + z_blocks);
+        if (gates == 0) hipLaunchKernelGGL((join_sums_kernel<T, 0>), grid, dim3(1024), 0, state().stream, a, shares, w_blocks);
+        else if (gates == 1) hipLaunchKernelGGL((join_sums_kernel<T, 1>), grid, dim3(1024), 0, state().stream, a, shares, w_blocks);
+        else hipLaunchKernelGGL((join_sums_kernel<T, 2>), grid, dim3(1024), 0, state().stream, a, shares, w_blocks);
     }
     return hip_ok(hipGetLastError(), "norm launch") ? 0 : 2;
 }
 
-template <typename T, int TPR, int NP>
+// Eight waves a compute unit (8192 rows of 4096 fp16 values with eight gates 90 us, with four 108, with twelve 100: the registers hold eight,
+// and each workgroup's sums are written and read), fewer where rows are few: a workgroup moves about 35 GB/s, its sums 8 bytes a column.
+template <typename T, int TPR>
+static int join_want(const JoinBw<T> &a) {
+    constexpr int of = TPR == 64 ? 4 : 1, waves = TPR == 64 ? 4 : TPR / 64;
+    const int few = (int)sqrtf(72.f * (float)a.rows * sizeof(T)), cu = state().num_cu, full = waves < 8 ? cu * 8 / waves : cu;
+    const int want = a.rows <= 3 * of ? 1 : few < full ? few : full;
+    return want > 0 ? want : 1;
+}
+template <typename T, int TPR, int NP, bool KEEP = false>
 static int join_bw_launch(JoinBw<T> &a, bool groups) {
-    constexpr int per = TPR == 64 ? 4 : 1;
-    const int best = (int)sqrtf(72.f * (float)a.rows * sizeof(T));
-    int want = a.rows <= 3 * per ? per : best * per;
-    want = want < a.rows ? want : a.rows;
-    const int walkers = join_deal(a, groups, want > 0 ? want : 1), grid = (walkers + per - 1) / per;
-    const size_t part = a.sums && (grid > 1) ? (size_t)grid * a.dim * (a.w_pre ? 2 : 1) : 0;
-    const size_t part_gate = a.sums && groups && a.parts > 1 ? (size_t)walkers * a.dim : 0;
-    if (part + part_gate) {
-        float *ws = workspace((part + part_gate) * sizeof(float));
-        if (!ws) return 2;
-        if (part) a.part = ws;
-        if (part_gate) a.part_gate = ws + part;
-    }
+    constexpr int of = TPR == 64 ? 4 : 1;
+    int gates;
+    const int grid = join_deal(a, groups, join_want<T, TPR>(a), of, gates);
+    if (a.sums && (grid > 1 || gates == 1) && !(a.part = workspace((size_t)grid * a.dim * (a.w_pre ? 2 : 1) * sizeof(float)))) return 2;
     const dim3 block(TPR == 64 ? 256 : TPR);
-    if (groups) hipLaunchKernelGGL((join_bw_kernel<T, TPR, NP, true>), dim3(grid), block, 0, state().stream, a);
-    else hipLaunchKernelGGL((join_bw_kernel<T, TPR, NP, false>), dim3(grid), block, 0, state().stream, a);
-    return join_finish(a, groups, grid);
+    constexpr int lds = KEEP ? 2 * NP * RowPiece<T>::VEC * TPR * 4 : 0;
+    if constexpr (KEEP) {
+        static bool ready = false;
+        if (!ready) {
+            for (const void *f : {reinterpret_cast<const void *>(join_bw_kernel<T, TPR, NP, 0, KEEP>), reinterpret_cast<const void *>(join_bw_kernel<T, TPR, NP, 1, KEEP>)})
+                if (!hip_ok(hipFuncSetAttribute(f, hipFuncAttributeMaxDynamicSharedMemorySize, lds), "hipFuncSetAttribute")) return 2;
+            ready = true;
+        }
+    }
+    if (gates == 0) hipLaunchKernelGGL((join_bw_kernel<T, TPR, NP, 0, KEEP>), dim3(grid), block, lds, state().stream, a);
+    else if (gates == 1) hipLaunchKernelGGL((join_bw_kernel<T, TPR, NP, 1, KEEP>), dim3(grid), block, lds, state().stream, a);
+    else if constexpr (!KEEP) hipLaunchKernelGGL((join_bw_kernel<T, TPR, NP, 2, KEEP>), dim3(grid), block, lds, state().stream, a);
+    return join_finish(a, gates, grid);
+}
+
+template <typename T>
+static int join_bw_columns(JoinBw<T> &a, bool groups) {
+    const int pieces = (a.dim + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC;
+    int gates;
+    const int grid = join_deal(a, groups, a.rows < 64 ? a.rows : 64, 1, gates);
+    const size_t stat = (size_t)a.rows * 4, part = a.sums ? (size_t)grid * a.dim * (a.w_pre ? 2 : 1) : 0;
+    float *ws = workspace((stat + part) * sizeof(float));
+    if (!ws) return 2;
+    a.stat = ws;
+    a.part = part ? ws + stat : nullptr;
+    constexpr int most = (int)(ROW_THREADS / 1024);
+    for (a.first = 0; a.first < a.rows; a.first += most)
+        hipLaunchKernelGGL((join_stat_kernel<T>), dim3(a.rows - a.first < most ? a.rows - a.first : most), dim3(1024), 0, state().stream, a);
+    const dim3 wide((pieces + 255) / 256, grid);
+    if (gates == 0) hipLaunchKernelGGL((join_columns_kernel<T, 0>), wide, dim3(256), 0, state().stream, a);
+    else if (gates == 1) hipLaunchKernelGGL((join_columns_kernel<T, 1>), wide, dim3(256), 0, state().stream, a);
+    else hipLaunchKernelGGL((join_columns_kernel<T, 2>), wide, dim3(256), 0, state().stream, a);
+    return join_finish(a, gates, grid);
 }
 
 template <typename T>
@@ -689,23 +734,17 @@ static int join_bw(JoinBw<T> &a, bool groups) {
     if (pieces <= 64) return join_bw_launch<T, 64, 1>(a, groups);
     if (pieces <= 128) return join_bw_launch<T, 64, 2>(a, groups);
     if (pieces <= 256) return join_bw_launch<T, 256, 1>(a, groups);
-    if (pieces <= 512) return join_bw_launch<T, 512, 1>(a, groups);
-    if (pieces <= 1024) return join_bw_launch<T, 512, 2>(a, groups);
-    const int walkers = join_deal(a, groups, a.rows < 64 ? a.rows : 64);
-    const size_t stat = (size_t)a.rows * 4, part = a.sums ? (size_t)walkers * a.dim * (a.w_pre ? 2 : 1) : 0;
-    const size_t part_gate = a.sums && groups && a.parts > 1 ? (size_t)walkers * a.dim : 0;
-    float *ws = workspace((stat + part + part_gate) * sizeof(float));
-    if (!ws) return 2;
-    a.stat = ws;
-    a.part = part ? ws + stat : nullptr;
-    a.part_gate = part_gate ? ws + stat + part : nullptr;
-    constexpr int most = (int)(ROW_THREADS / 1024);
-    for (a.first = 0; a.first < a.rows; a.first += most)
-        hipLaunchKernelGGL((join_stat_kernel<T>), dim3(a.rows - a.first < most ? a.rows - a.first : most), dim3(1024), 0, state().stream, a);
-    const dim3 grid((pieces + 255) / 256, walkers);
-    if (groups) hipLaunchKernelGGL((join_columns_kernel<T, true>), grid, dim3(256), 0, state().stream, a);
-    else hipLaunchKernelGGL((join_columns_kernel<T, false>), grid, dim3(256), 0, state().stream, a);
-    return join_finish(a, groups, walkers);
+    if (pieces <= 512) return join_bw_launch<T, 256, 2>(a, groups);
+    if constexpr (sizeof(T) == 4) {
+        if (pieces <= 1024) return join_bw_launch<T, 512, 2>(a, groups);
+        if (pieces <= 2048) return join_bw_launch<T, 1024, 2>(a, groups);
+    } else {
+        if (pieces <= 1024) return join_bw_launch<T, 1024, 1>(a, groups);
+        int gates;
+        join_deal(a, groups, join_want<T, 1024>(a), 1, gates);
+        if (pieces <= 2048 && gates < 2) return join_bw_launch<T, 1024, 2, true>(a, groups);  // (the sums of several gates do not fit LDS)
+    }
+    return join_bw_columns(a, groups);
 }
 
 template <typename T, typename Args>

@@ -31,14 +31,17 @@ struct RowPiece {
     static __device__ inline int cut(int p, int dim) { return p * VEC - min(p * VEC, max(dim - VEC, 0)); }
     // (a row held in registers is far shorter than 4 GB: the row's address plus an unsigned offset is one instruction's operand)
     static __device__ inline unsigned place(int p, int dim) { return (unsigned)min(p * VEC, dim - VEC) * (unsigned)sizeof(T); }
-    template <bool SHORT>
+    // STREAM: past the caches, for rows that nothing else of the launch reads.
+    template <bool SHORT, bool STREAM = false>
     __device__ inline void hold(const T *row, int p, int dim) {
         if (SHORT && dim < VEC) fetch(row, p, dim);
+        else if (STREAM) raw = __builtin_nontemporal_load(reinterpret_cast<const row_u4 *>(reinterpret_cast<const char *>(row) + place(p, dim)));
         else raw = *reinterpret_cast<const row_u4 *>(reinterpret_cast<const char *>(row) + place(p, dim));
     }
-    template <bool SHORT>
+    template <bool SHORT, bool STREAM = false>
     __device__ inline void put(T *row, int p, int dim) const {
         if (SHORT && dim < VEC) store(row, p, dim);
+        else if (STREAM && p * VEC < dim) __builtin_nontemporal_store(raw, reinterpret_cast<row_u4 *>(reinterpret_cast<char *>(row) + place(p, dim)));
         else if (p * VEC < dim) *reinterpret_cast<row_u4 *>(reinterpret_cast<char *>(row) + place(p, dim)) = raw;
     }
     // Piece p of a row of `dim` elements.  No load depends on where the row ends: a piece that reaches over the end is read so that
