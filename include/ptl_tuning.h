@@ -167,8 +167,9 @@ int ptl_policy_loss_fp16_batched(const struct policy_loss_args_fp16 *a, int nsam
  *   m, v            in fp32, weights->dim elements each; or
  *   m_root, v_root  in 8 bits with a scale for every 256 elements (ceil(dim / 256) in m_scale and v_scale): the signed root of m,
  *                   -127 .. 127, and the fourth root of v, 0 .. 255, which the scale multiplies; the scale is the largest root of the
- *                   256 over 127 or 255.  They are rounded to the nearest (ties to even), a v that is not 0 to 1 at least.  256 elements
- *                   with infinities or NaN get a scale that is no finite number.  w is formed from m and v before they are rounded.
+ *                   256 over 127 or 255.  They are rounded to the nearest (ties to even), a v that is not 0 to 1 at least (moments below
+ *                   fp32's normal range count as 0).  256 elements with infinities or NaN get a scale that is no finite number.  w is
+ *                   formed from m and v before they are rounded.
  *   master          (may be NULL; in both or neither of state and new_state) the weights in fp32: w is read from state->master and
  *                   written to new_state->master, and weights->data is not read; updated->data receives w rounded. */
 struct adamw_state {

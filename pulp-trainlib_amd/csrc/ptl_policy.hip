@@ -86,7 +86,10 @@ __device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first,
         if (MINE) {
             if (p < end) o.store(row, p, dim);
         } else {
-            o.template put<NP == 1>(row, p, dim);
+#ifndef NT_PUT
+#define NT_PUT false
+#endif
+            o.template put<NP == 1, NT_PUT>(row, p, dim);
         }
     }
 }

@@ -27,6 +27,20 @@ __device__ inline float lanes_sum(float v) {
     return lane_add32(lane_add16(v));
 }
 
+// The largest of the lanes' unsigned integers, as the float that it stands for.
+template <int CTRL>
+__device__ inline unsigned lane_most(unsigned u) {
+    return max(u, (unsigned)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, 0xf, 0xf, true));
+}
+__device__ inline float lanes_most(unsigned u) {
+    u = lane_most<LANE_MIRROR16>(lane_most<LANE_MIRROR8>(lane_most<LANE_XOR2>(lane_most<LANE_XOR1>(u))));
+    auto r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+    u = max((unsigned)r[0], (unsigned)r[1]);
+    r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+    u = max((unsigned)r[0], (unsigned)r[1]);
+    return __builtin_bit_cast(float, u);
+}
+
 // ... of N values over the TPR threads that have a row: one wave, or a workgroup.  A workgroup's waves leave their sums in `lds`, ROW_SUMS floats
 // that the caller does not use again without a barrier: of one value side by side, of several in eights.  Each wave then reads all of them in
 // one or two instructions, a value and wave to a lane, adds up across lanes and has every value as a scalar.  (Each thread reading the sums of
