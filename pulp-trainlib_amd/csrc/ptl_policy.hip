@@ -6,7 +6,10 @@
 // scalars need behind its sum is some hundred instructions, which every thread works on by itself: no further barrier.  The thread that has the
 // action's class adds to it where it writes.  Rows that no workgroup holds (more than 16384 pieces of 16 bytes) are read twice; where
 // the rows are too few to fill the chip each is cut into parts: one launch leaves every part's maximum and sum, the next one joins
-// them and writes.
+// them and writes.  Logits come and gradients go past the caches (2048 rows of 32000 classes in fp16: 54.5 us through them, 51.1 with the stores past
+// them, 49.3 with both).
+// Measured, loss and gradient: 2048 rows of 32000 classes in fp16 49 us (5.3 TB/s), 1024 in fp32 48 (5.4); 500 of 131072 in fp16 59; 8192 of 1000
+// 9; 4 rows of 131072 in fp32 8 us in two launches.
 #include "ptl_soft_rows.hpp"
 #include "ptl_tuning.h"
 
@@ -37,11 +40,11 @@ __device__ inline float policy_away(float d, float &rest) {
     return e;
 }
 template <typename T>
-__device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, size_t row, int action, float za, float max, float sum, bool mine) {
+__device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, size_t row, int action, float za, float max, float log_sum, bool mine) {
     PolicyRow r = {0.f, (unsigned)action < (unsigned)a.dim};
     float lp = 0.f, loss = 0.f;
     if (r.some) {
-        lp = (za - max) * a.inv_t - logf(sum);
+        lp = (za - max) * a.inv_t - log_sum;
         const float ratio = expf(lp - a.old[row]), A = a.adv[row], w = a.weight * (a.row_weight ? a.row_weight[row] : 1.f);
         // (no number: both products are compared in vain)
         const float whole = ratio * A, clipped = fminf(fmaxf(ratio, a.low), a.high) * A;
@@ -62,7 +65,7 @@ __device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, size_t row, int a
 }
 // The gradient of the classes that are held.
 template <typename T, int NT, int NP, bool MINE>
-__device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const SoftExp<T> &e, float sum, const PolicyRow &r, int action, int dim) {
+__device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const SoftRatio<T> &e, float sum, const PolicyRow &r, int action, int dim) {
     constexpr int VEC = RowPiece<T>::VEC;
     int mine = first + row_thread<NT>();
     asm volatile("" : "+v"(mine));  // (the loads' addresses are not kept for the stores)
@@ -86,10 +89,7 @@ __device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first,
         if (MINE) {
             if (p < end) o.store(row, p, dim);
         } else {
-#ifndef NT_PUT
-#define NT_PUT false
-#endif
-            o.template put<NP == 1, NT_PUT>(row, p, dim);
+            o.template put<NP == 1, true>(row, p, dim);
         }
     }
 }
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const P
     RowPiece<T> z[HELD];
     float top[2] = {-__builtin_inff(), 0.f}, sum[2] = {0.f, 0.f}, za;
     if constexpr (NP > 0) {
-        soft_hold<T, NT, HELD, MINE>(z, zr, 0, pieces, a.dim);
+        soft_hold<T, NT, HELD, MINE, true>(z, zr, 0, pieces, a.dim);
     }
     const int action = policy_action(a, row, za);
     float own = 0.f;
@@ -134,16 +134,17 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const P
         own = top[0];
     }
     group_reduce<NT, true>(top, lds);
-    const SoftExp<T> e(top[0], a);
+    const SoftRatio<T> e(top[0], a);
     if constexpr (NP > 0) {
         soft_as_read<T>(z);
         sum[0] = soft_sum<T, NT, HELD, MINE>(z, e, a.dim);
         soft_as_read<T>(z);
     } else {
         if (own != -__builtin_inff()) sum[0] *= soft_exp(own, top[0], a);
+        if constexpr (sizeof(T) == 2) sum[0] *= __builtin_amdgcn_exp2f(-e.rest);  // (the walk's are whole exponentials)
     }
     group_reduce<NT, false>(sum, lds + 32);
-    const PolicyRow r = policy_row(a, row, action, za, top[0], sum[0], row_thread<NT>() == 0);
+    const PolicyRow r = policy_row(a, row, action, za, top[0], e.log(sum[0]), row_thread<NT>() == 0);
     if (!a.grad) return;
     T *gr = a.grad + row * a.dim;
     if constexpr (NP > 0) {
@@ -198,9 +199,10 @@ __global__ __launch_bounds__(POLICY_NT) void policy_join_kernel(const PolicyArgs
         sum[0] += v.x == -__builtin_inff() ? v.y : v.y * soft_exp(v.x, top[0], a);
     }
     group_reduce<NT, false>(sum, lds + 32);
-    const PolicyRow r = policy_row(a, row, action, za, top[0], sum[0], blockIdx.x == 0 && threadIdx.x == 0);
+    const SoftRatio<T> e(top[0], a);
+    const PolicyRow r = policy_row(a, row, action, za, top[0], logf(sum[0]), blockIdx.x == 0 && threadIdx.x == 0);
     if (!a.grad) return;
-    policy_put<T, NT, NP, true>(z, a.grad + row * a.dim, first, end, SoftExp<T>(top[0], a), sum[0], r, action, a.dim);
+    policy_put<T, NT, NP, true>(z, a.grad + row * a.dim, first, end, e, sizeof(T) == 2 ? sum[0] * __builtin_amdgcn_exp2f(-e.rest) : sum[0], r, action, a.dim);
 }
 
 template <typename T, int NT, int NP>

@@ -52,6 +52,21 @@ struct SoftExp {
     }
 };
 
+// ... but for a factor of the whole row, the exponential of `rest`, where only ratios count and the logarithm of the sum is corrected by it: an
+// instruction less for each class.
+template <typename T>
+struct SoftRatio : SoftExp<T> {
+    __device__ inline SoftRatio(float max, const SoftScale &a) : SoftExp<T>(max, a) {}
+    __device__ inline float operator()(T z) const {
+        if constexpr (sizeof(T) == 4) return SoftExp<T>::operator()(z);
+        else return __builtin_amdgcn_exp2f(fmaf((float)z, this->a.hi, this->m));
+    }
+    __device__ inline float log(float sum) const {
+        if constexpr (sizeof(T) == 4) return logf(sum);
+        else return fmaf(this->rest, 0.693147181f, logf(sum));
+    }
+};
+
 // NT threads have a row: a workgroup, or (64) one wave of a workgroup of four, which needs no barriers.
 template <int NT>
 __device__ inline int row_thread() { return NT == 64 ? (int)(threadIdx.x & 63) : (int)threadIdx.x; }
@@ -90,13 +105,13 @@ __device__ inline void group_reduce(float (&v)[2], float *lds) {
 
 // NP pieces of logits in each of NT threads, from piece `first` on.  MINE: each piece has its own classes only, and what the row does
 // not have is -inf; else a thread may have classes that are another's too (RowPiece::cut), which only the sum has to know.
-template <typename T, int NT, int NP, bool MINE>
+template <typename T, int NT, int NP, bool MINE, bool STREAM = false>
 __device__ inline void soft_hold(RowPiece<T> (&z)[NP], const T *row, int first, int end, int dim) {
     constexpr int VEC = RowPiece<T>::VEC;
     constexpr bool SHORT = NP == 1;  // rows of less than a piece: one piece a thread
     if (!MINE && !(SHORT && dim < VEC)) {
 #pragma unroll
-        for (int j = 0; j < NP; ++j) z[j].template hold<false>(row, first + j * NT + row_thread<NT>(), dim);
+        for (int j = 0; j < NP; ++j) z[j].template hold<false, STREAM>(row, first + j * NT + row_thread<NT>(), dim);
         return;
     }
 #pragma unroll
@@ -138,8 +153,8 @@ __device__ inline float soft_max(const RowPiece<T> (&z)[NP]) {
         return m;
     }
 }
-template <typename T, int NT, int NP, bool MINE>
-__device__ inline float soft_sum(const RowPiece<T> (&z)[NP], const SoftExp<T> &e, int dim) {
+template <typename T, int NT, int NP, bool MINE, typename E>
+__device__ inline float soft_sum(const RowPiece<T> (&z)[NP], const E &e, int dim) {
     float s = 0.f;
 #pragma unroll
     for (int j = 0; j < NP; ++j) {
