@@ -1,6 +1,7 @@
-// Dense layers with bias, activation and residual in their product: y = act(x W^T + b) + skip, forward and backward.  The product and what follows it are
-// rows_product()'s: the residual's rows are read in the layout in which the outputs are written, one step ahead of it, and reach the lanes that have
-// the sums through the wave's share of LDS, so that both pass memory in whole 16-byte pieces and the output is rounded once.
+// Dense layers with bias, activation and residual in their product: y = act(x W^T + b) + skip, forward and backward.  The product and what
+// follows it are rows_product()'s: the sums go through the wave's share of LDS as they are, in 32 bits, and bias, activation and residual are
+// applied in the layout in which the outputs are written, so that residual, hidden values and outputs pass memory in whole 16-byte pieces
+// and are rounded once.
 #include "ptl_gate_bw.inc"
 #include "ptl_rows_mm.inc"
 #include "ptl_tuning.h"
