@@ -11,9 +11,10 @@
 //     slower).  The two products' tiles differ in length (2 n_out against the number of tokens): the longer ones come first in the grid and the
 //     shorter ones fill up behind them.
 //   * Where that leaves compute units idle k is cut into parts, each with sums of its own in fp32, which another launch adds up.
-// fp16, 2048 tokens, 2048 -> 5632: 205 us (920 TFLOP/s; with the gradients of the pre-activations 226 to 235), as a dense layer's call 245;
+// fp16, 2048 tokens, 2048 -> 5632: 200 us (945 TFLOP/s; with the gradients of the pre-activations 224 to 230), as a dense layer's call 245;
 // 256 tokens of the same layer 58 and 82, 64 tokens 31 and 49.  fp32, 2048 tokens, 1024 -> 2816: 391 us (121 TFLOP/s) and 461.
 // Rows that are no whole 16-byte pieces come as copies (rows_copy(), gate_back_kernel): fp16, 2047 -> 5631 252 us with them.
+// fp16: loads, fragments and matrix instructions follow each other one by one, a slab's last step behind its barrier (gated 229 -> 225 us).
 // Tried: slabs of 32 k, four of them in flight, instead of two of 64: 3 to 8 % longer.
 #include "ptl_rows_mm.inc"
 
@@ -136,34 +137,95 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
 #pragma unroll
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
     const int kg = lane >> 5, lr = lane & 31;
-    auto compute = [&](unsigned stage) {
-        const char *tf = smem + stage, *ts = tf + C::TILE;
-        uint4 ff[2][2], sf[2][FN];
-        auto load = [&](int ks, int set) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) ff[set][i] = grad_frag<T, 128>(tf, ww * 2 + i, lane, 2 * ks + kg);
-#pragma unroll
-            for (int j = 0; j < FN; ++j)
-                sf[set][j] = ROWS ? read_frag<half_t, XR, FILL_VEC_K>(ts, (wt * FN + j) * 32 + lr, ks, kg) : grad_frag<T, XR>(ts, wt * FN + j, lane, 2 * ks + kg);
-        };
-        load(0, 0);
-#pragma unroll
-        for (int t = 0; t < 4; ++t) {
-            if (t < 3) load(t + 1, (t + 1) & 1);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < FN; ++j) mfma_step<T>(acc[i][j], ff[t & 1][i], sf[t & 1][j]);
-        }
+    uint4 ff[2][2], sf[2][FN];  // fragments of a step and of the next
+    auto first = [&](unsigned stage, int ks, int i) { ff[ks & 1][i] = grad_frag<T, 128>(smem + stage, ww * 2 + i, lane, 2 * ks + kg); };
+    auto other = [&](unsigned stage, int ks, int j) {
+        const char *ts = smem + stage + C::TILE;
+        sf[ks & 1][j] = ROWS ? read_frag<half_t, XR, FILL_VEC_K>(ts, (wt * FN + j) * 32 + lr, ks, kg) : grad_frag<T, XR>(ts, wt * FN + j, lane, 2 * ks + kg);
     };
-    issue(0);
-    unsigned out = 0;
-    for (int s = 0; s < slabs; ++s) {
-        wait_vmcnt<0>();
+    auto load = [&](unsigned stage, int ks) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) first(stage, ks, i);
+#pragma unroll
+        for (int j = 0; j < FN; ++j) other(stage, ks, j);
+    };
+    if constexpr (ES == 2) {
+        // step t of what is in registers, while those of step `to` are read from `from` and (dma) a slab's loads go to `into`: one by one
+        // between the matrix instructions
+        static_assert(FN == 2, "four of each");
+        auto step = [&](int t, unsigned from, int to, bool dma, unsigned into) {
+            const unsigned at = ring + into + (unsigned)wave * 1024u;
+#pragma unroll
+            for (int m = 0; m < 4; ++m) {
+                if (m & 1) first(from, to, m >> 1);
+                else other(from, to, m >> 1);
+                if (dma) {
+                    lds_dma16_saddr(f_off[m], f_ptr, at + m * 4096u);
+                    lds_dma16_saddr(s_off[m], s_ptr, at + C::TILE + m * 4096u);
+                }
+                mfma_step<T>(acc[m >> 1][m & 1], ff[t & 1][m >> 1], sf[t & 1][m & 1]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        };
+        // The barrier of a slab lies in front of its last step, whose fragments are in registers by then: its place takes the next slab but one.
+        issue(0);
+        if (slabs > 1) {
+            issue(C::STAGE);
+            wait_vmcnt<4 + LX>();
+        } else {
+            wait_vmcnt<0>();
+        }
         __syncthreads();
-        if (s + 1 < slabs) issue(C::STAGE - out);
-        compute(out);
-        out = C::STAGE - out;
+        unsigned out = 0;
+        load(0, 0);
+        step(0, 0, 1, false, 0);
+        step(1, 0, 2, false, 0);
+        step(2, 0, 3, false, 0);
+        int s = 0;
+        for (; s + 2 < slabs - (tail == KS ? 0 : 1); ++s) {  // (slab s + 2 is a whole one)
+            wait_vmcnt<0>();
+            __syncthreads();
+            const unsigned from = C::STAGE - out;
+            step(3, from, 0, true, out);
+            f_ptr += f_step;
+            s_ptr += s_step;
+            step(0, from, 1, false, 0);
+            step(1, from, 2, false, 0);
+            step(2, from, 3, false, 0);
+            --left;
+            out = from;
+        }
+        for (; s + 1 < slabs; ++s) {
+            wait_vmcnt<0>();
+            __syncthreads();
+            if (s + 2 < slabs) issue(out);
+            const unsigned from = C::STAGE - out;
+            step(3, from, 0, false, 0);
+            step(0, from, 1, false, 0);
+            step(1, from, 2, false, 0);
+            step(2, from, 3, false, 0);
+            out = from;
+        }
+#pragma unroll
+        for (int m = 0; m < 4; ++m) mfma_step<T>(acc[m >> 1][m & 1], ff[1][m >> 1], sf[1][m & 1]);
+    } else {
+        issue(0);
+        unsigned out = 0;
+        for (int s = 0; s < slabs; ++s) {
+            wait_vmcnt<0>();
+            __syncthreads();
+            if (s + 1 < slabs) issue(C::STAGE - out);
+            load(out, 0);
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (t < 3) load(out, t + 1);
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < FN; ++j) mfma_step<T>(acc[i][j], ff[t & 1][i], sf[t & 1][j]);
+            }
+            out = C::STAGE - out;
+        }
     }
     __syncthreads();
     float *w_tab = reinterpret_cast<float *>(smem), *b_tab = w_tab + C::ROWS_W, *x_tab = b_tab + C::ROWS_W;

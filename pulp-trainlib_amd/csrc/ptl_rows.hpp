@@ -47,9 +47,11 @@ struct RowPiece {
     // Piece p of a row of `dim` elements.  No load depends on where the row ends: a piece that reaches over the end is read so that
     // it ends there, and trim() moves its values down and puts zeros behind them (only the waves that hold such a piece do).  All
     // of a thread's pieces are fetched before the first is trimmed.
+    template <bool STREAM = false>
     __device__ inline void fetch(const T *row, int p, int dim) {
         if (dim >= VEC) {
-            raw = *reinterpret_cast<const row_u4 *>(row + min(p * VEC, dim - VEC));
+            const row_u4 *from = reinterpret_cast<const row_u4 *>(row + min(p * VEC, dim - VEC));
+            raw = STREAM ? __builtin_nontemporal_load(from) : *from;
         } else {
             // (rows shorter than a piece: value by value, the last one first)
             typedef typename std::conditional<sizeof(T) == 4, unsigned, typename std::conditional<sizeof(T) == 2, unsigned short, unsigned char>::type>::type Bits;

@@ -71,6 +71,33 @@ struct Gate {
         const float d = slope > 0.f ? slope * (one ? 1.f : x * fmaf(3.f * k3 * x, x, k1)) : (x != x ? x : 0.f);
         return relu ? (x > 0.f ? 1.f : x != x ? x : 0.f) : one ? d : s + d;
     }
+    // The same of one activation (of each a code of its own, without the selects: 2048 x 5632 gradients through gelu in fp16, bound by the
+    // vector units, take 26 us with those and 20 so): slope = e / (1 + e)^2 with e = exp(-|p|) is the same on both sides of 0, and 0 where d p / d x, which is taken
+    // of a bounded x, could grow beyond all bounds.  EXACT: the exponent to 2^-24 of itself, otherwise to 2^-22.
+    template <int ACT, bool EXACT>
+    __device__ static inline float slope(float x) {
+        if constexpr (ACT == GATE_RELU) return x > 0.f ? 1.f : x != x ? x : 0.f;
+        constexpr bool GELU = ACT == GATE_GELU;
+        constexpr float K1 = 1.5957691216057308f, K3 = 0.07135481627260025f, LOG2E = 1.44269502f;
+        float p, n;  // n: -|p| log2(e)
+        if constexpr (EXACT) {
+            p = GELU ? x * fmaf(K3 * x, x, K1) : x;
+            n = -fabsf(p);
+            n = fmaf(n, LOG2E, n * 1.92596299e-8f);
+        } else {
+            p = GELU ? x * fmaf(K3 * LOG2E * x, x, K1 * LOG2E) : x * LOG2E;
+            n = -fabsf(p);
+        }
+        const float e = __builtin_amdgcn_exp2f(n), r = __builtin_amdgcn_rcpf(1.f + e), t = e * r, d = t * r;
+        if constexpr (ACT == GATE_SIGMOID) return d;
+        const float b = __builtin_amdgcn_fmed3f(x, -256.f, 256.f), s = p < 0.f ? t : r;
+        return fmaf(d, GELU ? b * fmaf(3.f * K3 * b, b, K1) : b, s);
+    }
+    template <bool EXACT>
+    __device__ static inline float slope(int act, float x) {
+        return act == GATE_SIGMOID ? slope<GATE_SIGMOID, EXACT>(x) : act == GATE_SILU ? slope<GATE_SILU, EXACT>(x)
+             : act == GATE_GELU ? slope<GATE_GELU, EXACT>(x) : slope<GATE_RELU, EXACT>(x);
+    }
 };
 
 // Both products behind the gradients of a gated layer's pre-activations (dw or dx NULL: not wanted).  x and w have rows of `cols` values
