@@ -6,12 +6,14 @@
 //     side; a fragment's reads touch eight k at the same 64 of them, a quarter of the banks: the 64-byte blocks of row k are therefore
 //     exchanged by k % 4 (on the way in, where a lane chooses which piece it loads).  fp32: a value is a dword, and a fragment four reads
 //     of 32 neighbours each.
-//   * fp16: tiles of 128 x 128 with two workgroups a compute unit, one of which stores or waits while the other multiplies; fp32: 128 x 64,
+//   * fp16: large layers take tiles of 256 x 128 and three slabs, one workgroup a compute unit: a fragment's way out of LDS costs half of what
+//     the matrix instructions take, and what comes in on top a third less than with 128 x 128.  Smaller ones those, with two workgroups a
+//     compute unit, one of which stores or waits while the other multiplies.  fp32: 128 x 64,
 //     three (its instructions take sixteen times as long: smaller tiles cost nothing and leave less of the chip idle; 128 x 128 were 5 to 30 %
 //     slower).  The two products' tiles differ in length (2 n_out against the number of tokens): the longer ones come first in the grid and the
 //     shorter ones fill up behind them.
 //   * Where that leaves compute units idle k is cut into parts, each with sums of its own in fp32, which another launch adds up.
-// fp16, 2048 tokens, 2048 -> 5632: 200 us (945 TFLOP/s; with the gradients of the pre-activations 224 to 230), as a dense layer's call 245;
+// fp16, 2048 tokens, 2048 -> 5632: 185 us (1020 TFLOP/s; with the gradients of the pre-activations 210), as a dense layer's call 245;
 // 256 tokens of the same layer 58 and 82, 64 tokens 31 and 49.  fp32, 2048 tokens, 1024 -> 2816: 391 us (121 TFLOP/s) and 461.
 // Rows that are no whole 16-byte pieces come as copies (rows_copy(), gate_back_kernel): fp16, 2047 -> 5631 252 us with them.
 // fp16: loads, fragments and matrix instructions follow each other one by one, a slab's last step behind its barrier (gated 229 -> 225 us).
@@ -20,15 +22,16 @@
 
 namespace ptl {
 
-template <typename OUT, int XR>  // tiles of 128 inputs by XR rows of the other operand
+template <typename OUT, int XR, int FW>  // tiles of FW inputs by XR rows of the other operand
 struct GradTile {
     typedef OUT Out;
     typedef f32x16 Acc;
     static constexpr RowsAfter AFTER_SUMS = ROWS_SCALED;
     static constexpr bool GATED = false;
-    static constexpr int ROWS_W = 128, ROWS_X = XR, WM = 64, WN = XR / 2, FM = 2, FN = XR / 64, OC = 64, PITCH = OC * (int)sizeof(OUT) + 16, GROUPS = 1;
-    static constexpr int NT = 256, TILE = 128 * ROWB, STAGE = TILE + XR * ROWB, RING = 2 * STAGE, TABLE = (2 * ROWS_W + ROWS_X) * 4;
-    static_assert(TABLE + 4 * 32 * PITCH <= RING, "what follows the sums fits the ring");
+    static constexpr int ROWS_W = FW, ROWS_X = XR, WM = 64, WN = XR / 2, FM = 2, FN = XR / 64, OC = 64, PITCH = OC * (int)sizeof(OUT) + 16, GROUPS = 1;
+    static constexpr int NT = 2 * FW, NS = FW == 256 ? 3 : 2, HALF = 128 * ROWB, TILE = FW * ROWB, STAGE = TILE + XR * ROWB, RING = NS * STAGE;
+    static constexpr int TABLE = (2 * ROWS_W + ROWS_X) * 4;
+    static_assert(TABLE + FW / 32 * 32 * PITCH <= RING, "what follows the sums fits the ring");
 };
 
 struct GradProd {
@@ -73,10 +76,10 @@ __device__ inline uint4 grad_frag(const char *tile, int block, int lane, int chu
 __host__ __device__ inline size_t grad_part(int tokens, int outs) { return ((size_t)tokens * outs + 3) & ~(size_t)3; }
 
 // ROWS: the second operand has k along its rows.
-template <typename T, int XR, bool ROWS>
+template <typename T, int XR, int FW, bool ROWS>
 __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
-    typedef GradTile<T, XR> C;
-    typedef GradTile<float, XR> P;
+    typedef GradTile<T, XR, FW> C;
+    typedef GradTile<float, XR, FW> P;
     constexpr int NT = C::NT, ES = (int)sizeof(T), VEC = 16 / ES, KS = ROWB / ES;  // k of a slab
     constexpr int PER = 128 / VEC, XPER = XR / VEC, LX = XR * 8 / NT, FN = C::FN;      // pieces of a k's rows, loads of a thread for the second tile
     const RowsArgs &a = g.out;
@@ -84,7 +87,7 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wt = wave & 1, ww = wave >> 1;
     int tw, tt;
     rows_place(a, id - z * tiles, tw, tt);
-    const int o0 = tw * 128, t0 = tt * XR, slabs = (k_n + KS - 1) / KS, tail = k_n - (slabs - 1) * KS;
+    const int o0 = tw * FW, t0 = tt * XR, slabs = (k_n + KS - 1) / KS, tail = k_n - (slabs - 1) * KS;
     const unsigned ring = (unsigned)(uintptr_t)(lds_char *)smem;
     const char *f_ptr = g.f + (long long)o0 * ES + (long long)k0 * g.f_b;
     const char *s_ptr = (z < g.high ? g.s : g.low) + (ROWS ? (long long)t0 * g.s_b + (long long)k0 * ES : (long long)t0 * ES + (long long)k0 * g.s_b);
@@ -96,8 +99,9 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
     bool f_none[4], s_none[LX];
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-        const int q = j * NT + tid, k = q / PER;
-        f_off[j] = (unsigned)k * (unsigned)g.f_b + (unsigned)min(place(q, PER), (g.f_n - o0) / VEC - 1) * 16u;
+        constexpr int HALF = C::HALF / 16;  // (a wide tile is two narrow ones, one behind the other)
+        const int q = (j * NT + tid) % HALF, k = q / PER;
+        f_off[j] = (unsigned)k * (unsigned)g.f_b + (unsigned)min(place(q, PER) + (j * NT + tid) / HALF * PER, (g.f_n - o0) / VEC - 1) * 16u;
         f_none[j] = k >= tail;
     }
 #pragma unroll
@@ -117,14 +121,14 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
         const unsigned to = ring + stage + (unsigned)wave * 1024u;
         if (--left > 0 || tail == KS) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) lds_dma16_saddr(f_off[j], f_ptr, to + j * 4096u);
+            for (int j = 0; j < 4; ++j) lds_dma16_saddr(f_off[j], f_ptr, to + j * NT * 16u);
 #pragma unroll
-            for (int j = 0; j < LX; ++j) lds_dma16_saddr(s_off[j], s_ptr, to + C::TILE + j * 4096u);
+            for (int j = 0; j < LX; ++j) lds_dma16_saddr(s_off[j], s_ptr, to + C::TILE + j * NT * 16u);
         } else {  // k that the last slab does not have
 #pragma unroll
-            for (int j = 0; j < 4; ++j) lds_dma<16>(f_none[j] ? a.zeros : f_ptr + f_off[j], to + j * 4096u);
+            for (int j = 0; j < 4; ++j) lds_dma<16>(f_none[j] ? a.zeros : f_ptr + f_off[j], to + j * NT * 16u);
 #pragma unroll
-            for (int j = 0; j < LX; ++j) lds_dma<16>(s_none[j] ? a.zeros : s_ptr + s_off[j], to + C::TILE + j * 4096u);
+            for (int j = 0; j < LX; ++j) lds_dma<16>(s_none[j] ? a.zeros : s_ptr + s_off[j], to + C::TILE + j * NT * 16u);
         }
         f_ptr += f_step;
         s_ptr += s_step;
@@ -138,7 +142,7 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
             for (int v = 0; v < 16; ++v) acc[i][j][v] = 0.f;
     const int kg = lane >> 5, lr = lane & 31;
     uint4 ff[2][2], sf[2][FN];  // fragments of a step and of the next
-    auto first = [&](unsigned stage, int ks, int i) { ff[ks & 1][i] = grad_frag<T, 128>(smem + stage, ww * 2 + i, lane, 2 * ks + kg); };
+    auto first = [&](unsigned stage, int ks, int i) { ff[ks & 1][i] = grad_frag<T, 128>(smem + stage + (ww >> 1) * C::HALF, (ww & 1) * 2 + i, lane, 2 * ks + kg); };
     auto other = [&](unsigned stage, int ks, int j) {
         const char *ts = smem + stage + C::TILE;
         sf[ks & 1][j] = ROWS ? read_frag<half_t, XR, FILL_VEC_K>(ts, (wt * FN + j) * 32 + lr, ks, kg) : grad_frag<T, XR>(ts, wt * FN + j, lane, 2 * ks + kg);
@@ -150,60 +154,68 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
         for (int j = 0; j < FN; ++j) other(stage, ks, j);
     };
     if constexpr (ES == 2) {
-        // step t of what is in registers, while those of step `to` are read from `from` and (dma) a slab's loads go to `into`: one by one
-        // between the matrix instructions
-        static_assert(FN == 2, "four of each");
-        auto step = [&](int t, unsigned from, int to, bool dma, unsigned into) {
+        // step t of what is in registers, while those of step `to` are read from `from` and loads d0 .. d0 + PER_STEP - 1 of a slab go to `into`
+        // (d0 < 0: none): one by one between the matrix instructions.  (Two slabs at a time in LDS: all loads in the first step, since they
+        // are needed a slab later; three: over the four of them.)
+        static_assert(FN == 2, "four matrix instructions a step");
+        constexpr int NS = C::NS, L = 4 + LX, PER_STEP = NS == 2 ? L : (L + 3) / 4;
+        auto step = [&](int t, unsigned from, int to, int d0, unsigned into) {
             const unsigned at = ring + into + (unsigned)wave * 1024u;
 #pragma unroll
             for (int m = 0; m < 4; ++m) {
                 if (m & 1) first(from, to, m >> 1);
                 else other(from, to, m >> 1);
-                if (dma) {
-                    lds_dma16_saddr(f_off[m], f_ptr, at + m * 4096u);
-                    lds_dma16_saddr(s_off[m], s_ptr, at + C::TILE + m * 4096u);
+                if (d0 >= 0) {
+#pragma unroll
+                    for (int j = d0 + m * PER_STEP / 4; j < d0 + (m + 1) * PER_STEP / 4; ++j) {
+                        if (j >= L) break;
+                        if (j < 4) lds_dma16_saddr(f_off[j], f_ptr, at + j * NT * 16u);
+                        else lds_dma16_saddr(s_off[j - 4], s_ptr, at + C::TILE + (j - 4) * NT * 16u);
+                    }
                 }
                 mfma_step<T>(acc[m >> 1][m & 1], ff[t & 1][m >> 1], sf[t & 1][m & 1]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         };
-        // The barrier of a slab lies in front of its last step, whose fragments are in registers by then: its place takes the next slab but one.
-        issue(0);
-        if (slabs > 1) {
-            issue(C::STAGE);
-            wait_vmcnt<4 + LX>();
-        } else {
-            wait_vmcnt<0>();
+        // Slab s lies in place s % NS.  Its barrier lies in front of its last step, whose fragments are in registers by then: its place takes
+        // slab s + NS.
+        auto next = [](unsigned stage) { return stage + C::STAGE == C::RING ? 0u : stage + C::STAGE; };
+        unsigned in = 0, out = 0;
+        for (int s = 0; s < NS; ++s) {
+            if (s < slabs) issue(in);
+            in = next(in);
         }
+        if (slabs >= NS) wait_vmcnt<(NS - 1) * L>();
+        else wait_vmcnt<0>();
         __syncthreads();
-        unsigned out = 0;
         load(0, 0);
-        step(0, 0, 1, false, 0);
-        step(1, 0, 2, false, 0);
-        step(2, 0, 3, false, 0);
+        step(0, 0, 1, -1, 0);
+        step(1, 0, 2, -1, 0);
+        step(2, 0, 3, -1, 0);
         int s = 0;
-        for (; s + 2 < slabs - (tail == KS ? 0 : 1); ++s) {  // (slab s + 2 is a whole one)
-            wait_vmcnt<0>();
+        for (; s + NS < slabs - (tail == KS ? 0 : 1); ++s) {  // (slab s + NS is a whole one)
+            wait_vmcnt<(NS - 2) * L>();
             __syncthreads();
-            const unsigned from = C::STAGE - out;
-            step(3, from, 0, true, out);
+            const unsigned from = next(out);
+            step(3, from, 0, 0, out);
+            step(0, from, 1, PER_STEP < L ? PER_STEP : -1, out);
+            step(1, from, 2, 2 * PER_STEP < L ? 2 * PER_STEP : -1, out);
+            step(2, from, 3, 3 * PER_STEP < L ? 3 * PER_STEP : -1, out);
             f_ptr += f_step;
             s_ptr += s_step;
-            step(0, from, 1, false, 0);
-            step(1, from, 2, false, 0);
-            step(2, from, 3, false, 0);
             --left;
             out = from;
         }
         for (; s + 1 < slabs; ++s) {
-            wait_vmcnt<0>();
+            if (s + NS <= slabs) wait_vmcnt<(NS - 2) * L>();
+            else wait_vmcnt<0>();
             __syncthreads();
-            if (s + 2 < slabs) issue(out);
-            const unsigned from = C::STAGE - out;
-            step(3, from, 0, false, 0);
-            step(0, from, 1, false, 0);
-            step(1, from, 2, false, 0);
-            step(2, from, 3, false, 0);
+            if (s + NS < slabs) issue(out);
+            const unsigned from = next(out);
+            step(3, from, 0, -1, 0);
+            step(0, from, 1, -1, 0);
+            step(1, from, 2, -1, 0);
+            step(2, from, 3, -1, 0);
             out = from;
         }
 #pragma unroll
@@ -240,12 +252,12 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
     }
 }
 
-template <typename T, int XR>
-__global__ __launch_bounds__((GradTile<T, XR>::NT)) void grad_kernel(const GradArgs a) {
+template <typename T, int XR, int FW>
+__global__ __launch_bounds__((GradTile<T, XR, FW>::NT)) void grad_kernel(const GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
     const int second = (int)blockIdx.x >= a.first, id = second ? (int)blockIdx.x - a.first : (int)blockIdx.x;
-    if ((second ^ a.lead) == 0) grad_tile<T, XR, true>(a.p[0], id, smem);
-    else grad_tile<T, XR, false>(a.p[1], id, smem);
+    if ((second ^ a.lead) == 0) grad_tile<T, XR, FW, true>(a.p[0], id, smem);
+    else grad_tile<T, XR, FW, false>(a.p[1], id, smem);
 }
 
 // The parts' sums, in their order, rounded once: four values a thread.
@@ -288,7 +300,7 @@ __global__ __launch_bounds__(256) void grad_join_kernel(const GradJoin<T> a) {
 // and tile is 0.67 of a compute unit, 1.18 to a workgroup alone, the rest of a workgroup two slabs, what remains behind 1.7 times a
 // short one (fitted to 14 layers with 20 choices each: 7 % off in the mean, the choice 1.05 times the best in the mean, 1.11 at most).
 // Parts cost their sums, written and read at 5 TB/s, and a launch.
-static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const double (&values)[2], const int (&parts)[2], bool fp32) {
+static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const double (&values)[2], const int (&parts)[2], bool fp32, int wide) {
     const int cu = state().num_cu;
     const float rest = fp32 ? 1.8f : 0.f;
     float work = 0, longest = 0, shortest = 1e9f, extra = 0, groups = 0;
@@ -307,13 +319,13 @@ static float grad_cost(const int (&tiles)[2], const int (&slabs)[2], const doubl
         const float spread = 0.67f * (work / cu + 1.7f * shortest), chain = longest * (groups <= 3.f * cu ? alone : 1.18f);
         return (spread > chain ? spread : chain) + (extra > 0 ? 0.72f * extra + 3.5f : 0.f);
     }
-    const float spread = work / (2 * cu) + 0.5f * shortest;
+    const float spread = work / ((wide == 128 ? 2 : 1) * cu) + 0.5f * shortest;
     return (spread > longest ? spread : longest) + (extra > 0 ? extra + 4.f : 0.f);
 }
 
 template <typename T>
 struct GradSizes {
-    static constexpr int XR = sizeof(T) == 4 ? 64 : 128, RING = GradTile<T, XR>::RING, KS = ROWB / (int)sizeof(T);
+    static constexpr int XR = sizeof(T) == 4 ? 64 : 128, KS = ROWB / (int)sizeof(T);
 };
 // Slabs of k of product i, of a part, and parts.
 template <typename T>
@@ -323,31 +335,39 @@ static void grad_cut(int i, int parts, int ns, int rows, int &chunk, int &high) 
     high = (slabs + chunk - 1) / chunk;
 }
 
+template <typename T, int FW>
+static bool grad_ready() {
+    static bool ready = false;
+    constexpr int XR = GradSizes<T>::XR;
+    if (!ready)
+        ready = hip_ok(hipFuncSetAttribute(reinterpret_cast<const void *>(grad_kernel<T, XR, FW>), hipFuncAttributeMaxDynamicSharedMemorySize, GradTile<T, XR, FW>::RING),
+                       "hipFuncSetAttribute");
+    return ready;
+}
+
 template <typename T>
 int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in, int rows) {
     constexpr int XR = GradSizes<T>::XR, KS = GradSizes<T>::KS;
-    static bool ready = false;
-    if (!ready) {
-        if (!hip_ok(hipFuncSetAttribute(reinterpret_cast<const void *>(grad_kernel<T, XR>), hipFuncAttributeMaxDynamicSharedMemorySize, GradSizes<T>::RING),
-                    "hipFuncSetAttribute"))
-            return 2;
-        ready = true;
-    }
+    // Of 30 layers in fp16 (256 to 8192 tokens, 256 to 8192 inputs and outputs) tiles of 256 inputs take 0.94 times as long from 16 GFLOP on
+    // (0.89 to 1.03) and below 1.01 (0.99 to 1.05): one workgroup a compute unit shares what two would read, but fewer of them fill the chip less evenly.
+    p.wide = sizeof(T) == 2 && 2.0 * ns * in * rows * (dw + dx) >= 16e9 ? 256 : 128;
+    if (!(p.wide == 128 ? grad_ready<T, 128>() : grad_ready<T, sizeof(T) == 2 ? 256 : 128>())) return 2;
     const bool wanted[2] = {dx, dw};
     const int n[2] = {ns, rows}, k[2] = {rows, ns};
     int tiles[2], slabs[2];
     double values[2];
     for (int i = 0; i < 2; ++i) {
-        tiles[i] = wanted[i] ? (in + 127) / 128 * ((n[i] + XR - 1) / XR) : 0;
+        tiles[i] = wanted[i] ? (in + p.wide - 1) / p.wide * ((n[i] + XR - 1) / XR) : 0;
         slabs[i] = (k[i] + KS - 1) / KS;
         values[i] = (double)n[i] * in;
     }
-    p = {{1, 1}, 0};
+    p.parts[0] = p.parts[1] = 1;
+    p.bytes = 0;
     float best = 1e30f;
     for (int u = 1; u <= 32 && (u == 1 || (tiles[0] && u * 4 <= slabs[0])); u *= 2)
         for (int v = 1; v <= 32 && (v == 1 || (tiles[1] && v * 4 <= slabs[1])); v *= 2) {
             const int parts[2] = {u, v};
-            const float c = grad_cost(tiles, slabs, values, parts, sizeof(T) == 4);
+            const float c = grad_cost(tiles, slabs, values, parts, sizeof(T) == 4, p.wide);
             if (c < best) {
                 best = c;
                 p.parts[0] = u;
@@ -366,7 +386,7 @@ int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in
 template <typename T>
 int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols,
                    int pitch) {
-    constexpr int XR = GradSizes<T>::XR, RING = GradSizes<T>::RING;
+    constexpr int XR = GradSizes<T>::XR;
     GradArgs a = {};
     T *y[2] = {dx, dw};
     const int n[2] = {ns, rows}, k[2] = {rows, ns};
@@ -377,7 +397,7 @@ int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, co
         p.out.outs = in;
         p.out.tokens = n[i];
         p.out.zeros = static_cast<const char *>(state().zeros);
-        p.out.tiles_w = (in + 127) / 128;
+        p.out.tiles_w = (in + parts.wide - 1) / parts.wide;
         p.out.tiles_t = (n[i] + XR - 1) / XR;
         p.f = reinterpret_cast<const char *>(i ? x : w);
         p.s = reinterpret_cast<const char *>(dh);
@@ -403,7 +423,12 @@ int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, co
     int groups[2];
     for (int i = 0; i < 2; ++i) groups[i] = y[i] ? a.p[i].out.tiles_w * a.p[i].out.tiles_t * a.p[i].parts : 0;
     a.first = groups[a.lead];
-    hipLaunchKernelGGL((grad_kernel<T, XR>), dim3(groups[0] + groups[1]), dim3(GradTile<T, XR>::NT), RING, state().stream, a);
+    auto launch = [&](auto wide) {
+        typedef GradTile<T, XR, decltype(wide)::value> C;
+        hipLaunchKernelGGL((grad_kernel<T, XR, decltype(wide)::value>), dim3(groups[0] + groups[1]), dim3(C::NT), C::RING, state().stream, a);
+    };
+    if (parts.wide == 128) launch(std::integral_constant<int, 128>{});
+    else launch(std::integral_constant<int, sizeof(T) == 2 ? 256 : 128>{});
     if (parts.bytes) {
         const size_t fours = j.n[0] + j.n[1];
         hipLaunchKernelGGL((grad_join_kernel<T>), dim3((unsigned)((fours + 255) / 256)), dim3(256), 0, state().stream, j);

@@ -106,6 +106,7 @@ struct Gate {
 // dx and of dw is taken and what workspace their sums need, `ws`, which a call has in hand before its first launch.
 constexpr float GRAD_LOW = 2048.f;
 struct GradParts {
+    int wide;  // inputs of a tile
     int parts[2];
     size_t bytes;
 };
