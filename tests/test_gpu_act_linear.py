@@ -251,3 +251,47 @@ def test_same_as_a_dense_layer(pkg, gpu, dt):
     pkg.call("ptl_linear_%s_fw_batched" % dt, l, n)
     ref = x.double() @ w.double().t() + b.double()
     tr.within(y, out.double().cpu(), 2 * (U * (n_in + 4) * (x.double().abs() @ w.double().abs().t()) + U * 2 * ref.abs() + tr.step(ref, dt)))
+
+
+@pytest.mark.parametrize("n,n_in,n_out", [(1000, 1500, 4100), (4096, 1000, 1100), (1500, 2056, 4000), (4000, 1000, 2100), (2500, 776, 3001)])
+def test_forward_large_tiles(pkg, gpu, n, n_in, n_out):
+    """fp16 tiles of 256 x 128, 256 x 256 and 128 x 128 whose last rows, tokens and values of k are no whole tiles, slabs or pieces."""
+    for act, skip, keep in (("gelu", 1, 1), ("none", 1, 0)):
+        x, w, b, s = inputs(n, "fp16", n, n_in, n_out, 1, skip)
+        check_forward("fp16", act, x, w, b, s, *forward(pkg, gpu, "fp16", act, x, w, b, s, keep))
+
+
+@pytest.mark.parametrize("n,n_in,n_out", [(2100, 1000, 2003), (2048, 1032, 2048), (2000, 1001, 2100), (8300, 300, 1700)])
+def test_backward_large_tiles(pkg, gpu, n, n_in, n_out):
+    """Gradients of 16 GFLOP and more in fp16: tiles of 256 x 128, both products and each alone."""
+    x, w, _, _ = inputs(n, "fp16", n, n_in, n_out)
+    h, dy = tr.rand(n + 5, n, n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    check_backward("fp16", "gelu", x, w, h, dy, *backward(pkg, gpu, "fp16", "gelu", x, w, h, dy, 1))
+
+
+@pytest.mark.parametrize("n,n_in,n_out", [(4100, 1000, 2003), (2100, 2050, 2000)])
+def test_backward_large_tiles_alone(pkg, gpu, n, n_in, n_out):
+    x, w, _, _ = inputs(n, "fp16", n, n_in, n_out)
+    h, dy = tr.rand(n + 5, n, n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, 1, skip_wg=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, dx, None, None)
+    dh, dx, dw, db = backward(pkg, gpu, "fp16", "silu", x, w, h, dy, 1, skip_ig=1)
+    check_backward("fp16", "silu", x, w, h, dy, dh, None, dw, db)
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("act", ["silu", "gelu", "relu", "sigmoid"])
+@pytest.mark.parametrize("n", [1, 40])
+def test_backward_far_values(pkg, gpu, dt, act, n):
+    """Derivatives of far and infinite pre-activations take their limits; what is no number stays where it is."""
+    top = torch.finfo(tr.t_dtype(dt)).max
+    far = [0.0, -0.0, 200.0, -200.0, 300.0, -300.0, top, -top, float("inf"), -float("inf"), float("nan"), 1.0]
+    h = torch.tensor([far] * n, dtype=tr.t_dtype(dt))
+    dy = torch.ones_like(h)
+    x, w = torch.zeros(n, 5, dtype=h.dtype), torch.zeros(len(far), 5, dtype=h.dtype)
+    dh, _, _, _ = backward(pkg, gpu, dt, act, x, w, h, dy, 0)
+    at0 = {"silu": 0.5, "gelu": 0.5, "relu": 0.0, "sigmoid": 0.25}[act]
+    hi = 0.0 if act == "sigmoid" else 1.0
+    want = torch.tensor([at0, at0] + [hi, 0.0] * 4, dtype=torch.float64).expand(n, 10)
+    assert torch.equal(dh[:, :10].double().cpu(), want)
+    assert torch.isnan(dh[:, 10]).all() and torch.isfinite(dh[:, 11]).all()
