@@ -175,23 +175,25 @@ __device__ inline void adam_copy(const AdamTensor &t, size_t at, long left, size
         for (int i = 0; i < 4; ++i) f.e[i] = (float)p.w.e[i];
         f.store(t.master_out, at, left);
     }
-    if (t.m_out == t.m) return;
+    // (each moment and each scale may have a place of its own, or that of the old one)
     if (t.m_scale_out) {
-        Adam4<int8_t> c = {};
-        if (t.m) c.load<false>(t.m, at, left);
-        c.store(t.m_out, at, left);
-        if (t.m) c.load<false>(t.v, at, left);
-        c.store(t.v_out, at, left);
-        if (lane == 0) {
-            t.m_scale_out[block] = t.m ? t.m_scale[block] : 0.f;
-            t.v_scale_out[block] = t.m ? t.v_scale[block] : 0.f;
-        }
+        auto codes = [&](const void *from, void *to) {
+            Adam4<int8_t> c = {};
+            if (from) c.load<false>(from, at, left);
+            if (from != to) c.store(to, at, left);
+        };
+        codes(t.m, t.m_out);
+        codes(t.v, t.v_out);
+        if (lane == 0 && t.m_scale != t.m_scale_out) t.m_scale_out[block] = t.m ? t.m_scale[block] : 0.f;
+        if (lane == 0 && t.v_scale != t.v_scale_out) t.v_scale_out[block] = t.m ? t.v_scale[block] : 0.f;
     } else {
-        Adam4<float> f = {};
-        if (t.m) f.load<false>(t.m, at, left);
-        f.store(t.m_out, at, left);
-        if (t.m) f.load<false>(t.v, at, left);
-        f.store(t.v_out, at, left);
+        auto moments = [&](const void *from, void *to) {
+            Adam4<float> f = {};
+            if (from) f.load<false>(from, at, left);
+            if (from != to) f.store(to, at, left);
+        };
+        moments(t.m, t.m_out);
+        moments(t.v, t.v_out);
     }
 }
 
@@ -409,7 +411,8 @@ static int adamw_multi(const Args *list, int count, const adamw_step *s, const c
         if (n == 0) continue;
         const adamw_state *from = a.state, *to = a.new_state ? a.new_state : a.state;
         const auto *out = a.updated ? a.updated : a.weights;
-        if (k.count == ADAM_TENSORS && !flush()) return sg.finish(2);
+        const size_t more = (n + group - 1) / group;
+        if ((k.count == ADAM_TENSORS || (groups + more) * 256 > (size_t)ROW_THREADS) && !flush()) return sg.finish(2);
         AdamTensor &t = k.t[k.count];
         t = {};
         auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
@@ -443,7 +446,7 @@ static int adamw_multi(const Args *list, int count, const adamw_step *s, const c
         t.lr = a.learning_rate;
         t.decay = a.weight_decay;
         k.first[k.count] = groups;
-        groups += (unsigned)((n + group - 1) / group);
+        groups += (unsigned)more;
         ++k.count;
     }
     return sg.finish(flush() ? 0 : 2);

@@ -316,3 +316,24 @@ def test_host_arrays(pkg, gpu, eight):
     before = [{k: v.clone() for k, v in d.items() if v is not None} for d in c.dev]
     got = c.run(t=2, in_place=True, factor=torch.tensor([float("inf")]))
     assert all(torch.equal(d[k], v) for d, b in zip(got, before) for k, v in b.items())
+
+
+@pytest.mark.parametrize("master", [False, True])
+@pytest.mark.parametrize("eight", [False, True])
+@pytest.mark.parametrize("shared", [("m", "mq"), ("v", "vq", "ms"), ("ms",), ("vs", "mq", "vq"), ("master",)])
+def test_some_places_shared_without_a_step(pkg, gpu, eight, master, shared):
+    """Without a finite factor every part of a new state that is not the old one's place receives what that holds, whichever others are."""
+    c = Case(pkg, "fp16", [5, 700], lambda i: eight, master=master)
+    for d, o in zip(c.dev, c.out):
+        for k in shared:
+            if o.get(k) is not None:
+                o[k] = d[k]
+    before = [{k: v.clone() for k, v in d.items() if v is not None} for d in c.dev]
+    for o, d, b in zip(c.run(t=3, factor=torch.tensor([float("nan")], device="cuda")), c.dev, before):
+        assert all(torch.equal(d[k], b[k]) for k in b)
+        assert torch.equal(o["w"], (b["master"] if master else b["w"]).to(o["w"].dtype))
+        assert all(torch.equal(v, b[k]) for k, v in o.items() if k != "w" and v is not None)
+    c.untouched()
+    for d, o in zip(c.dev, c.out):
+        for k in shared:
+            assert o.get(k) is None or o[k] is d[k]
