@@ -652,8 +652,9 @@ __global__ __launch_bounds__(1024) void join_sums_kernel(const JoinBw<T> a, int 
 template <typename T>
 static int join_deal(JoinBw<T> &a, bool groups, int want, int of, int &gates) {
     const int all = (a.rows + a.per - 1) / a.per;
+    const bool fits = (long)all * ((a.dim + 31) / 32) <= ROW_THREADS / 2048;  // (workgroups that add up a gate's columns, of 1024 threads)
     a.parts = 1;
-    gates = !groups ? 0 : want >= 2 * all && a.per >= 2 * of ? 1 : 2;
+    gates = !groups ? 0 : want >= 2 * all && a.per >= 2 * of && fits ? 1 : 2;
     if (gates == 1) {
         const int most = (a.per + of - 1) / of;
         a.parts = want / all < most ? want / all : most;

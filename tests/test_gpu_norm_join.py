@@ -287,3 +287,18 @@ def test_host_arrays(pkg, gpu):
     a, keep = tn.join_args(pkg, dim, alpha=ALPHA, per=per, **{k: h[k] for k in ("b", "s", "w1", "w2", "gate", "dy", "ds")}, **out)
     pkg.call("ptl_norm_join_fp16_bw_batched", a, n)
     assert all(torch.equal(torch.from_numpy(out[k]), want[k].cpu()) for k in out)
+
+
+def test_many_gates_of_the_longest_rows(pkg, gpu, monkeypatch):
+    """Rows of 2^24 values with six gates: more columns of gates than one launch has threads to add up in parts.  The rows repeat 1024 values, so
+    that means are those of 1024, and every column's results are those of the first 1024; the sums are as long as the rows."""
+    n, dim, per = 12, 1024, 2
+    t = make(11, "fp16", n, dim, per)
+    long = {k: None if v is None else v.cuda().repeat(*([1] * (v.dim() - 1)), 1 << 14) for k, v in t.items()}
+    got = backward(pkg, gpu, "fp16", long, per=per)
+    for k, v in got.items():
+        blocks = v.view(-1, 1 << 14, dim)
+        assert (blocks == blocks[:, :1]).all(), k
+    reach = chain(1 << 24)
+    monkeypatch.setitem(globals(), "chain", lambda d: reach)
+    check_backward("fp16", t, {k: v[..., :dim] for k, v in got.items()}, per=per)
