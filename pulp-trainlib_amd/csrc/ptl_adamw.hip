@@ -6,7 +6,7 @@
 // root is found without a barrier.  The tensors' places travel in the kernel's arguments, 32 tensors a launch: no table in memory has to
 // be written, and the launches can be captured.
 // Measured: 23 million fp32 weights and moments 110 us (5.9 TB/s), 92 million fp16 weights with copies and moments in 8 bits 247 us (6.0); a large
-// copy reaches 5.0 on the same card.  1 million fp32 weights in 16 tensors 7.3 us.
+// copy reaches 5.0 on the same card.  1 million fp32 weights in 12 tensors 7.3 us.
 // In 8 bits the roots are held, not the moments: a block's moments span decades (v the squares of m's), and the fourth root brings
 // the 65025^2 that v spans between its smallest code and its largest to 255.
 #include "ptl_row_sums.hpp"
