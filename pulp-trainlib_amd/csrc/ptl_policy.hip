@@ -8,8 +8,8 @@
 // the rows are too few to fill the chip each is cut into parts: one launch leaves every part's maximum and sum, the next one joins
 // them and writes.  Logits come and gradients go past the caches (2048 rows of 32000 classes in fp16: 54.5 us through them, 51.1 with the stores past
 // them, 49.3 with both).
-// Measured, loss and gradient: 2048 rows of 32000 classes in fp16 49 us (5.3 TB/s), 1024 in fp32 48 (5.4); 500 of 131072 in fp16 59; 8192 of 1000
-// 9; 4 rows of 131072 in fp32 8 us in two launches.
+// Measured, loss and gradient: 2048 rows of 32000 classes in fp16 48 us (5.4 TB/s), 1024 in fp32 48 (5.4); 500 of 131072 in fp16 59; 8192 of 1000
+// 9; 4 rows of 131072 in fp32 8 to 9 us in two launches.
 #include "ptl_soft_rows.hpp"
 #include "ptl_tuning.h"
 
@@ -27,6 +27,14 @@ struct PolicyArgs : SoftScale {
     float low, high, beta, weight;  // low, high: the borders of the ratio
 };
 
+// What a row is given, on its way while its logits are (2048 rows of 32000 classes in fp16 49.2 us, 48.4 so).
+struct PolicyGiven {
+    float old, ref, adv, weight;
+};
+template <typename T>
+__device__ inline PolicyGiven policy_given(const PolicyArgs<T> &a, size_t row) {
+    return {a.old[row], a.ref ? a.ref[row] : 0.f, a.adv[row], a.row_weight ? a.row_weight[row] : 1.f};
+}
 // What is left of a row behind its maximum and sum.
 struct PolicyRow {
     float slope;  // d loss / d z_a but for the softmax, 0 for rows that are left out
@@ -40,19 +48,19 @@ __device__ inline float policy_away(float d, float &rest) {
     return e;
 }
 template <typename T>
-__device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, size_t row, int action, float za, float max, float log_sum, bool mine) {
+__device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, const PolicyGiven &given, size_t row, int action, float za, float max, float log_sum, bool mine) {
     PolicyRow r = {0.f, (unsigned)action < (unsigned)a.dim};
     float lp = 0.f, loss = 0.f;
     if (r.some) {
         lp = (za - max) * a.inv_t - log_sum;
-        const float ratio = expf(lp - a.old[row]), A = a.adv[row], w = a.weight * (a.row_weight ? a.row_weight[row] : 1.f);
+        const float ratio = expf(lp - given.old), A = given.adv, w = a.weight * given.weight;
         // (no number: both products are compared in vain)
         const float whole = ratio * A, clipped = fminf(fmaxf(ratio, a.low), a.high) * A;
         loss = whole <= clipped ? -whole : clipped < whole ? -clipped : whole + clipped;
         r.slope = whole <= clipped ? -whole : clipped < whole ? 0.f : whole + clipped;
         if (a.ref) {
             float rest;
-            const float e = policy_away(a.ref[row] - lp, rest);
+            const float e = policy_away(given.ref - lp, rest);
             loss = fmaf(a.beta, rest, loss);
             r.slope = fmaf(-a.beta, e, r.slope);
         }
@@ -118,6 +126,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const P
         soft_hold<T, NT, HELD, MINE, true>(z, zr, 0, pieces, a.dim);
     }
     const int action = policy_action(a, row, za);
+    const PolicyGiven given = policy_given(a, row);
     float own = 0.f;
     if constexpr (NP > 0) {
         top[0] = soft_max<T>(z);
@@ -144,7 +153,7 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const P
         if constexpr (sizeof(T) == 2) sum[0] *= __builtin_amdgcn_exp2f(-e.rest);  // (the walk's are whole exponentials)
     }
     group_reduce<NT, false>(sum, lds + 32);
-    const PolicyRow r = policy_row(a, row, action, za, top[0], e.log(sum[0]), row_thread<NT>() == 0);
+    const PolicyRow r = policy_row(a, given, row, action, za, top[0], e.log(sum[0]), row_thread<NT>() == 0);
     if (!a.grad) return;
     T *gr = a.grad + row * a.dim;
     if constexpr (NP > 0) {
@@ -190,17 +199,22 @@ __global__ __launch_bounds__(POLICY_NT) void policy_join_kernel(const PolicyArgs
     RowPiece<T> z[NP];
     if (a.grad) soft_hold<T, NT, NP, true>(z, a.z + row * a.dim, first, end, a.dim);
     const int action = a.action[row];
+    const PolicyGiven given = policy_given(a, row);
     const float za = part[a.parts].x;
     float top[2] = {-__builtin_inff(), 0.f}, sum[2] = {0.f, 0.f};
-    for (int i = threadIdx.x; i < a.parts; i += NT) top[0] = fmaxf(top[0], part[i].x);
+    float2 mine = threadIdx.x < a.parts ? part[threadIdx.x] : make_float2(-__builtin_inff(), 0.f);  // (most rows have no more than that)
+    top[0] = mine.x;
+    for (int i = threadIdx.x + NT; i < a.parts; i += NT) top[0] = fmaxf(top[0], part[i].x);
     group_reduce<NT, true>(top, lds);
-    for (int i = threadIdx.x; i < a.parts; i += NT) {
-        const float2 v = part[i];
-        sum[0] += v.x == -__builtin_inff() ? v.y : v.y * soft_exp(v.x, top[0], a);
+    for (int i = threadIdx.x;;) {
+        sum[0] += mine.x == -__builtin_inff() ? mine.y : mine.y * soft_exp(mine.x, top[0], a);
+        i += NT;
+        if (i >= a.parts) break;
+        mine = part[i];
     }
     group_reduce<NT, false>(sum, lds + 32);
     const SoftRatio<T> e(top[0], a);
-    const PolicyRow r = policy_row(a, row, action, za, top[0], logf(sum[0]), blockIdx.x == 0 && threadIdx.x == 0);
+    const PolicyRow r = policy_row(a, given, row, action, za, top[0], logf(sum[0]), blockIdx.x == 0 && threadIdx.x == 0);
     if (!a.grad) return;
     policy_put<T, NT, NP, true>(z, a.grad + row * a.dim, first, end, e, sizeof(T) == 2 ? sum[0] * __builtin_amdgcn_exp2f(-e.rest) : sum[0], r, action, a.dim);
 }

@@ -295,3 +295,11 @@ def test_backward_far_values(pkg, gpu, dt, act, n):
     want = torch.tensor([at0, at0] + [hi, 0.0] * 4, dtype=torch.float64).expand(n, 10)
     assert torch.equal(dh[:, :10].double().cpu(), want)
     assert torch.isnan(dh[:, 10]).all() and torch.isfinite(dh[:, 11]).all()
+
+
+@pytest.mark.parametrize("dt", ["fp32", "fp16"])
+@pytest.mark.parametrize("n_in,n_out", [(1, 2050), (1000, 3001), (3001, 2111), (6100, 2048), (6200, 2049)])
+def test_one_token_many_outputs(pkg, gpu, dt, n_in, n_out):
+    for act, skip, keep in (("silu", 1, 1), ("none", 0, 0)):
+        x, w, b, s = inputs(n_in, dt, 1, n_in, n_out, 1, skip)
+        check_forward(dt, act, x, w, b, s, *forward(pkg, gpu, dt, act, x, w, b, s, keep))
