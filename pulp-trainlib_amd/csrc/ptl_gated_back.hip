@@ -47,6 +47,10 @@ struct GradProd {
 struct GradArgs {
     GradProd p[2];  // dx, dW
     int first, lead;  // workgroups of the product that comes first, and which one that is
+    int tiles;        // ... of both; behind them: of db
+    const float *shares;
+    void *db;
+    int rows, n_shares;
 };
 
 // 16 bytes of a row (eight k; fp32: four) of a 32-row fragment from a [k][row] tile; chunk: k / 8, k / 4.
@@ -255,6 +259,12 @@ __device__ inline void grad_tile(const GradProd &g, int id, char *smem) {
 template <typename T, int XR, int FW>
 __global__ __launch_bounds__((GradTile<T, XR, FW>::NT)) void grad_kernel(const GradArgs a) {
     extern __shared__ __attribute__((aligned(16))) char smem[];
+    if ((int)blockIdx.x >= a.tiles) {
+        typedef GradTile<T, XR, FW> C;
+        static_assert(sizeof(LongSum<T>) * 1024 <= C::RING, "fits the ring");
+        row_shares_of<T, C::NT>(a.shares, static_cast<T *>(a.db), a.rows, a.n_shares, (int)blockIdx.x - a.tiles, reinterpret_cast<LongSum<T>(*)[32]>(smem));
+        return;
+    }
     const int second = (int)blockIdx.x >= a.first, id = second ? (int)blockIdx.x - a.first : (int)blockIdx.x;
     if ((second ^ a.lead) == 0) grad_tile<T, XR, FW, true>(a.p[0], id, smem);
     else grad_tile<T, XR, FW, false>(a.p[1], id, smem);
@@ -385,7 +395,7 @@ int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in
 
 template <typename T>
 int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols,
-                   int pitch) {
+                   int pitch, const float *shares, T *db, int n_shares) {
     constexpr int XR = GradSizes<T>::XR;
     GradArgs a = {};
     T *y[2] = {dx, dw};
@@ -423,9 +433,15 @@ int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, co
     int groups[2];
     for (int i = 0; i < 2; ++i) groups[i] = y[i] ? a.p[i].out.tiles_w * a.p[i].out.tiles_t * a.p[i].parts : 0;
     a.first = groups[a.lead];
+    a.tiles = groups[0] + groups[1];
+    a.shares = shares;
+    a.db = db;
+    a.rows = rows;
+    a.n_shares = n_shares;
+    const int all = a.tiles + (db ? (rows + 31) / 32 : 0);
     auto launch = [&](auto wide) {
         typedef GradTile<T, XR, decltype(wide)::value> C;
-        hipLaunchKernelGGL((grad_kernel<T, XR, decltype(wide)::value>), dim3(groups[0] + groups[1]), dim3(C::NT), C::RING, state().stream, a);
+        hipLaunchKernelGGL((grad_kernel<T, XR, decltype(wide)::value>), dim3(all), dim3(C::NT), C::RING, state().stream, a);
     };
     if (parts.wide == 128) launch(std::integral_constant<int, 128>{});
     else launch(std::integral_constant<int, sizeof(T) == 2 ? 256 : 128>{});
@@ -439,8 +455,9 @@ int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, co
 template int gated_products_plan<half_t>(GradParts &, bool, bool, bool, int, int, int);
 template int gated_products_plan<float>(GradParts &, bool, bool, bool, int, int, int);
 template int gated_products<half_t>(const GradParts &, float *, const half_t *, const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int,
-                                    int);
-template int gated_products<float>(const GradParts &, float *, const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int);
+                                    int, const float *, half_t *, int);
+template int gated_products<float>(const GradParts &, float *, const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int,
+                                   const float *, float *, int);
 
 void rows_copy(const void *w, size_t n_w, const void *x, size_t n_x, void *to, int bytes, int pitch) {
     rows_copies(static_cast<const char *>(w), n_w, static_cast<const char *>(x), n_x, static_cast<char *>(to), bytes, pitch);

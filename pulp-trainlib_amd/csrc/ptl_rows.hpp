@@ -152,28 +152,37 @@ __device__ inline void row_reduce(float (&v)[N], float (*lds)[N]) {
 
 // out[c] = the sum over the shares of part[share][c]: 32 columns (a 128-byte line) a workgroup, 32 shares at a time with four loads in
 // flight, so that a few thousand columns fill the chip (1024 shares of 4096: 18 us with 64 columns and 4 shares at a time, 5 so).
-template <typename T>
-__global__ __launch_bounds__(1024) void row_shares_kernel(const float *__restrict__ part, T *__restrict__ out, int dim, int shares) {
-    const int o = threadIdx.x & 31, g = threadIdx.x >> 5, c = (int)(blockIdx.y * gridDim.x + blockIdx.x) * 32 + o;
-    LongSum<T> s;
-    s.clear();
-    if (c < dim) {
-        int z = g;
-        for (; z + 96 < shares; z += 128) {
-            float v[4];
+// The columns 32 group .. of a workgroup of NT threads: each of the 32 walks in its order, whichever thread has it.
+template <typename T, int NT>
+__device__ inline void row_shares_of(const float *__restrict__ part, T *__restrict__ out, int dim, int shares, int group, LongSum<T> (*red)[32]) {
+    const int o = threadIdx.x & 31, c = group * 32 + o;
 #pragma unroll
-            for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(z + 32 * u) * dim + c];
+    for (int g = threadIdx.x >> 5; g < 32; g += NT / 32) {
+        LongSum<T> s;
+        s.clear();
+        if (c < dim) {
+            int z = g;
+            for (; z + 96 < shares; z += 128) {
+                float v[4];
 #pragma unroll
-            for (int u = 0; u < 4; ++u) s.add(v[u]);
+                for (int u = 0; u < 4; ++u) v[u] = part[(size_t)(z + 32 * u) * dim + c];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) s.add(v[u]);
+            }
+            for (; z < shares; z += 32) s.add(part[(size_t)z * dim + c]);
         }
-        for (; z < shares; z += 32) s.add(part[(size_t)z * dim + c]);
+        red[g][o] = s;
     }
-    __shared__ LongSum<T> red[32][32];
-    red[g][o] = s;
     __syncthreads();
-    if (g != 0 || c >= dim) return;
+    if (threadIdx.x >= 32 || c >= dim) return;
+    LongSum<T> s = red[0][o];
     for (int k = 1; k < 32; ++k) s.add(red[k][o]);
     out[c] = (T)s.value();
+}
+template <typename T>
+__global__ __launch_bounds__(1024) void row_shares_kernel(const float *__restrict__ part, T *__restrict__ out, int dim, int shares) {
+    __shared__ LongSum<T> red[32][32];
+    row_shares_of<T, 1024>(part, out, dim, shares, (int)(blockIdx.y * gridDim.x + blockIdx.x), red);
 }
 template <typename T>
 inline void row_shares(const float *part, T *out, int dim, int shares) {
