@@ -303,3 +303,13 @@ def test_one_token_many_outputs(pkg, gpu, dt, n_in, n_out):
     for act, skip, keep in (("silu", 1, 1), ("none", 0, 0)):
         x, w, b, s = inputs(n_in, dt, 1, n_in, n_out, 1, skip)
         check_forward(dt, act, x, w, b, s, *forward(pkg, gpu, dt, act, x, w, b, s, keep))
+
+
+@pytest.mark.parametrize("act", ["none", "relu"])
+@pytest.mark.parametrize("bias", [0, 1])
+@pytest.mark.parametrize("n,n_in,n_out", [(1200, 80, 2564), (4000, 100, 2001), (2500, 600, 515), (530, 1031, 2500), (3100, 512, 500), (340, 1801, 2050)])
+def test_backward_with_and_without_copies(pkg, gpu, act, bias, n, n_in, n_out):
+    """fp16 rows of which some or all are no whole 16-byte pieces, on both sides of the sizes from which they are copied."""
+    x, w, _, _ = inputs(n, "fp16", n, n_in, n_out)
+    h, dy = None if act == "none" else tr.rand(n + 5, n, n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    check_backward("fp16", act, x, w, h, dy, *backward(pkg, gpu, "fp16", act, x, w, h, dy, bias))
