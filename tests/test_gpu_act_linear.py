@@ -313,3 +313,11 @@ def test_backward_with_and_without_copies(pkg, gpu, act, bias, n, n_in, n_out):
     x, w, _, _ = inputs(n, "fp16", n, n_in, n_out)
     h, dy = None if act == "none" else tr.rand(n + 5, n, n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
     check_backward("fp16", act, x, w, h, dy, *backward(pkg, gpu, "fp16", act, x, w, h, dy, bias))
+
+
+@pytest.mark.parametrize("act", ["none", "gelu"])
+@pytest.mark.parametrize("n,n_in,n_out", [(10, 2048, 1640), (16, 1504, 1400), (33, 1024, 2000), (100, 2056, 1000), (9, 2048, 1824), (17, 8192, 256)])
+def test_backward_few_tokens_and_large_weights(pkg, gpu, act, n, n_in, n_out):
+    x, w, _, _ = inputs(n, "fp16", n, n_in, n_out)
+    h, dy = None if act == "none" else tr.rand(n + 5, n, n_out, scale=1.5, dt="fp16"), tr.rand(n + 6, n, n_out, scale=0.5, dt="fp16")
+    check_backward("fp16", act, x, w, h, dy, *backward(pkg, gpu, "fp16", act, x, w, h, dy, 1))
