@@ -72,8 +72,8 @@ __device__ inline PolicyRow policy_row(const PolicyArgs<T> &a, const PolicyGiven
     return r;
 }
 // The gradient of the classes that are held.
-template <typename T, int NT, int NP, bool MINE>
-__device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const SoftRatio<T> &e, float sum, const PolicyRow &r, int action, int dim) {
+template <typename T, int NT, int NP, bool MINE, typename E>
+__device__ inline void policy_put(const RowPiece<T> (&z)[NP], T *row, int first, int end, const E &e, float sum, const PolicyRow &r, int action, int dim) {
     constexpr int VEC = RowPiece<T>::VEC;
     int mine = first + row_thread<NT>();
     asm volatile("" : "+v"(mine));  // (the loads' addresses are not kept for the stores)
@@ -109,8 +109,8 @@ __device__ inline int policy_action(const PolicyArgs<T> &a, size_t row, float &z
     return c;
 }
 
-// NP = 0: the row is read twice.
-template <typename T, int NT, int NP>
+// NP = 0: the row is read twice.  E: the classes' exponentials.
+template <typename T, typename E, int NT, int NP>
 __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const PolicyArgs<T> a) {
     __shared__ __attribute__((aligned(16))) float lds[64];
     const int wave = NT == 64 ? __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) : 0;
@@ -143,14 +143,14 @@ __global__ __launch_bounds__(NT == 64 ? 256 : NT) void policy_row_kernel(const P
         own = top[0];
     }
     group_reduce<NT, true>(top, lds);
-    const SoftRatio<T> e(top[0], a);
+    const E e(top[0], a);
     if constexpr (NP > 0) {
         soft_as_read<T>(z);
         sum[0] = soft_sum<T, NT, HELD, MINE>(z, e, a.dim);
         soft_as_read<T>(z);
     } else {
         if (own != -__builtin_inff()) sum[0] *= soft_exp(own, top[0], a);
-        if constexpr (sizeof(T) == 2) sum[0] *= __builtin_amdgcn_exp2f(-e.rest);  // (the walk's are whole exponentials)
+        sum[0] = e.unit(sum[0]);  // (the walk's are whole exponentials)
     }
     group_reduce<NT, false>(sum, lds + 32);
     const PolicyRow r = policy_row(a, given, row, action, za, top[0], e.log(sum[0]), row_thread<NT>() == 0);
@@ -189,7 +189,7 @@ __global__ __launch_bounds__(POLICY_NT) void policy_part_kernel(const PolicyArgs
     if (blockIdx.x == 0) part[a.parts] = make_float2(za, 0.f);
 }
 // ... which every workgroup of the row joins before it writes its part's gradient.
-template <typename T>
+template <typename T, typename E>
 __global__ __launch_bounds__(POLICY_NT) void policy_join_kernel(const PolicyArgs<T> a) {
     constexpr int NT = POLICY_NT, NP = POLICY_NP, VEC = RowPiece<T>::VEC;
     __shared__ __attribute__((aligned(16))) float lds[64];
@@ -213,24 +213,24 @@ __global__ __launch_bounds__(POLICY_NT) void policy_join_kernel(const PolicyArgs
         mine = part[i];
     }
     group_reduce<NT, false>(sum, lds + 32);
-    const SoftRatio<T> e(top[0], a);
+    const E e(top[0], a);
     const PolicyRow r = policy_row(a, given, row, action, za, top[0], logf(sum[0]), blockIdx.x == 0 && threadIdx.x == 0);
     if (!a.grad) return;
-    policy_put<T, NT, NP, true>(z, a.grad + row * a.dim, first, end, e, sizeof(T) == 2 ? sum[0] * __builtin_amdgcn_exp2f(-e.rest) : sum[0], r, action, a.dim);
+    policy_put<T, NT, NP, true>(z, a.grad + row * a.dim, first, end, e, e.unit(sum[0]), r, action, a.dim);
 }
 
-template <typename T, int NT, int NP>
+template <typename T, typename E, int NT, int NP>
 static void policy_rows(PolicyArgs<T> a, int ns) {
     const int most = (int)(ROW_THREADS / NT);
     for (; a.first < ns; a.first += most) {
         const int n = ns - a.first < most ? ns - a.first : most;
         a.rows = a.first + n;
-        if (NT == 64) hipLaunchKernelGGL((policy_row_kernel<T, NT, NP>), dim3((n + 3) / 4), dim3(256), 0, state().stream, a);
-        else hipLaunchKernelGGL((policy_row_kernel<T, NT, NP>), dim3(n), dim3(NT), 0, state().stream, a);
+        if (NT == 64) hipLaunchKernelGGL((policy_row_kernel<T, E, NT, NP>), dim3((n + 3) / 4), dim3(256), 0, state().stream, a);
+        else hipLaunchKernelGGL((policy_row_kernel<T, E, NT, NP>), dim3(n), dim3(NT), 0, state().stream, a);
     }
 }
 
-template <typename T>
+template <typename T, typename E>
 static int policy_launch(PolicyArgs<T> &a, int ns) {
     const int pieces = (a.dim + RowPiece<T>::VEC - 1) / RowPiece<T>::VEC, cu = state().num_cu;
     if (pieces > 4096 && (long)ns * (a.dim > 65536 ? 2 : 6) <= cu) {
@@ -243,30 +243,30 @@ static int policy_launch(PolicyArgs<T> &a, int ns) {
         a.part = reinterpret_cast<float2 *>(workspace(sizeof(float2) * (size_t)ns * (a.parts + 1)));
         if (!a.part) return 2;
         hipLaunchKernelGGL((policy_part_kernel<T>), dim3(a.parts, ns), dim3(POLICY_NT), 0, state().stream, a);
-        hipLaunchKernelGGL((policy_join_kernel<T>), dim3(a.grad ? a.parts : 1, ns), dim3(POLICY_NT), 0, state().stream, a);
+        hipLaunchKernelGGL((policy_join_kernel<T, E>), dim3(a.grad ? a.parts : 1, ns), dim3(POLICY_NT), 0, state().stream, a);
     } else if ((pieces <= 256 && ns >= 4 * cu) || (pieces <= 512 && ns >= 16 * cu)) {
-        if (pieces <= 64) policy_rows<T, 64, 1>(a, ns);
-        else if (pieces <= 128) policy_rows<T, 64, 2>(a, ns);
-        else if (pieces <= 256) policy_rows<T, 64, 4>(a, ns);
-        else policy_rows<T, 64, 8>(a, ns);
+        if (pieces <= 64) policy_rows<T, E, 64, 1>(a, ns);
+        else if (pieces <= 128) policy_rows<T, E, 64, 2>(a, ns);
+        else if (pieces <= 256) policy_rows<T, E, 64, 4>(a, ns);
+        else policy_rows<T, E, 64, 8>(a, ns);
     } else if (pieces <= 256) {
-        policy_rows<T, 256, 1>(a, ns);
+        policy_rows<T, E, 256, 1>(a, ns);
     } else if (pieces <= 512) {
-        policy_rows<T, 256, 2>(a, ns);
+        policy_rows<T, E, 256, 2>(a, ns);
     } else if (pieces <= 1024) {
-        policy_rows<T, 256, 4>(a, ns);
+        policy_rows<T, E, 256, 4>(a, ns);
     } else if (pieces <= 2048) {
-        policy_rows<T, 256, 8>(a, ns);
+        policy_rows<T, E, 256, 8>(a, ns);
     } else if (pieces <= 4096) {
-        policy_rows<T, 512, 8>(a, ns);
+        policy_rows<T, E, 512, 8>(a, ns);
     } else if (pieces <= 8192) {
-        policy_rows<T, 1024, 8>(a, ns);
+        policy_rows<T, E, 1024, 8>(a, ns);
     } else if (pieces <= 12288) {
-        policy_rows<T, 1024, 12>(a, ns);
+        policy_rows<T, E, 1024, 12>(a, ns);
     } else if (pieces <= 16384) {
-        policy_rows<T, 1024, 16>(a, ns);
+        policy_rows<T, E, 1024, 16>(a, ns);
     } else {
-        policy_rows<T, 1024, 0>(a, ns);
+        policy_rows<T, E, 1024, 0>(a, ns);
     }
     return hip_ok(hipGetLastError(), "policy loss launch") ? 0 : 2;
 }
@@ -305,7 +305,10 @@ static int policy_step(const Args *a, int ns, int step, const char *fn) {
     d.high = 1.f + a->clip_high;
     d.beta = a->beta;
     d.weight = a->weight;
-    return sg.finish(policy_launch<T>(d, ns));
+    if constexpr (sizeof(T) == 2) {
+        if (a->temperature >= SOFT_RATIO_LEAST) return sg.finish(policy_launch<T, SoftRatio>(d, ns));
+    }
+    return sg.finish(policy_launch<T, SoftExp<T>>(d, ns));
 }
 
 }  // namespace ptl

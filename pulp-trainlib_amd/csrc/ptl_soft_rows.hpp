@@ -50,21 +50,21 @@ struct SoftExp {
             return __builtin_amdgcn_exp2f(fmaf((float)z, a.hi, m) + rest);
         }
     }
+    // The logarithm of a sum of these, and what a sum of whole exponentials is in their unit.
+    __device__ inline float log(float sum) const { return logf(sum); }
+    __device__ inline float unit(float sum) const { return sum; }
 };
 
-// ... but for a factor of the whole row, the exponential of `rest`, where only ratios count and the logarithm of the sum is corrected by it: an
-// instruction less for each class.
-template <typename T>
-struct SoftRatio : SoftExp<T> {
-    __device__ inline SoftRatio(float max, const SoftScale &a) : SoftExp<T>(max, a) {}
-    __device__ inline float operator()(T z) const {
-        if constexpr (sizeof(T) == 4) return SoftExp<T>::operator()(z);
-        else return __builtin_amdgcn_exp2f(fmaf((float)z, this->a.hi, this->m));
-    }
-    __device__ inline float log(float sum) const {
-        if constexpr (sizeof(T) == 4) return logf(sum);
-        else return fmaf(this->rest, 0.693147181f, logf(sum));
-    }
+// ... of fp16 but for a factor of the whole row, 2^-rest, where only ratios count and the logarithm of the sum is corrected by it: an instruction less
+// for each class.  Only where the factor is near 1: `rest` is up to half a step of m / T, and logits of 65504 at a temperature of 2^-7 have
+// m / T log2(e) below 2^24, whose half step is 1/2.  (Unbounded it would be 944 at a maximum of 30000 and the smallest temperature, where the
+// largest class's exponential is then infinite or 0.)
+constexpr float SOFT_RATIO_LEAST = 0x1p-7f;  // the temperature from which on
+struct SoftRatio : SoftExp<half_t> {
+    __device__ inline SoftRatio(float max, const SoftScale &a) : SoftExp<half_t>(max, a) {}
+    __device__ inline float operator()(half_t z) const { return __builtin_amdgcn_exp2f(fmaf((float)z, a.hi, m)); }
+    __device__ inline float log(float sum) const { return fmaf(rest, 0.693147181f, logf(sum)); }
+    __device__ inline float unit(float sum) const { return sum * __builtin_amdgcn_exp2f(-rest); }
 };
 
 // NT threads have a row: a workgroup, or (64) one wave of a workgroup of four, which needs no barriers.
