@@ -9,6 +9,9 @@
 // copy reaches 5.0 on the same card.  1 million fp32 weights in 12 tensors 7.3 us.
 // In 8 bits the roots are held, not the moments: a block's moments span decades (v the squares of m's), and the fourth root brings
 // the 65025^2 that v spans between its smallest code and its largest to 255.
+#include <memory>
+#include <new>
+
 #include "ptl_row_sums.hpp"
 #include "ptl_rows.hpp"
 #include "ptl_tuning.h"
@@ -383,21 +386,6 @@ static int adamw_multi(const Args *list, int count, const adamw_step *s, const c
         k.root2 = (float)sqrt(i2);
     }
     if (s->grad_factor) k.factor = sg.in<float>(s->grad_factor, 1);
-    // More than the 256 MB of the memory's cache: past it, one block a wave (23 million fp32 weights 110 us, 116 with two, 126 with four, and
-    // 119 with one through the caches); less: two, through them (1 million 7.3 us; one 7.9; past them 8.8).
-    const bool large = bytes > 256e6;
-    const int group = 4 * ADAM_BLOCK * (large ? 1 : 2);  // elements of a workgroup
-    unsigned groups = 0;
-    auto flush = [&]() {
-        for (int i = k.count; i < ADAM_TENSORS; ++i) k.first[i] = 0xffffffffu;
-        if (k.count > 0) {
-            if (large) hipLaunchKernelGGL((adamw_kernel<T, 1, true>), dim3(groups), dim3(256), 0, state().stream, k);
-            else hipLaunchKernelGGL((adamw_kernel<T, 2, false>), dim3(groups), dim3(256), 0, state().stream, k);
-        }
-        k.count = 0;
-        groups = 0;
-        return hip_ok(hipGetLastError(), "optimizer launch");
-    };
     AdamMemory known;
     auto map = [&](auto *p, size_t n, bool in, bool out) {
         if (known.has(p, n * sizeof(*p))) return p;
@@ -405,16 +393,25 @@ static int adamw_multi(const Args *list, int count, const adamw_step *s, const c
         if (q && q == p) known.add(p);
         return q;
     };
+    // Every tensor has its place before the first launch: a call that gets no memory for one has changed none.  (What one launch takes lies in its
+    // table from the start: 7.3 us for 12 tensors, 7.7 by way of a list.)
+    std::unique_ptr<AdamTensor[]> more_than_one;
+    if (count > ADAM_TENSORS) {
+        more_than_one.reset(new (std::nothrow) AdamTensor[count]);
+        if (!more_than_one) {
+            set_error("%s: no memory for %d tensors' places", fn, count);
+            return 2;
+        }
+    }
+    AdamTensor *const all = more_than_one ? more_than_one.get() : k.t;
     for (int i = 0; i < count; ++i) {
         const Args &a = list[i];
         const size_t n = (size_t)a.weights->dim, blocks = (n + ADAM_BLOCK - 1) / ADAM_BLOCK;
+        AdamTensor &t = all[i];
+        t = {};
         if (n == 0) continue;
         const adamw_state *from = a.state, *to = a.new_state ? a.new_state : a.state;
         const auto *out = a.updated ? a.updated : a.weights;
-        const size_t more = (n + group - 1) / group;
-        if ((k.count == ADAM_TENSORS || (groups + more) * 256 > (size_t)ROW_THREADS) && !flush()) return sg.finish(2);
-        AdamTensor &t = k.t[k.count];
-        t = {};
         auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
         t.g = map(as(a.weights->diff), n, true, false);
         if (from && from->master) t.master = map(from->master, n, true, false);
@@ -441,10 +438,31 @@ static int adamw_multi(const Args *list, int count, const adamw_step *s, const c
             t.m_out = map(to->m, n, false, true);
             t.v_out = map(to->v, n, false, true);
         }
-        if (sg.failed()) return 2;
         t.n = (unsigned)n;
         t.lr = a.learning_rate;
         t.decay = a.weight_decay;
+    }
+    if (sg.failed()) return 2;
+    // More than the 256 MB of the memory's cache: past it, one block a wave (23 million fp32 weights 110 us, 116 with two, 126 with four, and
+    // 119 with one through the caches); less: two, through them (1 million 7.3 us; one 7.9; past them 8.8).
+    const bool large = bytes > 256e6;
+    const int group = 4 * ADAM_BLOCK * (large ? 1 : 2);  // elements of a workgroup
+    unsigned groups = 0;
+    auto flush = [&]() {
+        for (int i = k.count; i < ADAM_TENSORS; ++i) k.first[i] = 0xffffffffu;
+        if (k.count > 0) {
+            if (large) hipLaunchKernelGGL((adamw_kernel<T, 1, true>), dim3(groups), dim3(256), 0, state().stream, k);
+            else hipLaunchKernelGGL((adamw_kernel<T, 2, false>), dim3(groups), dim3(256), 0, state().stream, k);
+        }
+        k.count = 0;
+        groups = 0;
+        return hip_ok(hipGetLastError(), "optimizer launch");
+    };
+    for (int i = 0; i < count; ++i) {
+        if (all[i].n == 0) continue;
+        const size_t more = ((size_t)all[i].n + group - 1) / group;
+        if ((k.count == ADAM_TENSORS || (groups + more) * 256 > (size_t)ROW_THREADS) && !flush()) return sg.finish(2);
+        k.t[k.count] = all[i];  // (k.count is at most i)
         k.first[k.count] = groups;
         groups += (unsigned)more;
         ++k.count;
