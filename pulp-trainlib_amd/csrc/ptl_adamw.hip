@@ -326,7 +326,9 @@ static const char *adamw_check(const Args &a) {
 }
 
 // Allocations of the device that a call has met: a program's tensors lie in a few, and to ask the runtime for each of a tensor's ten addresses takes
-// longer than the step of a small model (72 tensors: 25 us of asking, 9 of work).
+// longer than the step of a small model (72 tensors: 25 us of asking, 9 of work).  Tensors that lie in more than these are asked for one by one, and
+// each time for their allocation too: a call for 72 tensors with four addresses each takes the host 14 us where they lie in one allocation, 53 in 24
+// in turn, 57 in one each.
 struct AdamMemory {
     struct Range {
         uintptr_t base, end;
