@@ -355,29 +355,25 @@ static bool grad_ready() {
     return ready;
 }
 
+// In tiles of so many inputs, the parts of least cost and what their sums take.
 template <typename T>
-int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in, int rows) {
+static GradParts grad_plan(int wide, bool dw, bool dx, bool low, int ns, int in, int rows) {
     constexpr int XR = GradSizes<T>::XR, KS = GradSizes<T>::KS;
-    // Of 30 layers in fp16 (256 to 8192 tokens, 256 to 8192 inputs and outputs) tiles of 256 inputs take 0.94 times as long from 16 GFLOP on
-    // (0.89 to 1.03) and below 1.01 (0.99 to 1.05): one workgroup a compute unit shares what two would read, but fewer of them fill the chip less evenly.
-    p.wide = sizeof(T) == 2 && 2.0 * ns * in * rows * (dw + dx) >= 16e9 ? 256 : 128;
-    if (!(p.wide == 128 ? grad_ready<T, 128>() : grad_ready<T, sizeof(T) == 2 ? 256 : 128>())) return 2;
+    GradParts p = {wide, {1, 1}, 0};
     const bool wanted[2] = {dx, dw};
     const int n[2] = {ns, rows}, k[2] = {rows, ns};
     int tiles[2], slabs[2];
     double values[2];
     for (int i = 0; i < 2; ++i) {
-        tiles[i] = wanted[i] ? (in + p.wide - 1) / p.wide * ((n[i] + XR - 1) / XR) : 0;
+        tiles[i] = wanted[i] ? (in + wide - 1) / wide * ((n[i] + XR - 1) / XR) : 0;
         slabs[i] = (k[i] + KS - 1) / KS;
         values[i] = (double)n[i] * in;
     }
-    p.parts[0] = p.parts[1] = 1;
-    p.bytes = 0;
     float best = 1e30f;
     for (int u = 1; u <= 32 && (u == 1 || (tiles[0] && u * 4 <= slabs[0])); u *= 2)
         for (int v = 1; v <= 32 && (v == 1 || (tiles[1] && v * 4 <= slabs[1])); v *= 2) {
             const int parts[2] = {u, v};
-            const float c = grad_cost(tiles, slabs, values, parts, sizeof(T) == 4, p.wide);
+            const float c = grad_cost(tiles, slabs, values, parts, sizeof(T) == 4, wide);
             if (c < best) {
                 best = c;
                 p.parts[0] = u;
@@ -390,7 +386,21 @@ int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in
         const size_t parts = low && wanted[i] ? 2 * high : high;
         if (parts > 1) p.bytes += parts * grad_part(n[i], in) * sizeof(float);
     }
-    return 0;
+    return p;
+}
+template <typename T>
+int gated_products_plan(GradParts &p, GradParts &less, bool dw, bool dx, bool low, int ns, int in, int rows) {
+    p = less = grad_plan<T>(128, dw, dx, low, ns, in, rows);
+    if constexpr (sizeof(T) == 2) {
+        // Of 30 layers in fp16 (256 to 8192 tokens, 256 to 8192 inputs and outputs) tiles of 256 inputs take 0.94 times as long from 16 GFLOP on
+        // (0.89 to 1.03) and below 1.01 (0.99 to 1.05): one workgroup a compute unit shares what two would read, but fewer of them fill the chip
+        // less evenly.  Half as many tiles of a layer of few inputs may want their k in more parts, whose sums take more memory (7385 tokens,
+        // 256 -> 3752 gated 129 us and 30 MB, 153 and none).
+        if (2.0 * ns * in * rows * (dw + dx) >= 16e9) p = grad_plan<T>(256, dw, dx, low, ns, in, rows);
+        if (p.bytes <= less.bytes) less = p;
+    }
+    const bool wide = p.wide == 256 || less.wide == 256, narrow = p.wide == 128 || less.wide == 128;
+    return (!narrow || grad_ready<T, 128>()) && (!wide || grad_ready<T, sizeof(T) == 2 ? 256 : 128>()) ? 0 : 2;
 }
 
 template <typename T>
@@ -452,8 +462,8 @@ int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, co
     return hip_ok(hipGetLastError(), "gated layer launch") ? 0 : 2;
 }
 
-template int gated_products_plan<half_t>(GradParts &, bool, bool, bool, int, int, int);
-template int gated_products_plan<float>(GradParts &, bool, bool, bool, int, int, int);
+template int gated_products_plan<half_t>(GradParts &, GradParts &, bool, bool, bool, int, int, int);
+template int gated_products_plan<float>(GradParts &, GradParts &, bool, bool, bool, int, int, int);
 template int gated_products<half_t>(const GradParts &, float *, const half_t *, const half_t *, const half_t *, const half_t *, half_t *, half_t *, int, int, int, int,
                                     int, const float *, half_t *, int);
 template int gated_products<float>(const GradParts &, float *, const float *, const float *, const float *, const float *, float *, float *, int, int, int, int, int,

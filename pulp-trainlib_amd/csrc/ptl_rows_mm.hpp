@@ -103,7 +103,8 @@ struct Gate {
 // Both products behind the gradients of a gated layer's pre-activations (dw or dx NULL: not wanted).  x and w have rows of `cols` values
 // (in and more), dh of `pitch` (rows and more), all of whole 16-byte pieces; what dh has beyond `rows` is 0.  low: what dh lost when it was
 // rounded, GRAD_LOW times, in the same layout (NULL: the products are of dh as it is).  The plan comes first: it says in how many parts k of
-// dx and of dw is taken and what workspace their sums need, `ws`, which a call has in hand before its first launch.  db (NULL: not wanted): the sum of
+// dx and of dw is taken and what workspace their sums need, `ws`, which a call has in hand before its first launch; `less` is one that needs less
+// where there is one, for a call that cannot have so much.  db (NULL: not wanted): the sum of
 // n_shares rows of `shares`, which some workgroups behind the products' form while those end (512 tokens, 1024 -> 1024 dense in fp16 18.7 us, with a
 // launch of its own for them 21.7; 2048 tokens, 2048 -> 5632 112 and 114.6).
 constexpr float GRAD_LOW = 2048.f;
@@ -113,7 +114,7 @@ struct GradParts {
     size_t bytes;
 };
 template <typename T>
-int gated_products_plan(GradParts &p, bool dw, bool dx, bool low, int ns, int in, int rows);
+int gated_products_plan(GradParts &p, GradParts &less, bool dw, bool dx, bool low, int ns, int in, int rows);
 template <typename T>
 int gated_products(const GradParts &parts, float *ws, const T *x, const T *w, const T *dh, const T *low, T *dw, T *dx, int ns, int in, int rows, int cols,
                    int pitch, const float *shares, T *db, int n_shares);
