@@ -10,7 +10,8 @@
  * most 2^30 elements (norms: 2^24), a dense layer at most 2^27 inputs and fewer than 2^30 outputs, its backward call tensors of less than
  * 2^31 elements (samples times elements, and the weights), and a product as many outputs as 2^31 threads form (some 4 * 10^9 and more; 33
  * million outputs of a few tokens); larger ones are rejected.  Tensors a call writes must not overlap those it reads or the other ones
- * it writes except where a comment says so.  A call that gets no memory (status 2) leaves what it reads as it was, also a
+ * it writes except where a comment says so.  Blobs of a call whose dims do not fit together are rejected, those that it does not use are not looked
+ * at.  A call that gets no memory (status 2) leaves what it reads as it was, also a
  * tensor that its results would have replaced; other outputs may be written in part.  Calls share the library's workspace: graphs
  * captured from them are replayed one after the other, as the calls would run.
  */
@@ -72,7 +73,7 @@ int ptl_act_linear_fp16_bw_batched(const struct ActLinear_args_fp16 *a, int nsam
 /* Between two blocks: the norm behind the first, its gate, the residual, and the norm in front of the second.
  *   forward:  u = b / sqrt(mean(b^2) + eps) * coeff_post;  s = skip_scale * x + gate * u;  y = s / sqrt(mean(s^2) + eps) * coeff_pre
  *     input->data b, skip->data x; sum->data receives s, output->data y (coeff_pre NULL: there is no second norm, output is not used).
- *     gate (NULL: 1) holds gates of dim elements one behind the other: sample n has gate n / rows_per_gate; with
+ *     gate (NULL: 1) holds gates of dim elements one behind the other (gate->dim: of one or of all): sample n has gate n / rows_per_gate; with
  *     rows_per_gate = 0 all samples have the first.  y is formed from s before it is rounded.
  *     With eps = 0 a row whose squares are all 0 in fp32 has 0 in the place of its root's inverse.
  *     sum->data and output->data may be input->data or skip->data (not each other).

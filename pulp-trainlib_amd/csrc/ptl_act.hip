@@ -22,6 +22,10 @@ static int act_linear_step(const Args *a, int ns, bool back, const char *fn) {
     const bool bias = a->use_biases == 1, none = a->activation == PTL_ACT_NONE;
     if (bias && !a->bias) return rows_bad(fn, "use_biases=1 with a null bias blob");
     if (back && !none && !a->hidden) return rows_bad(fn, "null argument structure");
+    const bool keeps = back ? !none : blob_data(a->hidden) != nullptr, weights = !back || !a->skip_wg_grad || !a->skip_in_grad;  // (what the call uses)
+    const bool fits = (size_t)in * outs > 0x7fffffffu || a->coeff->dim == in * outs;  // (a blob of more has no dim that says so)
+    if ((weights && !fits) || (bias && !(back && a->skip_wg_grad) && a->bias->dim != outs) || (keeps && a->hidden->dim != outs) || (!back && a->skip && a->skip->dim != outs))
+        return rows_bad(fn, "tensors whose sizes do not fit together");
     if (ns > ROW_MOST) return rows_bad(fn, "more than 2^30 samples");
     if (ns <= 0) return 0;
     auto as = [](auto *p) { return reinterpret_cast<T *>(p); };

@@ -756,14 +756,19 @@ static int norm_join_step(const Args *a, int ns, bool back, const char *fn) {
     if (!(a->eps >= 0.f && a->eps < __builtin_inff())) return rows_bad(fn, "eps is no finite number from 0 on");
     if (!(fabsf(a->skip_scale) < __builtin_inff())) return rows_bad(fn, "skip_scale is no finite number");
     if (a->rows_per_gate < 0) return rows_bad(fn, "rows_per_gate is negative");
+    const bool pre = a->coeff_pre;
+    if (((!back || !a->skip_in_grad) && a->skip->dim != dim) || a->sum->dim != dim || a->coeff_post->dim != dim || (pre && (a->coeff_pre->dim != dim || a->output->dim != dim)))
+        return rows_bad(fn, "tensors whose sizes do not fit together");
     if (ns > ROW_MOST) return rows_bad(fn, "more than 2^30 samples");
     if (ns <= 0) return 0;
     auto as = [](auto *p) { return reinterpret_cast<T *>(p); };
-    const bool pre = a->coeff_pre;
     T *b = as(a->input->data), *w_post = as(a->coeff_post->data), *w_pre = as(blob_data(a->coeff_pre)), *gate = as(blob_data(a->gate));
     if (!b || !w_post || (pre && !w_pre) || (a->gate && !gate)) return rows_bad(fn, "null buffer");
     const int per = a->rows_per_gate && a->rows_per_gate < ns ? a->rows_per_gate : ns;
     const size_t n = (size_t)ns * dim, n_gate = (size_t)((ns + per - 1) / per) * dim;
+    // (a gate's blob has the elements of one, as a sample's has, or of all)
+    if (gate && a->gate->dim != dim && n_gate <= 0x7fffffffu && (a->gate->dim % dim != 0 || a->gate->dim < (int)n_gate))
+        return rows_bad(fn, "tensors whose sizes do not fit together");
     if (!back) {
         if (!a->skip->data || !a->sum->data || (pre && !a->output->data)) return rows_bad(fn, "null buffer");
         if (!ensure_init()) return 2;
