@@ -199,7 +199,8 @@ struct adamw_args_fp16 {
     float weight_decay;
 };
 /* What the tensors share: beta1 and beta2 in 0 .. 1 (below 1), eps from 1e-30 on.  step is t, from 1 on; step_data (may be NULL: step) a place
- * that holds it when the step runs, so that a captured graph can be replayed with another.  grad_factor (may be NULL: 1) holds a factor
+ * that holds it when the step runs, so that a captured graph can be replayed with another (learning_rate and weight_decay are what they were at the
+ * call: a graph keeps them).  grad_factor (may be NULL: 1) holds a factor
  * of the gradients (the inverse of a loss scale, a clipped norm's); where it is no finite number the step changes nothing that is updated in
  * place, and elsewhere copies what it would have updated (zeros for moments that are 0). */
 struct adamw_step {

@@ -73,7 +73,9 @@ struct Gate {
     }
     // The same of one activation (of each a code of its own, without the selects: 2048 x 5632 gradients through gelu in fp16, bound by the
     // vector units, take 26 us with those and 20 so): slope = e / (1 + e)^2 with e = exp(-|p|) is the same on both sides of 0, and 0 where d p / d x, which is taken
-    // of a bounded x, could grow beyond all bounds.  EXACT: the exponent to 2^-24 of itself, otherwise to 2^-22.
+    // of a bounded x, could grow beyond all bounds.  EXACT: the exponent to 2^-24 of itself, otherwise to 2^-22 - for
+    // fp16, whose slopes come from pre-activations of 11 bits and go into gradients of 11: an exponent of 16, where the slope is 1e-7, is then 4e-6 off, of a
+    // rounding's 5e-4.
     template <int ACT, bool EXACT>
     __device__ static inline float slope(float x) {
         if constexpr (ACT == GATE_RELU) return x > 0.f ? 1.f : x != x ? x : 0.f;

@@ -56,7 +56,8 @@ struct SoftExp {
 };
 
 // ... of fp16 but for a factor of the whole row, 2^-rest, where only ratios count and the logarithm of the sum is corrected by it: an instruction less
-// for each class.  Only where the factor is near 1: `rest` is up to half a step of m / T, and logits of 65504 at a temperature of 2^-7 have
+// for each class (the policy loss of 2048 rows of 32000 classes 48.2 us and 48.6 with whole exponentials, 4096 of 8200 29.3 and 31.9, 300 of 32000 11.6 and
+// 12.3, 8192 of 1000 and 4 of 131072 the same).  Only where the factor is near 1: `rest` is up to half a step of m / T, and logits of 65504 at a temperature of 2^-7 have
 // m / T log2(e) below 2^24, whose half step is 1/2.  (Unbounded it would be 944 at a maximum of 30000 and the smallest temperature, where the
 // largest class's exponential is then infinite or 0.)
 constexpr float SOFT_RATIO_LEAST = 0x1p-7f;  // the temperature from which on
